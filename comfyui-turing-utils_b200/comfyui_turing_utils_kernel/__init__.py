@@ -15,11 +15,18 @@ from .ops import (
     turing_bf16_int8_convrot_quantize,
     turing_bf16_int8_convrot_quantize_b128,
     turing_codebook_w4a8_linear,
+    turing_convrot_fp4_linear,
     turing_convrot_int8_linear,
     turing_dequantize_int8_bf16,
+    turing_fp4_block_scale_tiles,
+    turing_fp4_dequantize,
+    turing_fp4_linear,
+    turing_fp4_linear_grad_input,
+    turing_fp4_quantize,
     turing_gelu_int4_convrot_quantize,
     turing_gelu_int8_convrot_quantize,
     turing_int8_linear,
+    turing_layer_norm,
     turing_layer_norm_adaln,
     turing_segmented_rms_adaln,
     turing_swiglu_int4_convrot_quantize,
@@ -42,11 +49,18 @@ __all__ = [
     "turing_bf16_int8_convrot_quantize",
     "turing_bf16_int8_convrot_quantize_b128",
     "turing_codebook_w4a8_linear",
+    "turing_convrot_fp4_linear",
     "turing_convrot_int8_linear",
     "turing_dequantize_int8_bf16",
+    "turing_fp4_block_scale_tiles",
+    "turing_fp4_dequantize",
+    "turing_fp4_linear",
+    "turing_fp4_linear_grad_input",
+    "turing_fp4_quantize",
     "turing_gelu_int4_convrot_quantize",
     "turing_gelu_int8_convrot_quantize",
     "turing_int8_linear",
+    "turing_layer_norm",
     "turing_layer_norm_adaln",
     "turing_segmented_rms_adaln",
     "turing_swiglu_int4_convrot_quantize",

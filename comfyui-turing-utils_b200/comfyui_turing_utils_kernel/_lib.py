@@ -52,6 +52,15 @@ SIGNATURES = {
                                        _vp]),
     "ctu_layer_norm_adaln": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i32, _vp]),
     "ctu_debug_gemm_injected_timeout": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _u64, _vp]),
+    "ctu_layer_norm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _i32, _i32, _vp]),
+    "ctu_layer_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "ctu_layer_norm_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
+    "ctu_fp4_block_scale_bytes": (_i64, [_i64, _i64, _i32]),
+    "ctu_fp4_quantize": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "ctu_fp4_dequantize": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp]),
+    "ctu_fp4_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "ctu_fp4_grad_workspace_bytes": (_i64, [_i64, _i64]),
+    "ctu_fp4_linear_grad_input": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "ctu_debug_set_gemm_kernel": (_i32, [_i32]),
     "ctu_debug_set_fused_linear": (_i32, [_i32]),
     "ctu_debug_set_gemm_split": (_i32, [_i32]),

@@ -466,3 +466,205 @@ def turing_w4a4_g128_linear(
 @turing_w4a4_g128_linear.register_fake
 def _turing_w4a4_g128_linear_fake(activation, weight, activation_scale, weight_scale, bias=None):
     return torch.empty((activation.size(0), weight.size(0)), dtype=torch.bfloat16, device=activation.device)
+
+
+# 4-bit floating point linear and affine layer norm (no reference ops; arithmetic and layouts in
+# ctu_b200.h).  A single token's call is bound by host time, so these are defined on a
+# torch.library.Library, whose call costs a third of a torch.library.custom_op's (8 us against 22 us
+# for an empty op of five arguments); schema, fake kernels and autograd are the same.
+_LIBRARY = torch.library.Library("turing_utils", "FRAGMENT")
+
+
+def _define(name: str, schema: str, impl) -> None:
+    _LIBRARY.define(name + schema)
+    _LIBRARY.impl(name, impl, "CompositeExplicitAutograd")
+
+
+def _fp4_block(block_scale: torch.Tensor) -> int:
+    return 16 if block_scale.dtype == torch.float8_e4m3fn else 32
+
+
+_define("fp4_quantize", "(Tensor x, str format='nvfp4', int rotation=0) -> (Tensor, Tensor, Tensor)", _C.fp4_quantize)
+
+
+@torch.library.register_fake("turing_utils::fp4_quantize")
+def _fp4_quantize_fake(x, format="nvfp4", rotation=0):
+    _, block, dtype = _C._FP4_FORMATS[format]
+    rows, k = x.shape
+    return (x.new_empty((rows, k // 2), dtype=torch.uint8), x.new_empty(_C._fp4_tiles(rows, k, block), dtype=dtype),
+            x.new_empty((rows, 1), dtype=torch.float32))
+
+
+def turing_fp4_quantize(x: torch.Tensor, format: str = "nvfp4", rotation: int = 0):
+    """bf16/fp16 rows to 4-bit floating point: (packed codes, block scale tiles, row scales).
+
+    ``format`` is ``"nvfp4"`` (e4m3 scale per 16 values, power-of-two row scale) or ``"mxfp4"`` (e8m0
+    scale per 32 values); ``rotation=256`` applies the ConvRot rotation first."""
+    return torch.ops.turing_utils.fp4_quantize.default(x, format, rotation)
+
+
+_define("fp4_dequantize", "(Tensor codes, Tensor block_scale, Tensor scale, ScalarType out_dtype=bfloat16) -> Tensor",
+        _C.fp4_dequantize)
+
+
+@torch.library.register_fake("turing_utils::fp4_dequantize")
+def _fp4_dequantize_fake(codes, block_scale, scale, out_dtype=torch.bfloat16):
+    return codes.new_empty((codes.size(0), codes.size(1) * 2), dtype=out_dtype)
+
+
+def turing_fp4_dequantize(codes: torch.Tensor, block_scale: torch.Tensor, scale: torch.Tensor,
+                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that FP4 codes and scales stand for (rotated values stay rotated)."""
+    return torch.ops.turing_utils.fp4_dequantize.default(codes, block_scale, scale, out_dtype)
+
+
+_define("fp4_linear", "(Tensor activation, Tensor weight, Tensor activation_block_scale, Tensor weight_block_scale, "
+        "Tensor activation_scale, Tensor weight_scale, Tensor? bias=None) -> Tensor", _C.fp4_linear)
+
+
+@torch.library.register_fake("turing_utils::fp4_linear")
+def _fp4_linear_fake(activation, weight, activation_block_scale, weight_block_scale, activation_scale, weight_scale,
+                     bias=None):
+    return activation.new_empty((activation.size(0), weight.size(0)), dtype=torch.bfloat16)
+
+
+def turing_fp4_linear(activation: torch.Tensor, weight: torch.Tensor, activation_block_scale: torch.Tensor,
+                      weight_block_scale: torch.Tensor, activation_scale: torch.Tensor, weight_scale: torch.Tensor,
+                      bias: torch.Tensor | None = None) -> torch.Tensor:
+    """W4A4 product of two FP4 operands of one format (tcgen05 block-scaled MMA), bf16 [m, n]."""
+    return torch.ops.turing_utils.fp4_linear.default(activation, weight, activation_block_scale, weight_block_scale,
+                                                     activation_scale, weight_scale, bias)
+
+
+_define("fp4_linear_grad_input", "(Tensor grad_output, Tensor weight, Tensor weight_block_scale, Tensor weight_scale, "
+        "int rotation=0) -> Tensor", _C.fp4_linear_grad_input)
+
+
+@torch.library.register_fake("turing_utils::fp4_linear_grad_input")
+def _fp4_linear_grad_input_fake(grad_output, weight, weight_block_scale, weight_scale, rotation=0):
+    return grad_output.new_empty((grad_output.size(0), weight.size(1) * 2))
+
+
+def turing_fp4_linear_grad_input(grad_output: torch.Tensor, weight: torch.Tensor, weight_block_scale: torch.Tensor,
+                                 weight_scale: torch.Tensor, rotation: int = 0) -> torch.Tensor:
+    """Gradient with respect to the input of a linear with frozen FP4 weights: bf16 [m, k]."""
+    return torch.ops.turing_utils.fp4_linear_grad_input.default(grad_output, weight, weight_block_scale, weight_scale,
+                                                                rotation)
+
+
+def _no_second_derivative(what: str) -> None:
+    if torch.is_grad_enabled():  # create_graph=True
+        raise RuntimeError(f"{what} has no second derivative")
+
+
+def _convrot_fp4_linear(x, weight, weight_block_scale, weight_scale, bias=None, rotation=256):
+    fmt = "nvfp4" if weight_block_scale.dtype == torch.float8_e4m3fn else "mxfp4"
+    codes, block_scale, scale = _C.fp4_quantize(x, fmt, rotation)
+    return _C.fp4_linear(codes, weight, block_scale, weight_block_scale, scale, weight_scale, bias)
+
+
+_define("convrot_fp4_linear", "(Tensor x, Tensor weight, Tensor weight_block_scale, Tensor weight_scale, "
+        "Tensor? bias=None, int rotation=256) -> Tensor", _convrot_fp4_linear)
+
+
+@torch.library.register_fake("turing_utils::convrot_fp4_linear")
+def _convrot_fp4_linear_fake(x, weight, weight_block_scale, weight_scale, bias=None, rotation=256):
+    return x.new_empty((x.size(0), weight.size(0)), dtype=torch.bfloat16)
+
+
+def _convrot_fp4_linear_setup(ctx, inputs, output):
+    x, weight, weight_block_scale, weight_scale, bias, rotation = inputs
+    if ctx.needs_input_grad[3] or ctx.needs_input_grad[4]:
+        raise RuntimeError("the FP4 linear's weight scale and bias are frozen: detach them")
+    if x.dtype != torch.bfloat16 or weight.size(0) % 8:
+        raise RuntimeError("the FP4 linear's gradient takes bfloat16 input and N divisible by 8")
+    ctx.save_for_backward(weight, weight_block_scale, weight_scale)
+    ctx.rotation = rotation
+
+
+def _convrot_fp4_linear_backward(ctx, grad):
+    _no_second_derivative("the FP4 linear")
+    dx = torch.ops.turing_utils.fp4_linear_grad_input.default(grad, *ctx.saved_tensors, ctx.rotation)
+    return dx, None, None, None, None, None
+
+
+torch.library.register_autograd("turing_utils::convrot_fp4_linear", _convrot_fp4_linear_backward,
+                                setup_context=_convrot_fp4_linear_setup)
+
+
+def turing_convrot_fp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_block_scale: torch.Tensor,
+                              weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                              rotation: int = 256) -> torch.Tensor:
+    """Linear of bf16/fp16 rows with FP4 weights: the rows are rotated and quantized to the weights'
+    format, then multiplied.  Differentiable in ``x`` (bf16): the quantization passes the gradient
+    straight through, the weights are frozen."""
+    return torch.ops.turing_utils.convrot_fp4_linear.default(x, weight, weight_block_scale, weight_scale, bias, rotation)
+
+
+_define("layer_norm", "(Tensor x, Tensor? weight=None, Tensor? bias=None, float epsilon=1e-5) -> "
+        "(Tensor, Tensor, Tensor)", _C.layer_norm)
+
+
+@torch.library.register_fake("turing_utils::layer_norm")
+def _layer_norm_fake(x, weight=None, bias=None, epsilon=1.0e-5):
+    rows = x.numel() // x.size(-1)
+    return torch.empty_like(x, memory_format=torch.contiguous_format), *(x.new_empty(rows, dtype=torch.float32) for _ in "mr")
+
+
+def _layer_norm_backward(grad, x, mean, rstd, weight=None, bias=None, needs=7):
+    grads = _C.layer_norm_backward(grad, x, mean, rstd, weight, bias, [bool(needs & b) for b in (1, 2, 4)])
+    return tuple(x.new_empty(0) if g is None else g for g in grads)
+
+
+_define("layer_norm_backward", "(Tensor grad, Tensor x, Tensor mean, Tensor rstd, Tensor? weight=None, "
+        "Tensor? bias=None, int needs=7) -> (Tensor, Tensor, Tensor)", _layer_norm_backward)
+
+
+@torch.library.register_fake("turing_utils::layer_norm_backward")
+def _layer_norm_backward_fake(grad, x, mean, rstd, weight=None, bias=None, needs=7):
+    none = x.new_empty(0)
+    return (torch.empty_like(x, memory_format=torch.contiguous_format) if needs & 1 else none,
+            torch.empty_like(weight) if needs & 2 and weight is not None else none,
+            torch.empty_like(bias) if needs & 4 and bias is not None else none)
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    ctx.save_for_backward(x, output[1], output[2], weight, bias)
+    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _layer_norm_autograd(ctx, grad, *_):
+    if grad is None:
+        return None, None, None, None
+    _no_second_derivative("LayerNorm")
+    x, mean, rstd, weight, bias = ctx.saved_tensors
+    wanted = ctx.needs_input_grad
+    needs = sum(bit for bit, want in zip((1, 2, 4), wanted) if want)
+    grads = torch.ops.turing_utils.layer_norm_backward.default(grad, x, mean, rstd, weight, bias, needs)
+    return (*(g if want else None for g, want in zip(grads, wanted)), None)
+
+
+torch.library.register_autograd("turing_utils::layer_norm", _layer_norm_autograd, setup_context=_layer_norm_setup)
+
+
+def turing_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                      epsilon: float = 1.0e-5) -> torch.Tensor:
+    """Affine layer norm over the last dimension, differentiable in x, weight and bias.
+
+    x is bf16, fp16 or fp32; weight and bias have its type or are fp32."""
+    return torch.ops.turing_utils.layer_norm.default(x, weight, bias, epsilon)[0]
+
+
+def turing_fp4_block_scale_tiles(block_scale: torch.Tensor) -> torch.Tensor:
+    """Plain block scales [rows, k / block] (float8_e4m3fn or float8_e8m0fnu), as checkpoints store them,
+    in the tiles that the FP4 ops read: once, when a layer is loaded."""
+    if block_scale.dim() != 2 or block_scale.dtype not in _C._FP4_BY_SCALE:
+        raise RuntimeError("block scales must be 2D float8_e4m3fn or float8_e8m0fnu")
+    rows, blocks = block_scale.shape
+    mt, kt = (rows + 127) // 128, (blocks + 3) // 4
+    full = torch.zeros((mt * 128, kt * 4), dtype=torch.uint8, device=block_scale.device)
+    full[:rows, :blocks] = block_scale.view(torch.uint8)
+    tiles = full.view(mt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).reshape(mt, kt, 32, 16)
+    return tiles.contiguous().view(block_scale.dtype)

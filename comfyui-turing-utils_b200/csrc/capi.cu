@@ -106,6 +106,16 @@ int device_info(DeviceInfo *info) {
     return CTU_OK;
 }
 
+int kernel_device(DeviceQuery *q, uint32_t **err) {
+    DeviceInfo info;
+    if (int rc = device_info(&info)) return rc;
+    q->device = info.device;
+    q->num_sms = info.num_sms;
+    q->smem_optin = info.smem_optin;
+    *err = info.err;
+    return CTU_OK;
+}
+
 // ---------------------------------------------------------------------------- tensor maps
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -123,6 +133,24 @@ int get_encoder(EncodeTiledFn *out) {
     });
     if (fn == nullptr) return fail(CTU_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
     *out = fn;
+    return CTU_OK;
+}
+
+int encode_tiled(CUtensorMap *map, CUtensorMapDataType type, int rank, const void *base, const uint64_t *dims,
+                 const uint64_t *strides, const uint32_t *box, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn enc;
+    if (int rc = get_encoder(&enc)) return rc;
+    cuuint64_t d[3] = {}, st[2] = {};
+    cuuint32_t b[3] = {}, es[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i > 0) st[i - 1] = strides[i - 1];
+    }
+    const CUresult r = enc(map, type, static_cast<cuuint32_t>(rank), const_cast<void *>(base), d, st, b, es,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(CTU_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
     return CTU_OK;
 }
 

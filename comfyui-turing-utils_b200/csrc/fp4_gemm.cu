@@ -1,0 +1,283 @@
+// Product of two 4-bit floating point matrices (CTA pair, tcgen05 block-scaled MMA):
+//
+//   out[m, n] = bf16( fma( (sum_k A[m, k] B[n, k]) * a_scale[m], w_scale[n], bias[n] ) )
+//
+// A and B are e2m1 codes times their block scales; the tensor cores apply both and accumulate in
+// fp32.  A pair of CTAs owns a 256 x 192 tile: CTA r stages rows [128 r, 128 r + 128) of A and 96
+// rows of B, the scales of its own A rows and those of all 192 B rows; one M = 256, N = 192, K = 64
+// instruction of the leader reads both CTAs' halves.  192 columns, not 256, so that two accumulators
+// (2 x 192 columns of tensor memory) and two sets of scales (2 x 48) fit its 512 columns, and the
+// epilogue of one tile runs under the next one's MMAs.
+//
+// Roles: warp 0 loads (TMA), warp 1 of the leader copies scales into tensor memory and issues the
+// MMAs, warps 2..5 write the output.  Every wait is bounded.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "fp4.cuh"
+#include "fp4_mma.cuh"
+#include "ptx.cuh"
+
+namespace ctu {
+namespace fp4 {
+
+namespace {
+
+constexpr int kStages = 6;
+constexpr int kStageK = 256;  // values of K per stage: 128 bytes of codes
+constexpr int kChunks = 4;    // MMAs per stage
+constexpr int kABytes = 128 * 128;
+constexpr int kHalfCols = kPairCols / 2;
+constexpr int kBBytes = kHalfCols * 128;
+constexpr int kAScaleBytes = 4 * 512;
+constexpr int kBScaleBytes = 2 * 4 * 512;
+constexpr int kAOffset = 0;
+constexpr int kBOffset = kStages * kABytes;
+constexpr int kAScaleOffset = kBOffset + kStages * kBBytes;
+constexpr int kBScaleOffset = kAScaleOffset + kStages * kAScaleBytes;
+constexpr int kStructOffset = kBScaleOffset + kStages * kBScaleBytes;
+constexpr int kEpilogueWarps = 4;
+constexpr int kThreadCount = 32 * (2 + kEpilogueWarps);
+constexpr int kTmemCols = 512;
+constexpr int kScaleCol = 2 * kPairCols;  // first column of the scales
+constexpr int kScaleSet = 48;             // 4 chunks x (4 of A + 8 of B)
+
+struct Shared {
+    uint64_t full[kStages];
+    uint64_t empty[kStages];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort_flag;
+    float col_scale[kPairCols];
+    float col_bias[kPairCols];
+};
+
+constexpr int kSmem = kStructOffset + static_cast<int>(sizeof(Shared)) + 1024;
+static_assert(kSmem <= 232448, "shared memory of one CTA");
+
+}  // namespace
+
+template <int kFormat>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
+    fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                           const __grid_constant__ CUtensorMap tmap_as, const __grid_constant__ CUtensorMap tmap_bs,
+                           const LinearArgs args) {
+    // Scale tiles of 128 rows per stage: 64 values of K per tile (nvfp4) or 128 (mxfp4).
+    constexpr int kTiles = kFormat == kNvfp4 ? 4 : 2;
+    constexpr uint32_t kStageTx = 2 * (kABytes + kBBytes + 3 * kTiles * 512);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Shared &S = *reinterpret_cast<Shared *>(smem + kStructOffset);
+
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int pair = blockIdx.x >> 1;
+    const int num_pairs = gridDim.x >> 1;
+    const int num_n = (args.n + kPairCols - 1) / kPairCols;
+    const int num_m = (args.m + kPairRows - 1) / kPairRows;
+    const int num_tiles = num_m * num_n;
+    const int nk = (args.k + kStageK - 1) / kStageK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&S.full[s], 1);
+            mbar_init(&S.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&S.acc_full[b], 1);
+            mbar_init(&S.acc_empty[b], 2 * kEpilogueWarps);
+        }
+        mbar_init(&S.drain, 1);
+        S.abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(&S.tmem_base, kTmemCols);
+        tmem_relinquish_pair();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&tmap_a);
+        prefetch_tmap(&tmap_b);
+        prefetch_tmap(&tmap_as);
+        prefetch_tmap(&tmap_bs);
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = S.tmem_base;
+    const PairAbort guard{&S.abort_flag, mapa_shared(smem_u32(&S.abort_flag), rank ^ 1u), args.err};
+    volatile int *abort_flag = &S.abort_flag;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+                const int m0 = (t / num_n) * kPairRows + static_cast<int>(rank) * 128;
+                const int n0 = (t % num_n) * kPairCols;
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!guard.wait(&S.empty[s], ph ^ 1u, kErrTimeoutEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t full = mapa_shared(smem_u32(&S.full[s]), 0u);
+                    if (leader) mbar_arrive_expect_tx(&S.full[s], kStageTx);
+                    tma_load_2d_pair(smem + kAOffset + s * kABytes, &tmap_a, kb * 128, m0, full);
+                    tma_load_2d_pair(smem + kBOffset + s * kBBytes, &tmap_b, kb * 128,
+                                     n0 + static_cast<int>(rank) * kHalfCols, full);
+                    tma_load_3d_pair(smem + kAScaleOffset + s * kAScaleBytes, &tmap_as, 0, kb * kTiles, m0 / 128, full);
+                    tma_load_3d_pair(smem + kBScaleOffset + s * kBScaleBytes, &tmap_bs, 0, kb * kTiles, n0 / 128, full);
+                    if (++s == kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            if (!ok || *abort_flag) settle_inflight_copies();
+        }
+    } else if (warp == 1) {
+        if (leader && lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            int local = 0;
+            bool ok = true;
+            uint32_t set = 0;
+            for (int t = pair; t < num_tiles && ok; t += num_pairs, ++local) {
+                const int ab = local & 1;
+                if (!guard.wait_cluster(&S.acc_empty[ab], ((local >> 1) & 1) ^ 1u, kErrTimeoutAccumFree)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(ab * kPairCols);
+                // The tile's first column may lie 64 rows into its first scale tile: two columns.
+                const uint32_t b_shift = static_cast<uint32_t>(((t % num_n) * kPairCols % 128) / 32);
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!guard.wait(&S.full[s], ph, kErrTimeoutFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    // Scale sets alternate, so copies for one stage do not wait for the MMAs of the
+                    // stage before; copies and MMAs of one thread execute in order.
+                    const uint32_t sa = tmem_base + kScaleCol + set * kScaleSet;
+                    const uint32_t sb = sa + 16;
+                    const uint32_t as = smem_u32(smem + kAScaleOffset + s * kAScaleBytes);
+                    const uint32_t bs = smem_u32(smem + kBScaleOffset + s * kBScaleBytes);
+#pragma unroll
+                    for (int c = 0; c < kTiles; ++c) {
+                        copy_scales_pair(sa + 4 * c, smem_desc_scales(as + c * 512));
+                        copy_scales_pair(sb + 8 * c, smem_desc_scales(bs + c * 512));
+                        copy_scales_pair(sb + 8 * c + 4, smem_desc_scales(bs + (kTiles + c) * 512));
+                    }
+                    const uint32_t a = smem_u32(smem + kAOffset + s * kABytes);
+                    const uint32_t b = smem_u32(smem + kBOffset + s * kBBytes);
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) {
+                        const int tile = kFormat == kNvfp4 ? c : c / 2;
+                        const uint32_t idesc = kFormat == kNvfp4 ? idesc_fp4(kFormat, kPairRows, kPairCols, 0)
+                                                                 : idesc_fp4(kFormat, kPairRows, kPairCols, 2 * (c & 1));
+                        mma_fp4_pair<kFormat>(d, smem_desc_sw128(a + 32 * c), smem_desc_sw128(b + 32 * c), idesc,
+                                              sa + 4 * tile, sb + 8 * tile + b_shift, (kb | c) != 0 ? 1u : 0u);
+                    }
+                    set ^= 1u;
+                    mma_commit_pair_both(&S.empty[s]);
+                    if (++s == kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                mma_commit_pair_both(&S.acc_full[ab]);
+            }
+            mma_commit_pair_local(&S.drain);
+            mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+        }
+    } else {
+        const int quad = warp & 3;
+        const int ethread = threadIdx.x - 64;
+        const uint32_t leader_empty = mapa_shared(smem_u32(&S.acc_empty[0]), 0u);
+        const bool vector = (args.n & 7) == 0;
+        bool alive = true;
+        int local = 0;
+        for (int t = pair; t < num_tiles; t += num_pairs, ++local) {
+            const int ab = local & 1;
+            const int m0 = (t / num_n) * kPairRows + static_cast<int>(rank) * 128;
+            const int n0 = (t % num_n) * kPairCols;
+            named_barrier(1, 32 * kEpilogueWarps);
+            for (int c = ethread; c < kPairCols; c += 32 * kEpilogueWarps) {
+                const int n = n0 + c;
+                const bool in = n < args.n;
+                S.col_scale[c] = in ? args.w_scale[args.w_scale_count == 1 ? 0 : n] : 0.0f;
+                S.col_bias[c] = in && args.bias != nullptr ? args.bias[n] : 0.0f;
+            }
+            named_barrier(1, 32 * kEpilogueWarps);
+            if (alive) {
+                int ok = 1;
+                if (lane == 0) ok = guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum) ? 1 : 0;
+                alive = __shfl_sync(0xffffffffu, ok, 0) != 0;
+            }
+            if (!alive) continue;
+            tc_fence_after();
+            const int m = m0 + quad * 32 + lane;
+            const bool row_ok = m < args.m;
+            const float a_s = row_ok ? args.a_scale[m] : 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < kPairCols / 32; ++c) {
+                uint32_t acc[32];
+                tmem_ld_32x32b_x32(tmem_base + static_cast<uint32_t>(ab * kPairCols + c * 32) +
+                                       (static_cast<uint32_t>(quad * 32) << 16),
+                                   acc);
+                tmem_ld_wait();
+                const int valid = args.n - (n0 + c * 32);
+                if (!row_ok || valid <= 0) continue;
+                __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(args.out) + static_cast<int64_t>(m) * args.n + n0 + c * 32;
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    v[j] = __fmaf_rn(__fmul_rn(__uint_as_float(acc[j]), a_s), S.col_scale[c * 32 + j],
+                                     S.col_bias[c * 32 + j]);
+                if (vector) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (8 * q < valid)
+                            reinterpret_cast<uint4 *>(dst)[q] =
+                                make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                                           pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j < valid) dst[j] = __float2bfloat16_rn(v[j]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(leader_empty + static_cast<uint32_t>(ab * sizeof(uint64_t)));
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+int linear_pair_smem() { return kSmem; }
+int linear_pair_threads() { return kThreadCount; }
+const void *linear_pair_kernel(int format) {
+    return format == kNvfp4 ? reinterpret_cast<const void *>(&fp4_linear_pair_kernel<kNvfp4>)
+                            : reinterpret_cast<const void *>(&fp4_linear_pair_kernel<kMxfp4>);
+}
+
+}  // namespace fp4
+}  // namespace ctu

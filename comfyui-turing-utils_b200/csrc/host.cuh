@@ -1,6 +1,7 @@
 // Host-side helpers shared by the C ABI translation units (not exported).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -22,6 +23,14 @@ bool aligned16(const void *p);
 // Current device's SM count and shared-memory limit; rejects anything but sm_100.
 // Performs no allocation.
 int device_query(DeviceQuery *q);
+
+// The same from the per-device table, with the device's error word (its first use on a device
+// allocates that word).
+int kernel_device(DeviceQuery *q, uint32_t **err);
+
+// Tensor map of `rank` dimensions (strides in bytes, outer dimensions only), out-of-range reads zero.
+int encode_tiled(CUtensorMap *map, CUtensorMapDataType type, int rank, const void *base, const uint64_t *dims,
+                 const uint64_t *strides, const uint32_t *box, CUtensorMapSwizzle swizzle);
 
 // Validated launches of the two kernels with an explicit error word.  Neither
 // allocates device memory.

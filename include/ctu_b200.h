@@ -304,6 +304,73 @@ CTU_API int ctu_layer_norm_adaln(const void *x, const void *scale, const void *s
                                  int dtype, void *stream);
 
 /*
+ * Affine layer norm (no reference op; the affine norm in front of a block's cross-attention):
+ * out = (x - mean) * rstd * weight + bias over rows of `hidden` values, rstd = 1 / sqrt(var + epsilon).
+ * weight and bias are [hidden] of weight_dtype (dtype or CTU_DTYPE_FP32), either may be NULL (1, 0).
+ * mean and rstd are fp32 [rows], kept for the backward pass.  Statistics and sums are fp32.
+ */
+CTU_API int ctu_layer_norm(const void *x, const void *weight, const void *bias, void *out, float *mean, float *rstd,
+                           int64_t rows, int64_t hidden, float epsilon, int dtype, int weight_dtype, void *stream);
+
+/*
+ * Its backward pass: dx [rows, hidden] (dtype), dweight and dbias [hidden] (weight_dtype); any of the
+ * three may be NULL.  workspace holds the partial sums of dweight and dbias
+ * (ctu_layer_norm_backward_workspace_bytes); it is not needed for dx alone.  The order of every sum is
+ * fixed by the shapes, so equal inputs give equal bits.
+ */
+CTU_API int64_t ctu_layer_norm_backward_workspace_bytes(int64_t rows, int64_t hidden);
+CTU_API int ctu_layer_norm_backward(const void *grad, const void *x, const void *weight, const float *mean,
+                                    const float *rstd, void *dx, void *dweight, void *dbias, void *workspace,
+                                    int64_t rows, int64_t hidden, int dtype, int weight_dtype, void *stream);
+
+/*
+ * 4-bit floating point (no reference op).  A matrix [rows, k] is held as e2m1 codes [rows, k / 2] (the
+ * even column in the low nibble), one scale per block of a row and one fp32 scale per row; the value is
+ * the product of the three.  CTU_FP4_NVFP4: blocks of 16, e4m3 block scales, a power-of-two row scale.
+ * CTU_FP4_MXFP4: blocks of 32, e8m0 block scales, row scale 1.  Block scales lie in tiles of 128 rows by
+ * four blocks, 512 bytes each, [ceil(rows / 128)][ceil(k / block / 4)]: row 32 j + l, block b of a tile
+ * at byte 16 l + 4 j + b; bytes beyond the matrix must be zero.  k is a multiple of 32.
+ *
+ * The quantizer takes bf16 or fp16 rows, rotation 0 or 256 (the ConvRot rotation in fp32, k % 256 = 0).
+ * Row scale: 2^ceil(log2(amax / 2688)), at least 2^-126, 1 for a zero row; block scale: e4m3(block amax /
+ * row scale / 6), or 2^(floor(log2(block amax)) - 2) at least 2^-127; codes to nearest, ties to even,
+ * saturating at 6.  A row that holds a NaN or an infinity (after the rotation) gets a NaN row scale, zero
+ * codes and zero block scales.
+ */
+#define CTU_FP4_NVFP4 0
+#define CTU_FP4_MXFP4 1
+#define CTU_FP4_MAX_QUANTIZE_K 49152
+CTU_API int64_t ctu_fp4_block_scale_bytes(int64_t rows, int64_t k, int format);
+CTU_API int ctu_fp4_quantize(const void *x, int64_t rows, int64_t k, int dtype, int format, int rotation,
+                             uint8_t *codes, uint8_t *block_scales, float *row_scales, void *stream);
+
+/* The values back, rounded once to dtype (CTU_DTYPE_*).  row_scales: one, or one per row. */
+CTU_API int ctu_fp4_dequantize(const uint8_t *codes, const uint8_t *block_scales, const float *row_scales,
+                               int64_t row_scale_count, int64_t rows, int64_t k, int format, int dtype, void *out,
+                               void *stream);
+
+/*
+ * out[m, n] = bf16(fma(acc * a_scale[m], w_scale[n], bias[n])), acc = sum over k of both operands' codes
+ * times block scales, accumulated in fp32 by the tensor cores.  a_scale is [m]; w_scale is [n] or scalar
+ * (w_scale_count = 1); bias is fp32 [n] or NULL; any m and n.
+ */
+CTU_API int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_scales,
+                           const uint8_t *w_block_scales, const float *a_scale, const float *w_scale,
+                           int64_t w_scale_count, const float *bias, void *out, int64_t m, int64_t n, int64_t k,
+                           int format, void *stream);
+
+/*
+ * dx[m, k] = grad[m, n] w[n, k], rotated back when rotation is 256 (the rotation is its own inverse);
+ * grad and dx bf16, n a multiple of 8.  The weights are decoded to bf16 in the workspace
+ * (ctu_fp4_grad_workspace_bytes), which is exact for power-of-two channel scales and rounds once for
+ * others; sums and the rotation are fp32.
+ */
+CTU_API int64_t ctu_fp4_grad_workspace_bytes(int64_t n, int64_t k);
+CTU_API int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t *w_block_scales,
+                                      const float *w_scale, int64_t w_scale_count, int rotation, void *workspace,
+                                      void *dx, int64_t m, int64_t n, int64_t k, int format, void *stream);
+
+/*
  * int32 accumulator -> bf16: out[r, c] = bf16((float(acc[r, c]) * a_scale[r]) * w_scale[c]),
  * acc row stride acc_stride (>= cols), w_scale [cols] or scalar (w_scale_count = 1),
  * out bf16 [rows, cols] contiguous.

@@ -1,0 +1,374 @@
+"""4-bit floating point quantizer, dequantizer, linear and its input gradient against 64-bit definitions."""
+
+import numpy as np
+import pytest
+import torch
+
+import fp4_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ("nvfp4", "mxfp4")
+HALF_BF16 = 2.0**-8  # a bf16 rounding, relative
+
+
+@pytest.fixture(scope="module")
+def k():
+    import comfyui_turing_utils_kernel as kernel
+
+    yield kernel
+    from comfyui_turing_utils_kernel import _lib
+
+    assert _lib.device_error(torch.cuda.current_device()) == 0
+
+
+def rows_like(rows, width, seed, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, width, generator=g) * torch.exp(torch.randn(rows, 1, generator=g))
+    x[:, :: max(1, width // 5)] *= 16
+    return x.to(dtype)
+
+
+def quantized(rows, width, fmt, seed, rotation=0):
+    """Codes, tiles and row scales on the GPU from the oracle, and the float64 values they stand for."""
+    x = rows_like(rows, width, seed)
+    codes, scales, row = oracle.quantize(x.float().numpy(), fmt, rotation)
+    dtype = torch.float8_e4m3fn if fmt == "nvfp4" else torch.float8_e8m0fnu
+    t = torch.from_numpy(oracle.tiles(scales)).cuda().view(dtype)
+    return (torch.from_numpy(codes).cuda(), t, torch.from_numpy(row).view(-1, 1).cuda()), oracle.values(codes, scales, fmt), row
+
+
+def check_quantized(k, x, fmt, rotation):
+    codes, tiles, row = k.turing_fp4_quantize(x.cuda() if not x.is_cuda else x, fmt, rotation)
+    want_codes, want_scales, want_row = oracle.quantize(x.float().cpu().numpy(), fmt, rotation)
+    np.testing.assert_array_equal(row.view(-1).cpu().numpy(), want_row)
+    np.testing.assert_array_equal(tiles.view(torch.uint8).cpu().numpy(), oracle.tiles(want_scales))
+    np.testing.assert_array_equal(codes.cpu().numpy(), want_codes)
+
+
+# ---------------------------------------------------------------------------- quantizer
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("rows,width,rotation", [
+    (1, 32, 0), (1, 256, 256), (3, 64, 0), (127, 96, 0), (129, 1568, 0), (5, 512, 256), (130, 5120, 256),
+    (2, 5120, 0), (33, 13824, 256), (7, 13824, 0), (1, 16384, 256), (2, 49152, 256), (1, 49152, 0), (300, 768, 256)])
+def test_quantizer_bits(k, fmt, dtype, rows, width, rotation):
+    check_quantized(k, rows_like(rows, width, rows + width, dtype), fmt, rotation)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rotation", (0, 256))
+def test_quantizer_edge_rows(k, fmt, rotation):
+    width = 512
+    x = rows_like(40, width, 7)
+    x[0] = 0
+    x[1] = -0.0
+    x[2] = float("nan")
+    x[3, 5] = float("inf")
+    x[4, 300] = float("-inf")
+    x[5, 17] = float("nan")
+    x[6] = 1e-40  # bf16 subnormals
+    x[7] = torch.finfo(torch.bfloat16).tiny
+    x[8] = 3e38
+    x[9, :] = 0
+    x[9, 100] = 3.0e38
+    x[10] = 2688.0  # the row scale's own border
+    x[11] = 2704.0
+    x[12] = 1e-30
+    x[12, 0] = 1.0  # blocks far below the row's largest
+    x[13, :256] = 0
+    x[14] = 6.0
+    # Every tie of the code grid, at several block scales.
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0])
+    for i in range(16):
+        scale = (8 + i % 8) / 8.0 * 2.0 ** (i - 8)
+        x[15 + i] = (ties * scale).repeat(width // 8).bfloat16()
+        x[15 + i, 1::2] *= -1
+    check_quantized(k, x, fmt, rotation)
+
+
+def test_quantizer_block_scale_ties(k):
+    # block amax = 6 * (a midpoint of two e4m3 values): bf16 holds it, the division must keep the tie.
+    x = torch.zeros(8, 512, dtype=torch.bfloat16)
+    for i in range(8):
+        for b in range(32):
+            x[i, 16 * b] = 6.0 * (2 * ((8 + (b % 8))) + 1) / 16.0 * 2.0 ** (i - 3)
+        x[i, 511] = 2688.0
+    check_quantized(k, x, "nvfp4", 0)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantizer_takes_strided_rows(k, fmt):
+    x = rows_like(20, 1024, 3).cuda()
+    check_quantized(k, x[::2, 256:768], fmt, 256)
+    check_quantized(k, rows_like(512, 64, 4).cuda().t()[:, :256], fmt, 0)
+    flat = rows_like(1, 3 * 512 + 8, 5).cuda().view(-1)
+    check_quantized(k, flat[3 : 3 + 1024].view(2, 512), fmt, 256)  # rows start off a 16-byte boundary
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_empty_rows(k, fmt):
+    codes, tiles, row = k.turing_fp4_quantize(torch.empty(0, 256, dtype=torch.bfloat16, device="cuda"), fmt, 256)
+    assert codes.shape == (0, 128) and row.shape == (0, 1) and tiles.shape[0] == 0
+    assert k.turing_fp4_dequantize(codes, tiles, row).shape == (0, 256)
+    (w, ws, wr), _, _ = quantized(24, 256, fmt, 1)
+    assert k.turing_fp4_linear(codes, w, tiles, ws, row, wr).shape == (0, 24)
+    assert k.turing_fp4_linear_grad_input(torch.empty(0, 24, dtype=torch.bfloat16, device="cuda"), w, ws, wr).shape == (0, 256)
+
+
+# ---------------------------------------------------------------------------- dequantizer
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16, torch.float32))
+@pytest.mark.parametrize("rows,width", [(1, 32), (3, 96), (129, 1568), (130, 512), (2, 13824)])
+def test_dequantizer(k, fmt, dtype, rows, width):
+    (codes, tiles, row), values, row_np = quantized(rows, width, fmt, rows)
+    out = k.turing_fp4_dequantize(codes, tiles, row, dtype)
+    want = torch.from_numpy(values * row_np[:, None].astype(np.float64)).to(dtype)  # one rounding, or none
+    torch.testing.assert_close(out.cpu(), want, rtol=0, atol=0)
+    scalar = k.turing_fp4_dequantize(codes, tiles, torch.full((1,), 0.25, device="cuda"), dtype)
+    torch.testing.assert_close(scalar.cpu(), torch.from_numpy(values * 0.25).to(dtype), rtol=0, atol=0)
+
+
+def test_every_code_and_scale_byte(k):
+    for fmt, block in oracle.BLOCK.items():
+        rows = 256
+        width = 2 * block
+        codes = np.tile(np.arange(256, dtype=np.uint8), (rows, 1))[:, :block]
+        for r in range(rows):
+            codes[r] = (np.arange(block) * 17 + r) % 256
+        scales = np.stack([np.arange(256), np.arange(255, -1, -1)], 1).astype(np.uint8)
+        dtype = torch.float8_e4m3fn if fmt == "nvfp4" else torch.float8_e8m0fnu
+        t = torch.from_numpy(oracle.tiles(scales)).cuda().view(dtype)
+        out = k.turing_fp4_dequantize(torch.from_numpy(codes).cuda(), t, torch.ones(1, device="cuda"), torch.float32)
+        np.testing.assert_array_equal(out.cpu().numpy(), oracle.values(codes, scales, fmt).astype(np.float32))
+        assert out.shape == (rows, width)
+
+
+# ---------------------------------------------------------------------------- linear
+def linear_bound(av, ar, wv, wr, exact):
+    """Half a bf16 step of the result, and the accumulation: at most one truncation (2^-23 of the sum of
+    magnitudes) for each K = 64 instruction and each of the sums inside it, taken as eight levels,
+    doubled for the products with the two fp32 scales."""
+    mags = np.abs(av) @ np.abs(wv).T * np.abs(ar)[:, None] * np.abs(wr)[None, :]
+    steps = -(-av.shape[1] // 64) + 8
+    return HALF_BF16 * np.abs(exact) + 2 * steps * 2.0**-23 * mags + 1e-37
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,width", [
+    (1, 1, 32), (1, 8, 64), (1, 5120, 5120), (2, 193, 96), (3, 64, 256), (7, 191, 288), (8, 192, 512), (9, 333, 1568),
+    (16, 384, 1024), (17, 1537, 2048), (31, 129, 13824), (32, 200, 768), (33, 64, 320), (64, 500, 512), (65, 72, 416),
+    (100, 1000, 1056), (127, 385, 544), (128, 128, 256), (129, 257, 512), (255, 40, 96), (256, 192, 256),
+    (257, 576, 2080), (300, 1153, 800), (513, 384, 5120), (1025, 1537, 1568)])
+def test_linear(k, fmt, m, n, width):
+    (a, a_s, a_r), av, ar = quantized(m, width, fmt, m + n)
+    (w, w_s, w_r), wv, wr = quantized(n, width, fmt, n + width)
+    bias = torch.linspace(-3, 3, n, device="cuda")
+    ar, wr = ar.astype(np.float64), wr.astype(np.float64)
+    plain = (av @ wv.T) * ar[:, None] * wr[None, :]
+    for b in (None, bias):
+        out = k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r, b)
+        exact = plain if b is None else plain + b.double().cpu().numpy()[None, :]
+        assert out.shape == (m, n) and out.dtype == torch.bfloat16
+        off = np.abs(out.double().cpu().numpy() - exact)
+        bound = linear_bound(av, ar, wv, wr, exact)
+        assert (off <= bound).all(), (off / bound).max()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", (1, 40, 300))
+def test_linear_scalar_weight_scale_and_nan_rows(k, fmt, m):
+    (a, a_s, a_r), av, ar = quantized(m, 512, fmt, 1)
+    (w, w_s, _), wv, _ = quantized(200, 512, fmt, 2)
+    a_r = a_r.clone()
+    a_r[m // 2] = float("nan")
+    out = k.turing_fp4_linear(a, w, a_s, w_s, a_r, torch.full((1,), 0.37, device="cuda")).double().cpu().numpy()
+    assert np.isnan(out[m // 2]).all()
+    keep = np.arange(m) != m // 2
+    scale = np.full(200, np.float32(0.37), np.float64)
+    exact = (av @ wv.T) * ar[:, None].astype(np.float64) * scale[None, :]
+    bound = linear_bound(av, ar.astype(np.float64), wv, scale, exact) + 2.0**-23 * np.abs(exact)
+    assert (np.abs(out - exact) <= bound)[keep].all()
+
+
+@pytest.mark.parametrize("m", (1, 5, 300))
+def test_linear_nan_block_scales(k, m):
+    # An e8m0 scale byte of 255 is NaN: its row's (or column's) outputs are, and no others.
+    (a, a_s, a_r), _, _ = quantized(m, 256, "mxfp4", 1)
+    (w, w_s, w_r), _, _ = quantized(200, 256, "mxfp4", 2)
+    clean = k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r)
+    w_s = w_s.clone()
+    w_s.view(torch.uint8)[0, 1, 7, 4 * 1 + 2] = 255  # row 39, block 6
+    out = k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r)
+    bad = torch.isnan(out)
+    assert bad[:, 39].all() and bad.sum() == m
+    assert torch.equal(out[:, :39], clean[:, :39]) and torch.equal(out[:, 40:], clean[:, 40:])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_repeats_bits_and_leaves_neighbours(k, fmt):
+    for m, n, width in ((1, 300, 2048), (20, 1000, 5120), (400, 777, 512)):
+        (a, a_s, a_r), _, _ = quantized(m, width, fmt, 5)
+        (w, w_s, w_r), _, _ = quantized(n, width, fmt, 6)
+        first = k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r)
+        for _ in range(3):
+            assert torch.equal(first, k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r))
+        # The C entry into a buffer with a margin on both sides.
+        from comfyui_turing_utils_kernel import _C
+
+        buf = torch.full((m * n + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+        _C._call(buf.device, "ctu_fp4_linear", a.data_ptr(), w.data_ptr(), a_s.data_ptr(), w_s.data_ptr(), a_r.data_ptr(),
+                 w_r.data_ptr(), n, None, buf.data_ptr() + 64, m, n, width, 0 if fmt == "nvfp4" else 1)
+        assert torch.equal(buf[32 : 32 + m * n].view(m, n), first)
+        assert (buf[:32] == 7).all() and (buf[32 + m * n :] == 7).all()
+
+
+# ---------------------------------------------------------------------------- input gradient
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,width,rotation", [
+    (1, 8, 32, 0), (1, 64, 256, 256), (3, 200, 96, 0), (17, 1544, 512, 256), (128, 72, 288, 0), (129, 520, 768, 256),
+    (257, 256, 1024, 256), (300, 1000, 1568, 0), (40, 5120, 5120, 256), (5, 13824, 512, 0)])
+def test_grad_input(k, fmt, m, n, width, rotation):
+    (w, w_s, w_r), wv, wr = quantized(n, width, fmt, n + width, rotation)
+    g = torch.randn(m, n, generator=torch.Generator().manual_seed(m)).bfloat16()
+    dx = k.turing_fp4_linear_grad_input(g.cuda(), w, w_s, w_r, rotation)
+    gd, wd = g.double().numpy(), wv * wr[:, None].astype(np.float64)
+    exact = gd @ wd
+    # Sums: one truncation per K = 16 instruction and four levels inside; rotation: 8 fp32 additions
+    # of values bounded by the rotated magnitudes; then half a bf16 step.
+    mags = np.abs(gd) @ np.abs(wd)
+    off = (-(-n // 16) + 4) * 2.0**-23 * mags
+    if rotation:
+        r = oracle.rotation_matrix()
+        exact = (exact.reshape(-1, 256) @ r).reshape(m, width)
+        mixed = (mags.reshape(-1, 256) @ np.abs(r)).reshape(m, width)
+        off = (off.reshape(-1, 256) @ np.abs(r)).reshape(m, width) + 12 * 2.0**-24 * mixed
+    assert dx.dtype == torch.bfloat16 and dx.shape == (m, width)
+    got = dx.double().cpu().numpy()
+    bound = HALF_BF16 * (np.abs(exact) + off) + off + 1e-37
+    assert (np.abs(got - exact) <= bound).all(), (np.abs(got - exact) / bound).max()
+
+
+def test_grad_input_arbitrary_channel_scales(k):
+    (w, w_s, _), wv, _ = quantized(64, 256, "nvfp4", 3)
+    scale = torch.rand(64, device="cuda") + 0.1
+    g = torch.randn(20, 64, generator=torch.Generator().manual_seed(1)).bfloat16()
+    for s in (scale, scale[:1]):
+        dx = k.turing_fp4_linear_grad_input(g.cuda(), w, w_s, s).double().cpu().numpy()
+        wd = wv * np.broadcast_to(s.double().cpu().numpy(), 64)[:, None]
+        gd = g.double().numpy()
+        exact, mags = gd @ wd, np.abs(gd) @ np.abs(wd)
+        off = (HALF_BF16 + 10 * 2.0**-23) * mags  # each decoded weight rounds once
+        assert (np.abs(dx - exact) <= HALF_BF16 * (np.abs(exact) + off) + off).all()
+
+
+def test_gradient_is_the_adjoint_of_the_layer(k):
+    """<grad, layer(d)> = <dx, d>: the layer is linear in what it multiplies, so its differences are exact."""
+    m, n, width = 24, 136, 512
+    (w, w_s, w_r), wv, wr = quantized(n, width, "nvfp4", 9, 256)
+    g = torch.randn(m, n, generator=torch.Generator().manual_seed(2)).bfloat16()
+    dx = k.turing_fp4_linear_grad_input(g.cuda(), w, w_s, w_r, 256).double().cpu().numpy()
+    wd = wv * wr[:, None].astype(np.float64)
+    r = oracle.rotation_matrix()
+    rng = np.random.default_rng(0)
+    for _ in range(8):
+        d = rng.standard_normal((m, width))
+        moved = (d.reshape(-1, 256) @ r).reshape(m, width) @ wd.T
+        left, right = (g.double().numpy() * moved).sum(), (dx * d).sum()
+        # dx carries one bf16 rounding per value.
+        assert abs(left - right) <= 1.01 * HALF_BF16 * (np.abs(dx) * np.abs(d)).sum()
+
+
+def test_autograd_of_the_layer(k):
+    m, n, width = 37, 200, 768
+    (w, w_s, w_r), _, _ = quantized(n, width, "mxfp4", 4, 256)
+    x = rows_like(m, width, 1).cuda().requires_grad_(True)
+    bias = torch.randn(n, device="cuda")
+    y = k.turing_convrot_fp4_linear(x, w, w_s, w_r, bias, 256)
+    codes, scale, row = k.turing_fp4_quantize(x.detach(), "mxfp4", 256)
+    assert torch.equal(y, k.turing_fp4_linear(codes, w, scale, w_s, row, w_r, bias))
+    g = torch.randn(n, m, device="cuda").bfloat16().t()  # a gradient that is not contiguous
+    (dx,) = torch.autograd.grad(y, x, g)
+    assert torch.equal(dx, k.turing_fp4_linear_grad_input(g.contiguous(), w, w_s, w_r, 256))
+    (dx1,) = torch.autograd.grad(k.turing_convrot_fp4_linear(x, w, w_s, w_r, bias, 256).sum(), x)  # expanded gradient
+    assert torch.equal(dx1, k.turing_fp4_linear_grad_input(torch.ones_like(g).contiguous(), w, w_s, w_r, 256))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(k.turing_convrot_fp4_linear(x, w, w_s, w_r, None, 256).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="frozen"):
+        k.turing_convrot_fp4_linear(x, w, w_s, w_r, bias.requires_grad_(True), 256)
+
+
+# ---------------------------------------------------------------------------- streams, graphs, refusals
+@pytest.mark.parametrize("m", (1, 48, 300))
+def test_other_stream_and_graph(k, m):
+    width, n = 1024, 520
+    x = rows_like(m, width, 2).cuda()
+    (w, w_s, w_r), _, _ = quantized(n, width, "nvfp4", 8, 256)
+    want = k.turing_convrot_fp4_linear(x, w, w_s, w_r, None, 256)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = k.turing_convrot_fp4_linear(x, w, w_s, w_r, None, 256)
+    stream.synchronize()
+    assert torch.equal(got, want)
+    graphs = []
+    static = [x.clone(), x.clone()]
+    for s in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = k.turing_convrot_fp4_linear(s, w, w_s, w_r, None, 256)
+            back = k.turing_fp4_linear_grad_input(y, w, w_s, w_r, 256)
+        graphs.append((graph, y, back))
+    other = rows_like(m, width, 3).cuda()
+    static[1].copy_(other)
+    for graph, _, _ in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    wants = [want, k.turing_convrot_fp4_linear(other, w, w_s, w_r, None, 256)]
+    for (_, y, back), y0 in zip(graphs, wants):
+        assert torch.equal(y, y0)
+        assert torch.equal(back, k.turing_fp4_linear_grad_input(y0, w, w_s, w_r, 256))
+
+
+def test_two_streams_at_once(k):
+    width, n = 2048, 1000
+    (w, w_s, w_r), _, _ = quantized(n, width, "nvfp4", 8)
+    inputs = [quantized(m, width, "nvfp4", m)[0] for m in (1, 9, 60, 500)]
+    want = [k.turing_fp4_linear(a, w, s, w_s, r, w_r) for a, s, r in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = [[] for _ in inputs]
+    for _ in range(10):
+        for i, (st, (a, s, r)) in enumerate(zip(streams, inputs)):
+            with torch.cuda.stream(st):
+                got[i].append(k.turing_fp4_linear(a, w, s, w_s, r, w_r))
+    torch.cuda.synchronize()
+    for y, ys in zip(want, got):
+        assert all(torch.equal(y, z) for z in ys)
+
+
+def test_refusals_on_the_gpu(k):
+    (a, a_s, a_r), _, _ = quantized(4, 256, "nvfp4", 1)
+    (w, w_s, w_r), _, _ = quantized(9, 256, "nvfp4", 2)
+    (v, v_s, v_r), _, _ = quantized(9, 256, "mxfp4", 2)
+    x = torch.zeros(4, 256, dtype=torch.bfloat16, device="cuda")
+    for call in (
+        lambda: k.turing_fp4_quantize(x.float()), lambda: k.turing_fp4_quantize(x[0]),
+        lambda: k.turing_fp4_quantize(x[:, :48].contiguous()), lambda: k.turing_fp4_quantize(x[:, :96], "nvfp4", 256),
+        lambda: k.turing_fp4_quantize(x, "fp4"), lambda: k.turing_fp4_quantize(x, "nvfp4", 128),
+        lambda: k.turing_fp4_quantize(torch.zeros(1, 49408, dtype=torch.bfloat16, device="cuda")),
+        lambda: k.turing_fp4_linear(a, v, a_s, v_s, a_r, v_r),
+        lambda: k.turing_fp4_linear(a, w, a_s[:, :2], w_s, a_r, w_r),
+        lambda: k.turing_fp4_linear(a, w[:, :64], a_s, w_s, a_r, w_r),
+        lambda: k.turing_fp4_linear(a, w, a_s, w_s, a_r[:2], w_r),
+        lambda: k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r.double()),
+        lambda: k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r, torch.zeros(8, device="cuda")),
+        lambda: k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r.requires_grad_(True)),
+        lambda: k.turing_fp4_linear_grad_input(torch.zeros(4, 9, dtype=torch.bfloat16, device="cuda"), w, w_s, v_r),
+        lambda: k.turing_fp4_linear_grad_input(torch.zeros(4, 8, dtype=torch.bfloat16, device="cuda"), w, w_s, v_r),
+        lambda: k.turing_fp4_dequantize(a, a_s, a_r, torch.float64),
+        lambda: k.turing_fp4_dequantize(a.view(torch.int8), a_s, a_r),
+        lambda: k.turing_fp4_dequantize(a, a_s.view(torch.uint8), a_r),
+    ):
+        with pytest.raises(RuntimeError):
+            call()
