@@ -187,6 +187,16 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
     if (int rc = encode_codes(&map_b, w, n, k, fp4::kPairCols / 2)) return rc;
     if (int rc = encode_scales(&map_as, a_block_scales, m, k, format, col_tiles, 1)) return rc;
     if (int rc = encode_scales(&map_bs, w_block_scales, n, k, format, col_tiles, 2)) return rc;
+    // The output's tile stores need rows on 16 bytes; others are written by the kernel's warps.
+    CUtensorMap map_out = map_a;
+    if (n % 8 == 0) {
+        const uint64_t dims[2] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m)};
+        const uint64_t strides[1] = {static_cast<uint64_t>(2 * n)};
+        const uint32_t box[2] = {64, 32};
+        if (int rc = encode_tiled(&map_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, dims, strides, box,
+                                  CU_TENSOR_MAP_SWIZZLE_128B))
+            return rc;
+    }
     fp4::LinearArgs args{a_scale, w_scale, bias, out, err, static_cast<int>(m), static_cast<int>(n),
                          static_cast<int>(k), w_scale_count == 1 ? 1 : 0, format};
     const void *kernel = fp4::linear_pair_kernel(format);
@@ -194,7 +204,7 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
     if (int rc = pair_clusters(g_linear_plan[format], kernel, fp4::linear_pair_threads(), fp4::linear_pair_smem(), q,
                                &clusters))
         return rc;
-    void *params[] = {&map_a, &map_b, &map_as, &map_bs, &args};
+    void *params[] = {&map_a, &map_b, &map_as, &map_bs, &map_out, &args};
     return launch_pairs(kernel, fp4::linear_pair_threads(), fp4::linear_pair_smem(),
                         std::min<int64_t>(tiles, clusters), params, static_cast<cudaStream_t>(stream));
 }

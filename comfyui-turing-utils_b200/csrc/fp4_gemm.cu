@@ -36,8 +36,11 @@ constexpr int kAOffset = 0;
 constexpr int kBOffset = kStages * kABytes;
 constexpr int kAScaleOffset = kBOffset + kStages * kBBytes;
 constexpr int kBScaleOffset = kAScaleOffset + kStages * kAScaleBytes;
-constexpr int kStructOffset = kBScaleOffset + kStages * kBScaleBytes;
+constexpr int kStageOutOffset = kBScaleOffset + kStages * kBScaleBytes;
 constexpr int kEpilogueWarps = 4;
+constexpr int kOutCols = 64;             // columns a warp stages at a time: 128 bytes a row
+constexpr int kOutBytes = 32 * 128;      // its 32 rows
+constexpr int kStructOffset = kStageOutOffset + kEpilogueWarps * kOutBytes;
 constexpr int kThreadCount = 32 * (2 + kEpilogueWarps);
 constexpr int kTmemCols = 512;
 constexpr int kScaleCol = 2 * kPairCols;  // first column of the scales
@@ -64,7 +67,7 @@ template <int kFormat>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                            const __grid_constant__ CUtensorMap tmap_as, const __grid_constant__ CUtensorMap tmap_bs,
-                           const LinearArgs args) {
+                           const __grid_constant__ CUtensorMap tmap_out, const LinearArgs args) {
     // Scale tiles of 128 rows per stage: 64 values of K per tile (nvfp4) or 128 (mxfp4).
     constexpr int kTiles = kFormat == kNvfp4 ? 4 : 2;
     constexpr uint32_t kStageTx = 2 * (kABytes + kBBytes + 3 * kTiles * 512);
@@ -105,6 +108,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
         prefetch_tmap(&tmap_b);
         prefetch_tmap(&tmap_as);
         prefetch_tmap(&tmap_bs);
+        prefetch_tmap(&tmap_out);
     }
     tc_fence_before();
     __syncthreads();
@@ -143,68 +147,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             if (!ok || *abort_flag) settle_inflight_copies();
         }
     } else if (warp == 1) {
-        if (leader && lane == 0) {
+        if (leader) {
+            // The whole warp runs this loop on warp-uniform values and one elected lane issues: the
+            // operands then sit in uniform registers already (a single-lane loop moves each of them
+            // there first, which costs more than an MMA of this width takes).
             int s = 0;
             uint32_t ph = 0;
+            uint32_t set = 0;
             int local = 0;
             bool ok = true;
-            uint32_t set = 0;
+            const uint32_t a0 = smem_desc_low(smem_u32(smem + kAOffset));
+            const uint32_t b0 = smem_desc_low(smem_u32(smem + kBOffset));
+            const uint32_t as0 = smem_desc_low(smem_u32(smem + kAScaleOffset));
+            const uint32_t bs0 = smem_desc_low(smem_u32(smem + kBScaleOffset));
+            const uint32_t empty0 = smem_u32(&S.empty[0]);
             for (int t = pair; t < num_tiles && ok; t += num_pairs, ++local) {
-                const int ab = local & 1;
-                if (!guard.wait_cluster(&S.acc_empty[ab], ((local >> 1) & 1) ^ 1u, kErrTimeoutAccumFree)) {
-                    ok = false;
-                    break;
-                }
+                const uint32_t ab = local & 1;
+                ok = __all_sync(0xffffffffu, guard.wait_cluster(&S.acc_empty[ab], ((local >> 1) & 1) ^ 1u, kErrTimeoutAccumFree));
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + static_cast<uint32_t>(ab * kPairCols);
+                const uint32_t d = tmem_base + ab * kPairCols;
                 // The tile's first column may lie 64 rows into its first scale tile: two columns.
                 const uint32_t b_shift = static_cast<uint32_t>(((t % num_n) * kPairCols % 128) / 32);
                 for (int kb = 0; kb < nk; ++kb) {
-                    if (!guard.wait(&S.full[s], ph, kErrTimeoutFull)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = __all_sync(0xffffffffu, guard.wait(&S.full[s], ph, kErrTimeoutFull));
+                    if (!ok) break;
                     tc_fence_after();
                     // Scale sets alternate, so copies for one stage do not wait for the MMAs of the
                     // stage before; copies and MMAs of one thread execute in order.
                     const uint32_t sa = tmem_base + kScaleCol + set * kScaleSet;
                     const uint32_t sb = sa + 16;
-                    const uint32_t as = smem_u32(smem + kAScaleOffset + s * kAScaleBytes);
-                    const uint32_t bs = smem_u32(smem + kBScaleOffset + s * kBScaleBytes);
+                    const uint32_t a = a0 + s * (kABytes >> 4);
+                    const uint32_t b = b0 + s * (kBBytes >> 4);
+                    const uint32_t as = as0 + s * (kAScaleBytes >> 4);
+                    const uint32_t bs = bs0 + s * (kBScaleBytes >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int c = 0; c < kTiles; ++c) {
-                        copy_scales_pair(sa + 4 * c, smem_desc_scales(as + c * 512));
-                        copy_scales_pair(sb + 8 * c, smem_desc_scales(bs + c * 512));
-                        copy_scales_pair(sb + 8 * c + 4, smem_desc_scales(bs + (kTiles + c) * 512));
-                    }
-                    const uint32_t a = smem_u32(smem + kAOffset + s * kABytes);
-                    const uint32_t b = smem_u32(smem + kBOffset + s * kBBytes);
+                        for (int c = 0; c < kTiles; ++c) {
+                            copy_scales_pair(sa + 4 * c, desc64(as + c * 32, kDescScalesHigh));
+                            copy_scales_pair(sb + 8 * c, desc64(bs + c * 32, kDescScalesHigh));
+                            copy_scales_pair(sb + 8 * c + 4, desc64(bs + (kTiles + c) * 32, kDescScalesHigh));
+                        }
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c) {
-                        const int tile = kFormat == kNvfp4 ? c : c / 2;
-                        const uint32_t idesc = kFormat == kNvfp4 ? idesc_fp4(kFormat, kPairRows, kPairCols, 0)
-                                                                 : idesc_fp4(kFormat, kPairRows, kPairCols, 2 * (c & 1));
-                        mma_fp4_pair<kFormat>(d, smem_desc_sw128(a + 32 * c), smem_desc_sw128(b + 32 * c), idesc,
-                                              sa + 4 * tile, sb + 8 * tile + b_shift, (kb | c) != 0 ? 1u : 0u);
+                        for (int c = 0; c < kChunks; ++c) {
+                            const int tile = kFormat == kNvfp4 ? c : c / 2;
+                            const uint32_t idesc = kFormat == kNvfp4
+                                                       ? idesc_fp4(kFormat, kPairRows, kPairCols, 0)
+                                                       : idesc_fp4(kFormat, kPairRows, kPairCols, 2 * (c & 1));
+                            mma_fp4_pair<kFormat>(d, desc64(a + 2 * c, kDescSw128High), desc64(b + 2 * c, kDescSw128High),
+                                                  idesc, sa + 4 * tile, sb + 8 * tile + b_shift, (kb | c) != 0 ? 1u : 0u);
+                        }
+                        mma_commit_pair_both_at(empty0 + 8 * s);
+                        if (kb == nk - 1) mma_commit_pair_both(&S.acc_full[ab]);
                     }
+                    __syncwarp();
                     set ^= 1u;
-                    mma_commit_pair_both(&S.empty[s]);
                     if (++s == kStages) {
                         s = 0;
                         ph ^= 1u;
                     }
                 }
-                if (!ok) break;
-                mma_commit_pair_both(&S.acc_full[ab]);
             }
-            mma_commit_pair_local(&S.drain);
-            mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+            if (elect_one()) {
+                mma_commit_pair_local(&S.drain);
+                mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+            }
+            __syncwarp();
         }
     } else {
         const int quad = warp & 3;
         const int ethread = threadIdx.x - 64;
         const uint32_t leader_empty = mapa_shared(smem_u32(&S.acc_empty[0]), 0u);
-        const bool vector = (args.n & 7) == 0;
+        const uint32_t staged = smem_u32(smem + kStageOutOffset + (warp - 2) * kOutBytes);
+        const bool tma_out = (args.n & 7) == 0;  // rows of the output start on 16 bytes
         bool alive = true;
         int local = 0;
         for (int t = pair; t < num_tiles; t += num_pairs, ++local) {
@@ -226,41 +241,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             }
             if (!alive) continue;
             tc_fence_after();
-            const int m = m0 + quad * 32 + lane;
-            const bool row_ok = m < args.m;
-            const float a_s = row_ok ? args.a_scale[m] : 0.0f;
+            const int m_warp = m0 + quad * 32;
+            const float a_s = m_warp + lane < args.m ? args.a_scale[m_warp + lane] : 0.0f;
 #pragma unroll 1
-            for (int c = 0; c < kPairCols / 32; ++c) {
-                uint32_t acc[32];
-                tmem_ld_32x32b_x32(tmem_base + static_cast<uint32_t>(ab * kPairCols + c * 32) +
-                                       (static_cast<uint32_t>(quad * 32) << 16),
-                                   acc);
+            for (int c = 0; c < kPairCols / kOutCols; ++c) {
+                const int n = n0 + c * kOutCols;
+                if (n >= args.n || m_warp >= args.m) break;
+                uint32_t acc[2][32];
+                const uint32_t src = tmem_base + static_cast<uint32_t>(ab * kPairCols + c * kOutCols) +
+                                     (static_cast<uint32_t>(quad * 32) << 16);
+                tmem_ld_32x32b_x32(src, acc[0]);
+                tmem_ld_32x32b_x32(src + 32, acc[1]);
+                // The staging rows are free once the last copy out of them has read them.
+                if (lane == 0) bulk_wait_read_all();
+                __syncwarp();
                 tmem_ld_wait();
-                const int valid = args.n - (n0 + c * 32);
-                if (!row_ok || valid <= 0) continue;
-                __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(args.out) + static_cast<int64_t>(m) * args.n + n0 + c * 32;
-                float v[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    v[j] = __fmaf_rn(__fmul_rn(__uint_as_float(acc[j]), a_s), S.col_scale[c * 32 + j],
-                                     S.col_bias[c * 32 + j]);
-                if (vector) {
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (8 * q < valid)
-                            reinterpret_cast<uint4 *>(dst)[q] =
-                                make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                                           pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t p[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int i = 8 * q + 2 * j;
+                            const int col = c * kOutCols + 32 * h + i;
+                            p[j] = pack_bf16x2(
+                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][i]), a_s), S.col_scale[col], S.col_bias[col]),
+                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][i + 1]), a_s), S.col_scale[col + 1],
+                                          S.col_bias[col + 1]));
+                        }
+                        st_shared_v4(staged + 128u * lane + ((static_cast<uint32_t>(4 * h + q) ^ (lane & 7u)) << 4), p);
+                    }
+                }
+                if (tma_out) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmap_out, staged, n, m_warp);
+                        bulk_commit();
+                    }
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (j < valid) dst[j] = __float2bfloat16_rn(v[j]);
+                    __syncwarp();
+                    store_rows(static_cast<__nv_bfloat16 *>(args.out), staged, m_warp, n, args.m, args.n, lane);
+                    __syncwarp();
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(leader_empty + static_cast<uint32_t>(ab * sizeof(uint64_t)));
         }
+        if (lane == 0) bulk_wait_all();  // the staged rows leave shared memory before the CTA does
     }
 
     tc_fence_before();

@@ -27,14 +27,32 @@ __device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const void *tma
         : "memory");
 }
 
-// Descriptor of one 512-byte scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(1) << 16;
-    d |= static_cast<uint64_t>(128 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    return d;
+// Operand descriptors: 128-byte-swizzled tiles (8-row groups 1024 bytes apart) and 512-byte scale tiles
+// (32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart).
+// The two halves of a descriptor: the low word holds the address (and a constant), so a step through
+// shared memory is one addition; the high words are constants.
+__device__ __forceinline__ uint32_t smem_desc_low(uint32_t smem_addr) {
+    return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16);
+}
+constexpr uint32_t kDescSw128High = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kDescScalesHigh = (128u >> 4) | (1u << 14);
+__device__ __forceinline__ uint64_t desc64(uint32_t low, uint32_t high) {
+    return (static_cast<uint64_t>(high) << 32) | low;
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r)::"memory");
+    return r != 0;
+}
+
+__device__ __forceinline__ void mma_commit_pair_both_at(uint32_t bar) {
+    const uint16_t mask = 0x3;
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(mask)
+        : "memory");
 }
 
 // One scale tile into four columns of tensor memory, repeated for the four groups of 32 lanes; in
@@ -96,6 +114,54 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
            | (1u << 10)                               // B: bf16
            | (static_cast<uint32_t>(n >> 3) << 17)    // N / 8
            | (static_cast<uint32_t>(m >> 4) << 24);   // M / 16
+}
+
+// 2D tile store from shared memory; what lies beyond the tensor is not written.
+__device__ __forceinline__ void tma_store_2d(const void *tmap, uint32_t smem_src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(tmap), "r"(x),
+                 "r"(y), "r"(smem_src)
+                 : "memory");
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// 32 staged rows of 64 bf16 values (128-byte swizzle) to an output whose rows need not start on 16
+// bytes: a warp writes a row at a time in aligned pairs.  Where a row starts on an odd element, a lane
+// pairs its neighbour's second value with its own first, and the row's ends go out alone.
+__device__ __forceinline__ void store_rows(__nv_bfloat16 *out, uint32_t staged, int m0, int n0, int rows, int cols,
+                                           int lane) {
+    const int valid = min(64, cols - n0);
+    const int count = min(32, rows - m0);
+    for (int r = 0; r < count; ++r) {
+        const int64_t first = static_cast<int64_t>(m0 + r) * cols + n0;
+        const uint32_t own = ld_shared_u32(staged + 128u * r + (((static_cast<uint32_t>(lane) >> 2) ^ (r & 7u)) << 4) +
+                                           (lane & 3u) * 4u);
+        uint16_t *dst = reinterpret_cast<uint16_t *>(out) + first;
+        if ((first & 1) == 0) {
+            if (2 * lane + 1 < valid)
+                *reinterpret_cast<uint32_t *>(dst + 2 * lane) = own;
+            else if (2 * lane < valid)
+                dst[2 * lane] = static_cast<uint16_t>(own);
+        } else {
+            const uint32_t before = __shfl_up_sync(0xffffffffu, own, 1);
+            if (lane == 0)
+                dst[0] = static_cast<uint16_t>(own);
+            else if (2 * lane < valid)
+                *reinterpret_cast<uint32_t *>(dst + 2 * lane - 1) = __byte_perm(before, own, 0x5432);
+            else if (2 * lane - 1 < valid)
+                dst[2 * lane - 1] = static_cast<uint16_t>(before >> 16);
+            if (lane == 31 && valid == 64) dst[63] = static_cast<uint16_t>(own >> 16);
+        }
+    }
 }
 
 __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
