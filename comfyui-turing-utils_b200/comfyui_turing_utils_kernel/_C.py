@@ -920,8 +920,8 @@ def layer_norm(input, weight=None, bias=None, epsilon=1.0e-5):
     x = input.contiguous()
     rows = x.numel() // hidden
     out = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
+    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
     _call(x.device, "ctu_layer_norm", x.data_ptr(), None if weight is None else weight.data_ptr(),
           None if bias is None else bias.data_ptr(), out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, hidden,
           float(epsilon), _NORM_TYPES[x.dtype], _NORM_TYPES[wtype])

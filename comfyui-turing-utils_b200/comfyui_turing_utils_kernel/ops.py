@@ -552,6 +552,12 @@ def turing_fp4_linear_grad_input(grad_output: torch.Tensor, weight: torch.Tensor
                                                                 rotation)
 
 
+# Gradients go through a torch.autograd.Function around the ops: an op with registered autograd costs
+# twice as much host time in both directions (layer norm: 45 and 91 us).
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _no_second_derivative(what: str) -> None:
     if torch.is_grad_enabled():  # create_graph=True
         raise RuntimeError(f"{what} has no second derivative")
@@ -572,24 +578,23 @@ def _convrot_fp4_linear_fake(x, weight, weight_block_scale, weight_scale, bias=N
     return x.new_empty((x.size(0), weight.size(0)), dtype=torch.bfloat16)
 
 
-def _convrot_fp4_linear_setup(ctx, inputs, output):
-    x, weight, weight_block_scale, weight_scale, bias, rotation = inputs
-    if ctx.needs_input_grad[3] or ctx.needs_input_grad[4]:
-        raise RuntimeError("the FP4 linear's weight scale and bias are frozen: detach them")
-    if x.dtype != torch.bfloat16 or weight.size(0) % 8:
-        raise RuntimeError("the FP4 linear's gradient takes bfloat16 input and N divisible by 8")
-    ctx.save_for_backward(weight, weight_block_scale, weight_scale)
-    ctx.rotation = rotation
+class _ConvrotFp4Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, weight_block_scale, weight_scale, bias, rotation):
+        if ctx.needs_input_grad[3] or ctx.needs_input_grad[4]:
+            raise RuntimeError("the FP4 linear's weight scale and bias are frozen: detach them")
+        if x.dtype != torch.bfloat16 or weight.size(0) % 8:
+            raise RuntimeError("the FP4 linear's gradient takes bfloat16 input and N divisible by 8")
+        ctx.save_for_backward(weight, weight_block_scale, weight_scale)
+        ctx.rotation = rotation
+        return torch.ops.turing_utils.convrot_fp4_linear.default(x, weight, weight_block_scale, weight_scale, bias,
+                                                                 rotation)
 
-
-def _convrot_fp4_linear_backward(ctx, grad):
-    _no_second_derivative("the FP4 linear")
-    dx = torch.ops.turing_utils.fp4_linear_grad_input.default(grad, *ctx.saved_tensors, ctx.rotation)
-    return dx, None, None, None, None, None
-
-
-torch.library.register_autograd("turing_utils::convrot_fp4_linear", _convrot_fp4_linear_backward,
-                                setup_context=_convrot_fp4_linear_setup)
+    @staticmethod
+    def backward(ctx, grad):
+        _no_second_derivative("the FP4 linear")
+        dx = torch.ops.turing_utils.fp4_linear_grad_input.default(grad, *ctx.saved_tensors, ctx.rotation)
+        return dx, None, None, None, None, None
 
 
 def turing_convrot_fp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_block_scale: torch.Tensor,
@@ -598,6 +603,8 @@ def turing_convrot_fp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_bloc
     """Linear of bf16/fp16 rows with FP4 weights: the rows are rotated and quantized to the weights'
     format, then multiplied.  Differentiable in ``x`` (bf16): the quantization passes the gradient
     straight through, the weights are frozen."""
+    if _wants_grad(x, weight_scale, bias):
+        return _ConvrotFp4Linear.apply(x, weight, weight_block_scale, weight_scale, bias, rotation)
     return torch.ops.turing_utils.convrot_fp4_linear.default(x, weight, weight_block_scale, weight_scale, bias, rotation)
 
 
@@ -628,25 +635,20 @@ def _layer_norm_backward_fake(grad, x, mean, rstd, weight=None, bias=None, needs
             torch.empty_like(bias) if needs & 4 and bias is not None else none)
 
 
-def _layer_norm_setup(ctx, inputs, output):
-    x, weight, bias, _ = inputs
-    ctx.save_for_backward(x, output[1], output[2], weight, bias)
-    ctx.mark_non_differentiable(output[1], output[2])
-    ctx.set_materialize_grads(False)
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, epsilon):
+        y, mean, rstd = torch.ops.turing_utils.layer_norm.default(x, weight, bias, epsilon)
+        ctx.save_for_backward(x, mean, rstd, weight, bias)
+        return y
 
-
-def _layer_norm_autograd(ctx, grad, *_):
-    if grad is None:
-        return None, None, None, None
-    _no_second_derivative("LayerNorm")
-    x, mean, rstd, weight, bias = ctx.saved_tensors
-    wanted = ctx.needs_input_grad
-    needs = sum(bit for bit, want in zip((1, 2, 4), wanted) if want)
-    grads = torch.ops.turing_utils.layer_norm_backward.default(grad, x, mean, rstd, weight, bias, needs)
-    return (*(g if want else None for g, want in zip(grads, wanted)), None)
-
-
-torch.library.register_autograd("turing_utils::layer_norm", _layer_norm_autograd, setup_context=_layer_norm_setup)
+    @staticmethod
+    def backward(ctx, grad):
+        _no_second_derivative("LayerNorm")
+        wanted = ctx.needs_input_grad
+        needs = wanted[0] + 2 * wanted[1] + 4 * wanted[2]
+        dx, dw, db = torch.ops.turing_utils.layer_norm_backward.default(grad, *ctx.saved_tensors, needs)
+        return dx if wanted[0] else None, dw if wanted[1] else None, db if wanted[2] else None, None
 
 
 def turing_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -654,6 +656,8 @@ def turing_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias:
     """Affine layer norm over the last dimension, differentiable in x, weight and bias.
 
     x is bf16, fp16 or fp32; weight and bias have its type or are fp32."""
+    if _wants_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, epsilon)
     return torch.ops.turing_utils.layer_norm.default(x, weight, bias, epsilon)[0]
 
 

@@ -72,7 +72,19 @@ struct LinearArgs {
     int m, n, k;
     int w_scale_count;
     int format;
+    int split;  // CTAs of a cluster that share K (the kernel for few rows)
 };
+
+// Kernel for few rows: a strip of 128 weight rows per CTA, `tokens` activation rows at a time.
+struct SmallKernel {
+    const void *kernel;
+    int smem;
+    int threads;
+    int tokens;
+    int per_sm;  // CTAs resident on an SM
+};
+constexpr int kStripRows = 128;
+SmallKernel linear_small_kernel(int format, int64_t m);
 
 // CTA-pair product (tcgen05 block-scaled MMA).
 constexpr int kPairRows = 256;  // output rows of a pair tile

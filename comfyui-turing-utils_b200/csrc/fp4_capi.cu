@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <mutex>
@@ -76,12 +77,28 @@ int pair_clusters(PairPlan &plan, const void *kernel, int threads, int smem, con
     return CTU_OK;
 }
 
-int launch_pairs(const void *kernel, int threads, int smem, int64_t pairs, void **params, cudaStream_t stream) {
+// Opts a kernel in to its shared memory, once per device.
+struct SmemPlan {
+    std::mutex mutex;
+    bool set[64] = {};
+};
+
+int opt_in_smem(SmemPlan &plan, const void *kernel, int smem, int device) {
+    std::lock_guard<std::mutex> lock(plan.mutex);
+    if (!plan.set[device]) {
+        CTU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        plan.set[device] = true;
+    }
+    return CTU_OK;
+}
+
+int launch_clusters(const void *kernel, int threads, int smem, int64_t ctas, int cluster, void **params,
+                    cudaStream_t stream) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {2, 1, 1};
+    attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -89,6 +106,10 @@ int launch_pairs(const void *kernel, int threads, int smem, int64_t pairs, void 
     cfg.numAttrs = 1;
     CTU_CUDA(cudaLaunchKernelExC(&cfg, kernel, params));
     return CTU_OK;
+}
+
+int launch_pairs(const void *kernel, int threads, int smem, int64_t pairs, void **params, cudaStream_t stream) {
+    return launch_clusters(kernel, threads, smem, 2 * pairs, 2, params, stream);
 }
 
 // Code rows of 128 bytes, `box_rows` of them, and whole scale tiles.
@@ -107,6 +128,11 @@ int encode_scales(CUtensorMap *map, const void *scales, int64_t rows, int64_t k,
     const uint32_t box[3] = {128, static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows)};
     return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, scales, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
+
+// Forces a product kernel for tests: 0 by size, 1 the pair kernel, 2 the kernel for few rows.
+std::atomic<int> g_fp4_kernel{0};
+
+SmemPlan g_small_plan[8];
 
 PairPlan g_linear_plan[2];
 PairPlan g_grad_plan[2];
@@ -182,6 +208,29 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
     uint32_t *err;
     if (int rc = kernel_device(&q, &err)) return rc;
     const int col_tiles = format == CTU_FP4_NVFP4 ? 4 : 2;
+    fp4::LinearArgs args{a_scale, w_scale, bias, out, err, static_cast<int>(m), static_cast<int>(n),
+                         static_cast<int>(k), w_scale_count == 1 ? 1 : 0, format, 1};
+    const int forced = g_fp4_kernel.load(std::memory_order_relaxed);
+    if (forced == 2 || (forced == 0 && m <= 128)) {
+        const fp4::SmallKernel sk = fp4::linear_small_kernel(format, m);
+        const int64_t strips =
+            ((m + sk.tokens - 1) / sk.tokens) * ((n + fp4::kStripRows - 1) / fp4::kStripRows);
+        const int64_t slots = static_cast<int64_t>(q.num_sms) * sk.per_sm;
+        const int64_t stages = (k + 255) / 256;
+        if (strips > INT32_MAX / 8)
+            return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 linear dimensions exceed the CUDA kernel range");
+        args.split = static_cast<int>(std::max<int64_t>(1, std::min({int64_t(8), slots / strips, stages})));
+        CUtensorMap map_w, map_a, map_ws, map_as;
+        if (int rc = encode_codes(&map_w, w, n, k, fp4::kStripRows)) return rc;
+        if (int rc = encode_codes(&map_a, a, m, k, sk.tokens)) return rc;
+        if (int rc = encode_scales(&map_ws, w_block_scales, n, k, format, col_tiles, 1)) return rc;
+        if (int rc = encode_scales(&map_as, a_block_scales, m, k, format, col_tiles, 1)) return rc;
+        const int which = (sk.tokens == 16 ? 0 : sk.tokens == 32 ? 1 : sk.tokens == 64 ? 2 : 3) + 4 * format;
+        if (int rc = opt_in_smem(g_small_plan[which], sk.kernel, sk.smem, q.device)) return rc;
+        void *params[] = {&map_w, &map_a, &map_ws, &map_as, &args};
+        return launch_clusters(sk.kernel, sk.threads, sk.smem, strips * args.split, args.split, params,
+                               static_cast<cudaStream_t>(stream));
+    }
     CUtensorMap map_a, map_b, map_as, map_bs;
     if (int rc = encode_codes(&map_a, a, m, k, 128)) return rc;
     if (int rc = encode_codes(&map_b, w, n, k, fp4::kPairCols / 2)) return rc;
@@ -197,8 +246,6 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
                                   CU_TENSOR_MAP_SWIZZLE_128B))
             return rc;
     }
-    fp4::LinearArgs args{a_scale, w_scale, bias, out, err, static_cast<int>(m), static_cast<int>(n),
-                         static_cast<int>(k), w_scale_count == 1 ? 1 : 0, format};
     const void *kernel = fp4::linear_pair_kernel(format);
     int clusters = 0;
     if (int rc = pair_clusters(g_linear_plan[format], kernel, fp4::linear_pair_threads(), fp4::linear_pair_smem(), q,
@@ -207,6 +254,11 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
     void *params[] = {&map_a, &map_b, &map_as, &map_bs, &map_out, &args};
     return launch_pairs(kernel, fp4::linear_pair_threads(), fp4::linear_pair_smem(),
                         std::min<int64_t>(tiles, clusters), params, static_cast<cudaStream_t>(stream));
+}
+
+int ctu_debug_set_fp4_kernel(int which) {
+    if (which < 0 || which > 2) return fail(CTU_ERR_INVALID_ARGUMENT, "unknown FP4 product kernel %d", which);
+    return g_fp4_kernel.exchange(which);
 }
 
 int64_t ctu_fp4_grad_workspace_bytes(int64_t n, int64_t k) { return n <= 0 || k <= 0 ? 0 : 2 * n * k; }

@@ -359,6 +359,9 @@ CTU_API int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_
                            int64_t w_scale_count, const float *bias, void *out, int64_t m, int64_t n, int64_t k,
                            int format, void *stream);
 
+/* Test hook: which kernel ctu_fp4_linear runs (0 by size, 1 CTA pair, 2 few rows); returns the last. */
+CTU_API int ctu_debug_set_fp4_kernel(int which);
+
 /*
  * dx[m, k] = grad[m, n] w[n, k], rotated back when rotation is 256 (the rotation is its own inverse);
  * grad and dx bf16, n a multiple of 8.  The weights are decoded to bf16 in the workspace

@@ -1,5 +1,7 @@
 """4-bit floating point quantizer, dequantizer, linear and its input gradient against 64-bit definitions."""
 
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -145,6 +147,17 @@ def test_every_code_and_scale_byte(k):
 
 
 # ---------------------------------------------------------------------------- linear
+@contextlib.contextmanager
+def forced_kernel(which):
+    from comfyui_turing_utils_kernel import _lib
+
+    before = _lib.load().ctu_debug_set_fp4_kernel(which)
+    try:
+        yield
+    finally:
+        _lib.load().ctu_debug_set_fp4_kernel(before)
+
+
 def linear_bound(av, ar, wv, wr, exact):
     """Half a bf16 step of the result, and the accumulation: at most one truncation (2^-23 of the sum of
     magnitudes) for each K = 64 instruction and each of the sums inside it, taken as eight levels,
@@ -166,8 +179,9 @@ def test_linear(k, fmt, m, n, width):
     bias = torch.linspace(-3, 3, n, device="cuda")
     ar, wr = ar.astype(np.float64), wr.astype(np.float64)
     plain = (av @ wv.T) * ar[:, None] * wr[None, :]
-    for b in (None, bias):
-        out = k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r, b)
+    for b, which in ((None, 0), (bias, 0), (bias, 1), (None, 2), (bias, 2)):  # by size, CTA pair, few rows
+        with forced_kernel(which):
+            out = k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r, b)
         exact = plain if b is None else plain + b.double().cpu().numpy()[None, :]
         assert out.shape == (m, n) and out.dtype == torch.bfloat16
         off = np.abs(out.double().cpu().numpy() - exact)
