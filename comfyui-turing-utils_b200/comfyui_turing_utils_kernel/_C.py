@@ -884,7 +884,7 @@ def fp4_linear_grad_input(grad_output, weight, weight_block_scale, weight_scale,
     dx = torch.empty((m, k), dtype=torch.bfloat16, device=dev)
     if m == 0:
         return dx
-    workspace = torch.empty(_lib.load().ctu_fp4_grad_workspace_bytes(n, k), dtype=torch.uint8, device=dev)
+    workspace = torch.empty(_lib.load().ctu_fp4_grad_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
     _call(dev, "ctu_fp4_linear_grad_input", g.data_ptr(), w.data_ptr(), w_bs.data_ptr(), w_s.data_ptr(), w_s.numel(),
           rotation, workspace.data_ptr(), dx.data_ptr(), m, n, k, fmt)
     return dx

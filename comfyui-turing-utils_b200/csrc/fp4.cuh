@@ -42,8 +42,12 @@ struct QuantArgs {
     int rotation;  // 0 or 256
     int dtype;     // CTU_DTYPE_BF16 / FP16
     int num_sms;
+    uint32_t *err;
+    int rows_per_warp;  // short rows side by side in a warp: 8, 4 or 2 of them (K <= 256, 512, 1024), else 1
+    int load_groups;    // groups of 256 columns per tile load (rotation)
 };
-cudaError_t launch_quantize(const QuantArgs &a, cudaStream_t stream);
+// `map` (rotation only): x as lines of 64 values, 4 * load_groups of them to a box, 128-byte swizzle.
+cudaError_t launch_quantize(const QuantArgs &a, const CUtensorMap &map, cudaStream_t stream);
 
 struct DequantArgs {
     const uint8_t *codes;
@@ -58,10 +62,6 @@ struct DequantArgs {
     int num_sms;
 };
 cudaError_t launch_dequantize(const DequantArgs &a, cudaStream_t stream);
-// The weights as the gradient's product reads them: bf16 [k, n], rounded once from
-// code * block_scale * row_scale.
-cudaError_t launch_decode_transposed(const DequantArgs &a, cudaStream_t stream);
-
 // out[m, n] = bf16(fma(acc * a_scale[m], w_scale[n], bias[n]))
 struct LinearArgs {
     const float *a_scale;  // [m]
@@ -95,15 +95,19 @@ int linear_pair_threads();
 
 // Gradient with respect to the input: dx[m, k] = grad[m, n] w[n, k], rotated back.
 struct GradArgs {
-    void *out;  // bf16 [m, k]
+    void *out;        // bf16 [m, k]
+    float *partials;  // [split][m][k] where split > 1
     uint32_t *err;
     int m, n, k;
     int rotation;
+    int split;  // parts of the sum over n
 };
 constexpr int kGradCols = 256;
 int grad_pair_smem();
 const void *grad_pair_kernel(int rotation);
 int grad_pair_threads();
+// Joins the partial sums of a split product: sum over parts in order, rotation, one rounding.
+cudaError_t launch_grad_join(const GradArgs &a, int num_sms, cudaStream_t stream);
 
 }  // namespace fp4
 }  // namespace ctu

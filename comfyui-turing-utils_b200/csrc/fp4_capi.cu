@@ -137,6 +137,27 @@ SmemPlan g_small_plan[8];
 PairPlan g_linear_plan[2];
 PairPlan g_grad_plan[2];
 
+// Parts of the gradient's sum over n.  Tiles that do not fill the pairs of a B200 (74) are cut along n
+// until the rounds of pairs, counted in 64-row stages, are as few as they get; each further part costs a
+// pass of fp32 sums over dx (about four stages' worth a tile), so up to eight.  333 x 13824 x 5120: 40
+// tiles of 216 stages, three parts are two rounds of 72.  Depends on the sizes alone, so that the
+// workspace and the sums' order do.
+int64_t grad_split(int64_t m, int64_t n, int64_t k) {
+    constexpr int64_t kPairs = 74;
+    const int64_t tiles = ((m + fp4::kPairRows - 1) / fp4::kPairRows) * ((k + fp4::kGradCols - 1) / fp4::kGradCols);
+    const int64_t stages = (n + 63) / 64;
+    if (tiles >= kPairs) return 1;
+    int64_t best = 1, cost = stages;
+    for (int64_t s = 2; s <= 8 && s <= stages; ++s) {
+        const int64_t c = (tiles * s + kPairs - 1) / kPairs * ((stages + s - 1) / s + 4) + 8;
+        if (c < cost) {
+            cost = c;
+            best = s;
+        }
+    }
+    return best;
+}
+
 }  // namespace
 
 extern "C" {
@@ -164,8 +185,23 @@ int ctu_fp4_quantize(const void *x, int64_t rows, int64_t k, int dtype, int form
     DeviceQuery q;
     uint32_t *err;
     if (int rc = kernel_device(&q, &err)) return rc;
-    fp4::QuantArgs a{x, codes, block_scales, row_scales, rows, static_cast<int>(k), format, rotation, dtype, q.num_sms};
-    CTU_CUDA(fp4::launch_quantize(a, static_cast<cudaStream_t>(stream)));
+    fp4::QuantArgs a{x, codes, block_scales, row_scales, rows, static_cast<int>(k), format, rotation, dtype, q.num_sms, err};
+    const int groups = static_cast<int>((k + 255) / 256);
+    a.rows_per_warp = groups == 1 ? 8 : groups == 2 ? 4 : groups <= 4 ? 2 : 1;
+    CUtensorMap map{};
+    if (rotation != 0) {
+        // Rows of three groups do not lie side by side: one to a warp.
+        if (groups == 3) a.rows_per_warp = 1;
+        a.load_groups = a.rows_per_warp > 1 || groups % 8 == 0 ? 8 : groups % 4 == 0 ? 4 : 2;
+        const uint64_t lines = static_cast<uint64_t>(rows) * static_cast<uint64_t>(k / 64);
+        if (lines > INT32_MAX) return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 quantizer dimensions exceed the CUDA kernel range");
+        const uint64_t dims[2] = {64, lines};
+        const uint64_t strides[1] = {128};
+        const uint32_t box[2] = {64, static_cast<uint32_t>(4 * a.load_groups)};
+        if (int rc = encode_tiled(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+            return rc;
+    }
+    CTU_CUDA(fp4::launch_quantize(a, map, static_cast<cudaStream_t>(stream)));
     return CTU_OK;
 }
 
@@ -261,7 +297,11 @@ int ctu_debug_set_fp4_kernel(int which) {
     return g_fp4_kernel.exchange(which);
 }
 
-int64_t ctu_fp4_grad_workspace_bytes(int64_t n, int64_t k) { return n <= 0 || k <= 0 ? 0 : 2 * n * k; }
+int64_t ctu_fp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    const int64_t split = grad_split(m, n, k);
+    return 2 * n * k + (split > 1 ? split * m * k * 4 : 0);
+}
 
 int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t *w_block_scales, const float *w_scale,
                               int64_t w_scale_count, int rotation, void *workspace, void *dx, int64_t m, int64_t n,
@@ -282,7 +322,7 @@ int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t 
     if (!aligned16(grad) || !aligned16(w) || !aligned16(w_block_scales) || !aligned16(workspace) || !aligned16(dx))
         return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 linear gradient tensors must be 16-byte aligned");
     const int64_t tiles = ((m + fp4::kPairRows - 1) / fp4::kPairRows) * ((k + fp4::kGradCols - 1) / fp4::kGradCols);
-    if (tiles > INT32_MAX / 2 || n > 65535ll * 32)
+    if (tiles > INT32_MAX / 2)
         return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 linear gradient dimensions exceed the CUDA kernel range");
     DeviceQuery q;
     uint32_t *err;
@@ -291,14 +331,14 @@ int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t 
     fp4::DequantArgs d{w, w_block_scales, w_scale, workspace, n, static_cast<int>(k), format, w_scale_count == 1 ? 1 : 0,
                        CTU_DTYPE_BF16, q.num_sms};
     CUtensorMap map_a, map_b;
-    const uint32_t box[2] = {64, 128};
+    const uint32_t box_a[2] = {64, 128}, box_b[2] = {64, 64};
     const uint64_t dims_a[2] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m)};
-    const uint64_t dims_b[2] = {static_cast<uint64_t>(n), static_cast<uint64_t>(k)};
-    const uint64_t stride[1] = {static_cast<uint64_t>(2 * n)};
-    if (int rc = encode_tiled(&map_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, grad, dims_a, stride, box,
+    const uint64_t dims_b[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)};
+    const uint64_t stride_a[1] = {static_cast<uint64_t>(2 * n)}, stride_b[1] = {static_cast<uint64_t>(2 * k)};
+    if (int rc = encode_tiled(&map_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, grad, dims_a, stride_a, box_a,
                               CU_TENSOR_MAP_SWIZZLE_128B))
         return rc;
-    if (int rc = encode_tiled(&map_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, workspace, dims_b, stride, box,
+    if (int rc = encode_tiled(&map_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, workspace, dims_b, stride_b, box_b,
                               CU_TENSOR_MAP_SWIZZLE_128B))
         return rc;
     const void *kernel = fp4::grad_pair_kernel(rotation);
@@ -306,11 +346,16 @@ int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t 
     if (int rc = pair_clusters(g_grad_plan[rotation ? 1 : 0], kernel, fp4::grad_pair_threads(), fp4::grad_pair_smem(), q,
                                &clusters))
         return rc;
-    CTU_CUDA(fp4::launch_decode_transposed(d, s));
-    fp4::GradArgs args{dx, err, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), rotation};
+    CTU_CUDA(fp4::launch_dequantize(d, s));
+    const int split = static_cast<int>(grad_split(m, n, k));
+    fp4::GradArgs args{dx, reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + 2 * n * k), err,
+                       static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), rotation, split};
     void *params[] = {&map_a, &map_b, &args};
-    return launch_pairs(kernel, fp4::grad_pair_threads(), fp4::grad_pair_smem(), std::min<int64_t>(tiles, clusters),
-                        params, s);
+    if (int rc = launch_pairs(kernel, fp4::grad_pair_threads(), fp4::grad_pair_smem(),
+                              std::min<int64_t>(tiles * split, clusters), params, s))
+        return rc;
+    if (split > 1) CTU_CUDA(fp4::launch_grad_join(args, q.num_sms, s));
+    return CTU_OK;
 }
 
 // ---------------------------------------------------------------------------- affine layer norm

@@ -2,15 +2,21 @@
 //
 //   dx[m, k] = sum_n grad[m, n] * w[n, k],  then rotated back (the rotation is its own inverse)
 //
-// The weights arrive decoded to bf16 [k, n] (code * block scale has six significant bits, a
-// power-of-two channel scale adds none, so the decoding of this library's own weights is exact).
+// The weights arrive decoded to bf16 [n, k] (code * block scale has six significant bits, a
+// power-of-two channel scale adds none, so the decoding of this library's own weights is exact).  The
+// sum runs over their rows, so the MMA reads them with k as the contiguous dimension (MN-major B).
 // A pair of CTAs owns a 256 x 256 tile of dx; accumulators are fp32, and a rotation block of 256
 // columns lies inside one tile, so the rotation runs on the fp32 sums: an epilogue thread holds one
 // row and takes the strides 1, 4 and 16 in registers, 64 columns at a time, writes them back to
 // tensor memory, and takes stride 64 from there.  Rounded once, to bf16.
+//
+// With too few tiles to fill the GPU the sum over n is split; each part leaves fp32 sums, and a second
+// kernel adds them in order, rotates and rounds.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "fp4.cuh"
 #include "fp4_mma.cuh"
@@ -93,6 +99,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     fp4_grad_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const GradArgs args) {
     constexpr uint32_t kStageTx = 2 * (kABytes + kBBytes);
+    // B: 64 rows of n by 128 columns of k, as two pieces of 64 columns; eight rows 1024 bytes apart.
+    constexpr uint32_t kDescBHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+    constexpr uint32_t kDescBLow = (8192u >> 4) << 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Shared &S = *reinterpret_cast<Shared *>(smem + kStructOffset);
@@ -105,8 +114,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     const int num_pairs = gridDim.x >> 1;
     const int num_n = (args.k + kGradCols - 1) / kGradCols;
     const int num_m = (args.m + kPairRows - 1) / kPairRows;
-    const int num_tiles = num_m * num_n;
-    const int nk = (args.n + kStageK - 1) / kStageK;
+    const int num_tiles = num_m * num_n * args.split;
+    const int nk_all = (args.n + kStageK - 1) / kStageK;
+    // Work item t: part t % split of the sum of tile t / split, over stages [first, last).
+    auto work_item = [&](int t, int &m_tile, int &n_tile, int &part, int &first, int &last) {
+        part = t % args.split;
+        const int tile = t / args.split;
+        m_tile = tile / num_n;
+        n_tile = tile - m_tile * num_n;
+        first = static_cast<int>(static_cast<int64_t>(nk_all) * part / args.split);
+        last = static_cast<int>(static_cast<int64_t>(nk_all) * (part + 1) / args.split);
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -143,9 +161,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             uint32_t ph = 0;
             bool ok = true;
             for (int t = pair; t < num_tiles && ok; t += num_pairs) {
-                const int m0 = (t / num_n) * kPairRows + static_cast<int>(rank) * 128;
-                const int n0 = (t % num_n) * kGradCols + static_cast<int>(rank) * 128;
-                for (int kb = 0; kb < nk; ++kb) {
+                int m_tile, n_tile, part, first, last;
+                work_item(t, m_tile, n_tile, part, first, last);
+                const int m0 = m_tile * kPairRows + static_cast<int>(rank) * 128;
+                const int n0 = n_tile * kGradCols + static_cast<int>(rank) * 128;
+                for (int kb = first; kb < last; ++kb) {
                     if (!guard.wait(&S.empty[s], ph ^ 1u, kErrTimeoutEmpty)) {
                         ok = false;
                         break;
@@ -153,7 +173,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     const uint32_t full = mapa_shared(smem_u32(&S.full[s]), 0u);
                     if (leader) mbar_arrive_expect_tx(&S.full[s], kStageTx);
                     tma_load_2d_pair(smem + s * kABytes, &tmap_a, kb * kStageK, m0, full);
-                    tma_load_2d_pair(smem + kBOffset + s * kBBytes, &tmap_b, kb * kStageK, n0, full);
+                    tma_load_2d_pair(smem + kBOffset + s * kBBytes, &tmap_b, n0, kb * kStageK, full);
+                    tma_load_2d_pair(smem + kBOffset + s * kBBytes + 8192, &tmap_b, n0 + 64, kb * kStageK, full);
                     if (++s == kStages) {
                         s = 0;
                         ph ^= 1u;
@@ -163,43 +184,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             if (!ok || *abort_flag) settle_inflight_copies();
         }
     } else if (warp == 1) {
-        if (leader && lane == 0) {
-            constexpr uint32_t idesc = idesc_bf16(kPairRows, kGradCols);
+        if (leader) {
+            // Warp-uniform, one elected lane issues (see the 4-bit product).
+            constexpr uint32_t idesc = idesc_bf16(kPairRows, kGradCols) | (1u << 16);  // B is MN-major
             int s = 0;
             uint32_t ph = 0;
             int local = 0;
             bool ok = true;
+            const uint32_t a0 = smem_desc_low(smem_u32(smem));
+            const uint32_t b0 = ((smem_u32(smem + kBOffset) & 0x3FFFFu) >> 4) | kDescBLow;
+            const uint32_t empty0 = smem_u32(&S.empty[0]);
             for (int t = pair; t < num_tiles && ok; t += num_pairs, ++local) {
-                const int ab = local & 1;
-                if (!guard.wait_cluster(&S.acc_empty[ab], ((local >> 1) & 1) ^ 1u, kErrTimeoutAccumFree)) {
-                    ok = false;
-                    break;
-                }
+                int m_tile, n_tile, part, first, last;
+                work_item(t, m_tile, n_tile, part, first, last);
+                const uint32_t ab = local & 1;
+                ok = __all_sync(0xffffffffu, guard.wait_cluster(&S.acc_empty[ab], ((local >> 1) & 1) ^ 1u, kErrTimeoutAccumFree));
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + static_cast<uint32_t>(ab * kGradCols);
-                for (int kb = 0; kb < nk; ++kb) {
-                    if (!guard.wait(&S.full[s], ph, kErrTimeoutFull)) {
-                        ok = false;
-                        break;
-                    }
+                const uint32_t d = tmem_base + ab * kGradCols;
+                for (int kb = first; kb < last; ++kb) {
+                    ok = __all_sync(0xffffffffu, guard.wait(&S.full[s], ph, kErrTimeoutFull));
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = smem_u32(smem + s * kABytes);
-                    const uint32_t b = smem_u32(smem + kBOffset + s * kBBytes);
+                    const uint32_t a = a0 + s * (kABytes >> 4);
+                    const uint32_t b = b0 + s * (kBBytes >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int c = 0; c < kStageK / 16; ++c)
-                        mma_bf16_pair(d, smem_desc_sw128(a + 32 * c), smem_desc_sw128(b + 32 * c), idesc,
-                                      (kb | c) != 0 ? 1u : 0u);
-                    mma_commit_pair_both(&S.empty[s]);
+                        for (int c = 0; c < kStageK / 16; ++c)
+                            mma_bf16_pair(d, desc64(a + 2 * c, kDescSw128High), desc64(b + 128 * c, kDescBHigh), idesc,
+                                          (kb != first || c != 0) ? 1u : 0u);
+                        mma_commit_pair_both_at(empty0 + 8 * s);
+                        if (kb == last - 1) mma_commit_pair_both(&S.acc_full[ab]);
+                    }
+                    __syncwarp();
                     if (++s == kStages) {
                         s = 0;
                         ph ^= 1u;
                     }
                 }
-                if (!ok) break;
-                mma_commit_pair_both(&S.acc_full[ab]);
             }
-            mma_commit_pair_local(&S.drain);
-            mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+            if (elect_one()) {
+                mma_commit_pair_local(&S.drain);
+                mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+            }
+            __syncwarp();
         }
     } else {
         const int quad = warp & 3;
@@ -215,12 +243,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             }
             if (!alive) continue;
             tc_fence_after();
-            const int m = (t / num_n) * kPairRows + static_cast<int>(rank) * 128 + quad * 32 + lane;
-            const int n0 = (t % num_n) * kGradCols;
+            int m_tile, n_tile, part, first, last;
+            work_item(t, m_tile, n_tile, part, first, last);
+            const int m = m_tile * kPairRows + static_cast<int>(rank) * 128 + quad * 32 + lane;
+            const int n0 = n_tile * kGradCols;
             const bool row_ok = m < args.m;
             const uint32_t acc = tmem_base + static_cast<uint32_t>(ab * kGradCols) + (static_cast<uint32_t>(quad * 32) << 16);
             __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(args.out) + static_cast<int64_t>(m) * args.k + n0;
-            if constexpr (kRotate) {
+            if (args.split > 1) {
+                float *sums = args.partials + (static_cast<int64_t>(part) * args.m + m) * args.k + n0;
+#pragma unroll 1
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(acc + c * 32, r);
+                    tmem_ld_wait();
+                    if (row_ok && n0 + c * 32 < args.k) {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            reinterpret_cast<uint4 *>(sums + c * 32)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+                    }
+                }
+            } else if constexpr (kRotate) {
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t lo[32], hi[32];
@@ -286,6 +329,98 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, kTmemCols);
     }
+}
+
+// Four lanes to 256 columns (a rotation block): lane q holds columns 64 j + 16 q + i, so strides 1, 4 and
+// 64 are in registers and stride 16 is across the lanes.
+template <bool kRotate>
+__global__ void __launch_bounds__(128) grad_join_kernel(const GradArgs a) {
+    const int64_t quads = static_cast<int64_t>(a.m) * ((a.k + 255) / 256);
+    const int groups = (a.k + 255) / 256;
+    const int64_t part = static_cast<int64_t>(a.m) * a.k;
+    const int q = threadIdx.x & 3;
+    const int64_t total = (quads * 4 + 31) / 32 * 32;  // whole warps stay together
+    for (int64_t i = blockIdx.x * 128ll + threadIdx.x; i < total; i += gridDim.x * 128ll) {
+        const int64_t row = (i >> 2) / groups;
+        const int col = static_cast<int>((i >> 2) - row * groups) * 256;
+        const bool in = (i >> 2) < quads;
+        const float *src = a.partials + row * a.k + col;
+        __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + row * a.k + col;
+        if constexpr (kRotate) {
+            float v[4][16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // columns 64 j + 16 q + i
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (in) {
+                        for (int p = 0; p < a.split; ++p) {
+                            const float4 x = __ldcs(reinterpret_cast<const float4 *>(src + p * part + 64 * j + 16 * q + 4 * c));
+                            sum.x += x.x;
+                            sum.y += x.y;
+                            sum.z += x.z;
+                            sum.w += x.w;
+                        }
+                    }
+                    v[j][4 * c] = sum.x * 0.0625f;
+                    v[j][4 * c + 1] = sum.y * 0.0625f;
+                    v[j][4 * c + 2] = sum.z * 0.0625f;
+                    v[j][4 * c + 3] = sum.w * 0.0625f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t(&u)[16] = reinterpret_cast<uint32_t(&)[16]>(v[j]);
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) radix4(u[i], u[i + 1], u[i + 2], u[i + 3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) radix4(u[i], u[i + 4], u[i + 8], u[i + 12]);
+                // Stride 16: the four lanes hold the four digits; each computes its own output.
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int lead = (threadIdx.x & 31) & ~3;
+                    const float x0 = __shfl_sync(0xffffffffu, v[j][i], lead), x1 = __shfl_sync(0xffffffffu, v[j][i], lead + 1);
+                    const float x2 = __shfl_sync(0xffffffffu, v[j][i], lead + 2), x3 = __shfl_sync(0xffffffffu, v[j][i], lead + 3);
+                    const float t = x0 + x1, b = x0 - x1;
+                    v[j][i] = q == 0 ? (t + x2) - x3 : q == 1 ? (t - x2) + x3 : q == 2 ? (b + x2) + x3 : (x2 - b) + x3;
+                }
+            }
+            uint32_t(&u)[4][16] = reinterpret_cast<uint32_t(&)[4][16]>(v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) radix4(u[0][i], u[1][i], u[2][i], u[3][i]);
+            if (in) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) store_row16(dst + 64 * j + 16 * q, u[j]);
+            }
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+                if (!in || col + 64 * j + 16 * q >= a.k) continue;
+                float4 sum[4] = {};
+                for (int p = 0; p < a.split; ++p) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float4 x = __ldcs(reinterpret_cast<const float4 *>(src + p * part + 64 * j + 16 * q + 4 * c));
+                        sum[c].x += x.x;
+                        sum[c].y += x.y;
+                        sum[c].z += x.z;
+                        sum[c].w += x.w;
+                    }
+                }
+                store_row16(dst + 64 * j + 16 * q, reinterpret_cast<const uint32_t *>(sum));
+            }
+        }
+    }
+}
+
+cudaError_t launch_grad_join(const GradArgs &a, int num_sms, cudaStream_t stream) {
+    const int64_t threads = static_cast<int64_t>(a.m) * ((a.k + 255) / 256) * 4;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((threads + 127) / 128, num_sms * 16ll));
+    if (a.rotation)
+        grad_join_kernel<true><<<grid, 128, 0, stream>>>(a);
+    else
+        grad_join_kernel<false><<<grid, 128, 0, stream>>>(a);
+    return cudaGetLastError();
 }
 
 int grad_pair_smem() { return kSmem; }

@@ -1,13 +1,16 @@
 // Rows to 4-bit floating point with block scales, and back.
 //
-// One CTA takes a row: the values (rotated, if asked, in blocks of 256) stay in shared memory as
-// fp32 between the pass that finds the row's largest magnitude and the one that writes codes.
-//
 // Row scale (nvfp4): 2^ceil(log2(amax / 2688)), 2688 = 6 * 448, so that the largest block scale
 // lies in (224, 448]; a power of two keeps every division by it exact.  Block scale: nvfp4
 // e4m3(block amax / 6 / row scale); mxfp4 2^(floor(log2(block amax)) - 2), the OCP rule.  Code:
 // e2m1(v / block scale / row scale) to nearest, ties to even, saturating at 6.  A row that holds a
 // NaN or an infinity gets a NaN row scale and zero codes and block scales.
+//
+// Four lanes share 256 columns: lane q holds columns 64 j + 16 q .. + 15 for j = 0..3, so a block of 16
+// lies in one lane and a block of 32 in two.  A warp covers 2048 columns, or several short rows; a
+// longer row takes several warps, which meet once, for the row's largest magnitude.  Values stay in
+// registers from the load to the codes.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -16,33 +19,12 @@
 
 #include "../../include/ctu_b200.h"
 #include "fp4.cuh"
+#include "ptx.cuh"
 
 namespace ctu {
 namespace fp4 {
 
 namespace {
-
-constexpr int kThreads = 256;
-
-__device__ __forceinline__ float load_value(const void *x, int64_t i, int dtype) {
-    return dtype == CTU_DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(x)[i])
-                                   : __half2float(static_cast<const __half *>(x)[i]);
-}
-
-// Two values to one byte of e2m1 codes, `lo` in the low nibble.
-__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
-    uint32_t r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}"
-        : "=r"(r)
-        : "f"(lo), "f"(hi));
-    return r;
-}
-
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-    const uint32_t e = (code >> 1) & 3u, m = code & 1u;
-    const float v = e == 0 ? 0.5f * m : __uint_as_float(((e + 126u) << 23) | (m << 22));
-    return (code & 8u) ? -v : v;
-}
 
 __device__ __forceinline__ float block_scale_value(uint32_t byte, int format) {
     if (format == kNvfp4) {
@@ -60,83 +42,351 @@ __device__ __forceinline__ float pow2_row_scale(float amax) {
     return __uint_as_float(max(e, 1u) << 23);
 }
 
-template <int kFormat>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantArgs a) {
-    extern __shared__ float v[];
-    __shared__ float red[kThreads / 32];
-    constexpr int kBlock = block_of(kFormat);
-    const int k = a.k;
-    const int64_t col_tiles = scale_col_tiles(k, kFormat);
-    const int blocks = k / kBlock;
-    for (int64_t r = blockIdx.x; r < scale_row_tiles(a.rows) * 128; r += gridDim.x) {
-        if (r >= a.rows) {
-            for (int b = threadIdx.x; b < col_tiles * 4; b += kThreads)
-                a.block_scales[scale_offset(r, b, col_tiles)] = 0;
-            continue;
-        }
+// max(a, |b|, |c|); a NaN among them comes out as NaN.
+__device__ __forceinline__ float max_abs3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Eight values (four pairs) to a word of e2m1 codes, the first in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1x8(const f32x2 (&q)[4]) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpk2(q[i], v[2 * i], v[2 * i + 1]);
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+
+// Where a lane's columns are.  A team of lanes owns a row: some lanes of a warp, a warp, or the CTA.
+struct Place {
+    int64_t row;
+    int group;    // of 256 columns in the row
+    int q;        // lane of the group
+    bool active;  // the row and the group exist
+};
+
+// Largest magnitude over a row's team.  `span` lanes of a warp hold a row, or (kMulti) all warps do.
+template <bool kMulti>
+__device__ __forceinline__ float row_max(float amax, int span, float *red) {
+    if (kMulti) span = 32;
+    for (int o = 1; o < span; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (kMulti) {
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
         __syncthreads();
-        const float pre = a.rotation ? 0.0625f : 1.0f;
-        for (int c = threadIdx.x; c < k; c += kThreads) v[c] = __fmul_rn(load_value(a.x, r * k + c, a.dtype), pre);
-        __syncthreads();
-        if (a.rotation) {
-            for (int stride = 1; stride <= 64; stride *= 4) {
-                for (int q = threadIdx.x; q < k / 4; q += kThreads) {
-                    const int base = (q / stride) * stride * 4 + q % stride;
-                    const float x0 = v[base], x1 = v[base + stride], x2 = v[base + 2 * stride], x3 = v[base + 3 * stride];
-                    const float t = __fadd_rn(x0, x1), b = __fsub_rn(x0, x1);
-                    v[base] = __fsub_rn(__fadd_rn(t, x2), x3);
-                    v[base + stride] = __fadd_rn(__fsub_rn(t, x2), x3);
-                    v[base + 2 * stride] = __fadd_rn(__fadd_rn(b, x2), x3);
-                    v[base + 3 * stride] = __fadd_rn(__fsub_rn(x2, b), x3);
-                }
-                __syncthreads();
-            }
-        }
-        // Largest magnitude as an unsigned integer: infinities and NaN come out above all else.
-        uint32_t top = 0;
-        for (int c = threadIdx.x; c < k; c += kThreads) top = max(top, __float_as_uint(v[c]) & 0x7fffffffu);
-        top = __reduce_max_sync(0xffffffffu, top);
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(top);
-        __syncthreads();
-        for (int i = 0; i < kThreads / 32; ++i) top = max(top, __float_as_uint(red[i]));
-        const bool bad = top >= 0x7f800000u;
-        const float row = kFormat == kNvfp4 && !bad ? pow2_row_scale(__uint_as_float(top)) : 1.0f;
-        if (threadIdx.x == 0) a.row_scales[r] = bad ? __uint_as_float(0x7fc00000u) : row;
-        const float inv_row = 1.0f / row;
-        for (int b = threadIdx.x; b < col_tiles * 4; b += kThreads) {
-            uint32_t scale_byte = 0;
-            if (b < blocks) {
-                uint32_t *out = reinterpret_cast<uint32_t *>(a.codes + r * (k / 2) + b * (kBlock / 2));
-                if (bad) {
-                    for (int i = 0; i < kBlock / 8; ++i) out[i] = 0;
-                } else {
-                    float amax = 0.0f;
-                    for (int i = 0; i < kBlock; ++i) amax = fmaxf(amax, fabsf(v[b * kBlock + i]));
-                    float divisor;
-                    if (kFormat == kNvfp4) {
-                        scale_byte = __nv_cvt_float_to_fp8(__fdiv_rn(amax * inv_row, 6.0f), __NV_SATFINITE, __NV_E4M3);
-                        divisor = block_scale_value(scale_byte, kFormat);
-                    } else {
-                        const uint32_t e = __float_as_uint(amax) >> 23;
-                        scale_byte = e > 2 ? e - 2 : 0;
-                        divisor = block_scale_value(scale_byte, kFormat);
-                    }
-                    for (int i = 0; i < kBlock / 8; ++i) {
-                        uint32_t word = 0;
-                        for (int j = 0; j < 4; ++j) {
-                            const float x0 = v[b * kBlock + 8 * i + 2 * j] * inv_row;
-                            const float x1 = v[b * kBlock + 8 * i + 2 * j + 1] * inv_row;
-                            const float q0 = divisor == 0.0f ? copysignf(0.0f, x0) : __fdiv_rn(x0, divisor);
-                            const float q1 = divisor == 0.0f ? copysignf(0.0f, x1) : __fdiv_rn(x1, divisor);
-                            word |= e2m1x2(q0, q1) << (8 * j);
-                        }
-                        out[i] = word;
-                    }
-                }
-            }
-            a.block_scales[scale_offset(r, b, col_tiles)] = static_cast<uint8_t>(scale_byte);
-        }
+        amax = red[0];
+        for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) amax = max_nan(amax, red[w]);
     }
+    return amax;
+}
+
+// Codes and scales of one lane's four blocks of 16; pair(j, p) is columns 2p, 2p + 1 of block j and
+// amax[j] its largest magnitude.
+template <int kFormat, bool kMulti, typename Pair>
+__device__ __forceinline__ void finish(const QuantArgs &a, const Place &at, float (&amax)[4], int span, float *red,
+                                       Pair pair) {
+    float row_amax = max_nan(max_nan(amax[0], amax[1]), max_nan(amax[2], amax[3]));
+    row_amax = row_max<kMulti>(at.active ? row_amax : 0.0f, span, red);
+    const bool bad = !(row_amax <= 3.402823466e38f);
+    float row = 1.0f;
+    if (kFormat == kNvfp4 && !bad) row = pow2_row_scale(row_amax);
+    if (kFormat == kMxfp4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax[j] = fmaxf(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], 1));
+    }
+    const float inv_row = 1.0f / row;
+    if (at.active && at.group == 0 && at.q == 0) a.row_scales[at.row] = bad ? __uint_as_float(0x7fc00000u) : row;
+
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int col = at.group * 256 + j * 64 + at.q * 16;
+        const bool in = at.active && col < a.k;
+        uint32_t byte = 0;
+        uint32_t word[2] = {0u, 0u};
+        if (!bad && in) {
+            if (kFormat == kNvfp4) {
+                byte = __nv_cvt_float_to_fp8(__fdiv_rn(amax[j] * inv_row, 6.0f), __NV_SATFINITE, __NV_E4M3);
+                const float s = block_scale_value(byte, kNvfp4);
+                // v / s rounded to nearest: a product with the reciprocal and one correction by its
+                // exact remainder (Markstein), so that ties of the code grid stay ties.  The signs are
+                // placed so that a zero keeps its own; a zero scale leaves such zeros.
+                const float inv = s == 0.0f ? 0.0f : __frcp_rn(s);
+                const f32x2 minus_inv = pk2(-inv, -inv), s2 = pk2(s, s), minus_row = pk2(-inv_row, -inv_row);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f32x2 q[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x2 minus_v = fmul2(pair(j, 4 * h + i), minus_row);
+                        const f32x2 q0 = fmul2(minus_v, minus_inv);
+                        q[i] = ffma2(ffma2(q0, s2, minus_v), minus_inv, q0);
+                    }
+                    word[h] = e2m1x8(q);
+                }
+            } else {
+                const uint32_t e = __float_as_uint(amax[j]) >> 23;
+                byte = e > 2 ? e - 2 : 0;
+                const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte), exact
+                const f32x2 inv2 = pk2(inv, inv);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f32x2 q[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) q[i] = fmul2(pair(j, 4 * h + i), inv2);
+                    word[h] = e2m1x8(q);
+                }
+            }
+        }
+        bytes |= byte << (8 * j);
+        if (in) *reinterpret_cast<uint2 *>(a.codes + at.row * (a.k / 2) + col / 2) = make_uint2(word[0], word[1]);
+    }
+    // The group's scale bytes to whole words of its tiles: a byte transpose among the four lanes.
+    const int64_t col_tiles = scale_col_tiles(a.k, kFormat);
+    uint32_t word;
+    int64_t tile;
+    if (kFormat == kNvfp4) {
+        uint32_t p = __shfl_xor_sync(0xffffffffu, bytes, 1);
+        bytes = __byte_perm(bytes, p, (at.q & 1) ? 0x3715 : 0x6240);
+        p = __shfl_xor_sync(0xffffffffu, bytes, 2);
+        word = __byte_perm(bytes, p, (at.q & 2) ? 0x3276 : 0x5410);
+        tile = at.group * 4 + at.q;
+    } else {
+        const uint32_t p = __shfl_xor_sync(0xffffffffu, bytes, 2);
+        word = __byte_perm(bytes, p, (at.q & 1) ? 0x7362 : 0x5140);
+        tile = at.q < 2 ? at.group * 2 + at.q : col_tiles;
+    }
+    if (at.active && tile < col_tiles)
+        *reinterpret_cast<uint32_t *>(a.block_scales + ((at.row >> 7) * col_tiles + tile) * 512 + (at.row & 31) * 16 +
+                                      ((at.row >> 5) & 3) * 4) = word;
+}
+
+// Scale bytes of the last tile's rows beyond the matrix.
+__device__ __forceinline__ void clear_padding(const QuantArgs &a, int format) {
+    const int col_tiles = static_cast<int>(scale_col_tiles(a.k, format));
+    const int first = static_cast<int>(a.rows & 127);
+    if (first == 0) return;
+    uint32_t *tiles = reinterpret_cast<uint32_t *>(a.block_scales) + (a.rows >> 7) * col_tiles * 128;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < col_tiles * 128; i += gridDim.x * blockDim.x) {
+        const int word = i & 127;  // row 32 (word & 3) + word / 4 of the tile
+        if (32 * (word & 3) + (word >> 2) >= first) tiles[i] = 0u;
+    }
+}
+
+template <bool kHalf>
+__device__ __forceinline__ float low_value(uint32_t w) {
+    return kHalf ? __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xffffu))) : bf16lo(w);
+}
+template <bool kHalf>
+__device__ __forceinline__ float high_value(uint32_t w) {
+    return kHalf ? __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16))) : bf16hi(w);
+}
+
+// Without rotation: loads go straight to registers, and magnitudes are compared as 16-bit integers,
+// where infinities and NaN rank above every finite value.
+template <int kFormat, bool kHalf, bool kMulti>
+__global__ void __launch_bounds__(kMulti ? 768 : 128) quantize_kernel(const QuantArgs a) {
+    __shared__ float red[2][24];
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    const int slots = a.rows_per_warp;  // rows side by side in a warp
+    const int span = 32 / slots;
+    const int64_t teams = kMulti ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4;
+    const int64_t team = kMulti ? blockIdx.x : blockIdx.x * 4ll + warp;
+    Place at;
+    at.q = lane & 3;
+    at.group = kMulti ? warp * 8 + (lane >> 2) : (lane % span) >> 2;
+    int flip = 0;
+    for (int64_t r0 = team * slots; r0 < a.rows; r0 += teams * slots, flip ^= 1) {
+        at.row = r0 + (kMulti ? 0 : lane / span);
+        at.active = at.row < a.rows && at.group * 256 < a.k;
+        uint4 w[4][2];
+        float amax[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int col = at.group * 256 + j * 64 + at.q * 16;
+            w[j][0] = w[j][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (at.active && col < a.k) {
+                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.x) + at.row * a.k + col);
+                w[j][0] = __ldcs(src);
+                w[j][1] = __ldcs(src + 1);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t *p = &w[j][0].x;
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = __vmaxu2(m, p[i] & 0x7fff7fffu);
+            m = max(m & 0xffffu, m >> 16);
+            if (kHalf)
+                amax[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+            else
+                amax[j] = __uint_as_float(m << 16);
+        }
+        finish<kFormat, kMulti>(a, at, amax, span, red[flip], [&](int j, int p) {
+            const uint32_t v = (&w[j][0].x)[p];
+            return pk2(low_value<kHalf>(v), high_value<kHalf>(v));
+        });
+    }
+    clear_padding(a, kFormat);
+}
+
+// Radix-4 butterfly of two tuples at once, in the rotation's order of sums; halvings are taken before
+// the first stage (exact: a 16-bit input over 16 is a fp32 value).
+__device__ __forceinline__ void radix4_pair(f32x2 &x0, f32x2 &x1, f32x2 &x2, f32x2 &x3) {
+    const f32x2 t = fadd2(x0, x1), b = fsub2(x0, x1);
+    x0 = fsub2(fadd2(t, x2), x3);
+    x1 = fadd2(fsub2(t, x2), x3);
+    const f32x2 y2 = fadd2(fadd2(b, x2), x3);
+    x3 = fadd2(fsub2(x2, b), x3);
+    x2 = y2;
+}
+
+// With rotation.  A warp's 2048 columns arrive by tile loads (128-byte swizzle) in 4 KB of its 8 KB of
+// shared memory.  A lane first holds 64 columns in a row (lane q: 64 q ..) and takes the strides 1, 4
+// and 16 in registers, two tuples to an instruction where the pairing allows; then the four lanes
+// exchange 16-column pieces through the same 8 KB, and stride 64 is in registers too, with whole blocks
+// of 16 left in each lane.  The next row's load runs under the codes of this one.
+template <int kFormat, bool kHalf, bool kMulti, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads)
+    rotate_quantize_kernel(const __grid_constant__ CUtensorMap tmap, const QuantArgs a) {
+    __shared__ float red[2][24];
+    __shared__ uint64_t bars[24];
+    extern __shared__ uint8_t smem_raw[];
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)) + warp * 8192;
+    const uint32_t base = smem_u32(smem);
+    uint64_t *bar = &bars[warp];
+    const int slots = a.rows_per_warp;
+    const int span = 32 / slots;
+    const int groups = a.k / 256;
+    const int64_t teams = kMulti ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4;
+    const int64_t team = kMulti ? blockIdx.x : blockIdx.x * 4ll + warp;
+    Place at;
+    at.q = lane & 3;
+    at.group = kMulti ? warp * 8 + (lane >> 2) : (lane % span) >> 2;
+    // Copies of `load_groups` groups each: this warp's part of a row, or several whole rows.
+    const int mine = kMulti ? min(8, groups - warp * 8) : slots > 1 ? 8 : groups;
+    const int copies = (mine + a.load_groups - 1) / a.load_groups;
+    auto load = [&](int64_t r0) {  // lane 0
+        mbar_arrive_expect_tx(bar, static_cast<uint32_t>(copies * a.load_groups * 512));
+        const int64_t line = r0 * (a.k / 64) + (kMulti ? warp * 32 : 0);
+        for (int c = 0; c < copies; ++c)
+            tma_load_2d(smem + c * a.load_groups * 512, &tmap, 0, static_cast<int>(line + c * a.load_groups * 4), bar);
+    };
+    if (lane == 0) {
+        mbar_init(bar, 1);
+        fence_mbar_init();
+        if (team * slots < a.rows) load(team * slots);
+    }
+    __syncwarp();
+    // 16-byte chunk c of (column digit d3, d2) of this lane's group in the exchange: the address bits are
+    // mixed so that eight lanes of a store or load touch eight different 16-byte banks.
+    const uint32_t area = base + (lane >> 2) * 1024u;
+    const uint32_t gp = ((lane >> 2) & 1) * 4u;
+    auto chunk = [&](uint32_t d3, uint32_t d2, uint32_t c) {
+        const uint32_t low = c ^ gp ^ d3 ^ ((d2 & 1u) * 5u) ^ (d2 & 2u);
+        return area + ((d3 * 16u + (d2 >> 1) * 8u + low) << 4);
+    };
+    uint32_t phase = 0;
+    int flip = 0;
+    for (int64_t r0 = team * slots; r0 < a.rows; r0 += teams * slots, flip ^= 1) {
+        at.row = r0 + (kMulti ? 0 : lane / span);
+        at.active = at.row < a.rows && at.group < groups;
+        mbar_wait(bar, phase, nullptr, a.err, kErrTimeoutFull);
+        phase ^= 1u;
+        __syncwarp();
+        // x[h][i]: column 16 h + i in the low half, 16 (h + 2) + i in the high half.
+        f32x2 x[2][16];
+        {
+            const uint32_t line = static_cast<uint32_t>(lane);
+            const f32x2 pre = pk2(0.0625f, 0.0625f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint4 lo = *reinterpret_cast<const uint4 *>(smem + line * 128 + (((2 * h + half) ^ (line & 7)) << 4));
+                    const uint4 hi = *reinterpret_cast<const uint4 *>(smem + line * 128 + (((2 * h + 4 + half) ^ (line & 7)) << 4));
+                    const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, u[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[h][8 * half + 2 * i] = fmul2(pk2(low_value<kHalf>(l[i]), low_value<kHalf>(u[i])), pre);
+                        x[h][8 * half + 2 * i + 1] = fmul2(pk2(high_value<kHalf>(l[i]), high_value<kHalf>(u[i])), pre);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) radix4_pair(x[h][i], x[h][i + 1], x[h][i + 2], x[h][i + 3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) radix4_pair(x[h][i], x[h][i + 4], x[h][i + 8], x[h][i + 12]);
+        }
+        __syncwarp();  // the load's bytes are in registers everywhere
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float o[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float x0, x1, x2, x3;
+                unpk2(x[0][4 * c + i], x0, x2);
+                unpk2(x[1][4 * c + i], x1, x3);
+                const float t = __fadd_rn(x0, x1), b = __fsub_rn(x0, x1);
+                o[0][i] = __fsub_rn(__fadd_rn(t, x2), x3);
+                o[1][i] = __fadd_rn(__fsub_rn(t, x2), x3);
+                o[2][i] = __fadd_rn(__fadd_rn(b, x2), x3);
+                o[3][i] = __fadd_rn(__fsub_rn(x2, b), x3);
+            }
+#pragma unroll
+            for (uint32_t d2 = 0; d2 < 4; ++d2)
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(chunk(at.q, d2, c)), "f"(o[d2][0]),
+                             "f"(o[d2][1]), "f"(o[d2][2]), "f"(o[d2][3])
+                             : "memory");
+        }
+        __syncwarp();
+        f32x2 v[4][8];
+#pragma unroll
+        for (uint32_t d3 = 0; d3 < 4; ++d3) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
+                             : "=l"(v[d3][2 * c]), "=l"(v[d3][2 * c + 1])
+                             : "r"(chunk(d3, at.q, c))
+                             : "memory");
+        }
+        fence_proxy_async_smem();  // the exchange is over before the next load writes here
+        __syncwarp();
+        if (lane == 0 && r0 + teams * slots < a.rows) load(r0 + teams * slots);
+        float amax[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            radix4_pair(v[0][p], v[1][p], v[2][p], v[3][p]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float lo, hi;
+                unpk2(v[j][p], lo, hi);
+                amax[j] = max_abs3_nan(amax[j], lo, hi);
+            }
+        }
+        finish<kFormat, kMulti>(a, at, amax, span, red[flip], [&](int j, int p) { return v[j][p]; });
+    }
+    clear_padding(a, kFormat);
 }
 
 template <typename T>
@@ -148,68 +398,114 @@ __device__ __forceinline__ __nv_bfloat16 store_as(float v) { return __float2bflo
 template <>
 __device__ __forceinline__ __half store_as(float v) { return __float2half_rn(v); }
 
-template <int kFormat, typename T>
-__global__ void __launch_bounds__(256) dequantize_kernel(const DequantArgs a) {
-    const int64_t half = a.k / 2;
-    const int64_t col_tiles = scale_col_tiles(a.k, kFormat);
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.rows * half; i += gridDim.x * 256ll) {
-        const int64_t r = i / half;
-        const int c = static_cast<int>(i - r * half) * 2;
-        const float s = block_scale_value(a.block_scales[scale_offset(r, c / block_of(kFormat), col_tiles)], kFormat);
-        const float rs = a.row_scales[a.row_scale_count == 1 ? 0 : r];
-        const uint32_t byte = a.codes[i];
-        T *out = static_cast<T *>(a.out) + r * a.k + c;
-        out[0] = store_as<T>(e2m1_value(byte & 15u) * s * rs);
-        out[1] = store_as<T>(e2m1_value(byte >> 4) * s * rs);
-    }
+// Four bytes of codes to four pairs of fp16, exact.
+__device__ __forceinline__ void decode8(uint32_t w, __half2 (&h)[4]) {
+    uint32_t r[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+        : "r"(w));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2 *>(&r[i]);
 }
 
-// 32 x 32 tiles through shared memory: reads run along k, writes along n.
-template <int kFormat>
-__global__ void __launch_bounds__(256) decode_transposed_kernel(const DequantArgs a) {
-    __shared__ float tile[32][33];
-    const int64_t n0 = blockIdx.y * 32ll;
-    const int k0 = blockIdx.x * 32;
+// A warp takes 256 columns of a row at a time, eight to a lane, four such pieces in flight.  code * block
+// scale is exact in fp32; the row scale rounds there unless it is a power of two.
+template <int kFormat, typename T>
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantArgs a) {
+    constexpr int kPieces = 4;
+    const int lane = threadIdx.x & 31;
+    const int segs = (a.k + 255) / 256;
+    const int64_t total = a.rows * segs;
     const int64_t col_tiles = scale_col_tiles(a.k, kFormat);
-    for (int i = threadIdx.x; i < 32 * 16; i += 256) {
-        const int64_t r = n0 + i / 16;
-        const int c = k0 + 2 * (i % 16);
-        float v0 = 0.0f, v1 = 0.0f;
-        if (r < a.rows && c < a.k) {
-            const uint32_t byte = a.codes[r * (a.k / 2) + c / 2];
-            const float s = block_scale_value(a.block_scales[scale_offset(r, c / block_of(kFormat), col_tiles)], kFormat);
-            const float rs = a.row_scales[a.row_scale_count == 1 ? 0 : r];
-            v0 = e2m1_value(byte & 15u) * s * rs;
-            v1 = e2m1_value(byte >> 4) * s * rs;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
+    for (int64_t i0 = blockIdx.x * 8ll + (threadIdx.x >> 5); i0 < total; i0 += warps * kPieces) {
+        uint32_t w[kPieces];
+        uint32_t byte[kPieces];
+        float row[kPieces];
+        int64_t at[kPieces];
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            const int64_t i = i0 + p * warps;
+            const int64_t r = i / segs;
+            const int c = static_cast<int>(i - r * segs) * 256 + 8 * lane;
+            const bool in = i < total && c < a.k;
+            at[p] = in ? r * a.k + c : -1;
+            if (in) {
+                w[p] = __ldcs(reinterpret_cast<const uint32_t *>(a.codes + at[p] / 2));
+                byte[p] = a.block_scales[scale_offset(r, c / block_of(kFormat), col_tiles)];
+                row[p] = a.row_scales[a.row_scale_count == 1 ? 0 : r];
+            }
         }
-        tile[i / 16][2 * (i % 16)] = v0;
-        tile[i / 16][2 * (i % 16) + 1] = v1;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * 32; i += 256) {
-        const int c = k0 + i / 32;
-        const int64_t r = n0 + i % 32;
-        if (c < a.k && r < a.rows)
-            static_cast<__nv_bfloat16 *>(a.out)[c * a.rows + r] = __float2bfloat16_rn(tile[i % 32][i / 32]);
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            if (at[p] < 0) continue;
+            const float s = block_scale_value(byte[p], kFormat);
+            __half2 h[4];
+            decode8(w[p], h);
+            T out[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float2 v = __half22float2(h[q]);
+                out[2 * q] = store_as<T>(v.x * s * row[p]);
+                out[2 * q + 1] = store_as<T>(v.y * s * row[p]);
+            }
+            uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + at[p]);
+#pragma unroll
+            for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) dst[q] = reinterpret_cast<const uint4 *>(out)[q];
+        }
     }
 }
 
 }  // namespace
 
-cudaError_t launch_quantize(const QuantArgs &a, cudaStream_t stream) {
-    const int smem = a.k * static_cast<int>(sizeof(float));
-    const unsigned grid =
-        static_cast<unsigned>(std::min<int64_t>(scale_row_tiles(a.rows) * 128, static_cast<int64_t>(a.num_sms) * 8));
-    auto kernel = a.format == kNvfp4 ? quantize_kernel<kNvfp4> : quantize_kernel<kMxfp4>;
+namespace {
+
+template <int kFormat, bool kHalf>
+cudaError_t quantize_as(const QuantArgs &a, const CUtensorMap &map, cudaStream_t stream) {
+    const int groups = (a.k + 255) / 256;
+    const bool multi = groups > 8;
+    const int warps = multi ? (groups + 7) / 8 : 4;
+    int64_t rows = multi ? a.rows : (a.rows + 4 * a.rows_per_warp - 1) / (4 * a.rows_per_warp);
+    // Enough CTAs to clear the last tile's padding at once, however few rows there are.
+    if (a.rows & 127) rows = std::max<int64_t>(rows, (scale_col_tiles(a.k, kFormat) * 128 + warps * 32 - 1) / (warps * 32));
+    if (a.rotation == 0) {
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows, a.num_sms * static_cast<int64_t>(64 / warps)));
+        if (multi)
+            quantize_kernel<kFormat, kHalf, true><<<grid, warps * 32, 0, stream>>>(a);
+        else
+            quantize_kernel<kFormat, kHalf, false><<<grid, warps * 32, 0, stream>>>(a);
+        return cudaGetLastError();
+    }
+    const int smem = warps * 8192 + 1024;
+    auto kernel = !multi        ? rotate_quantize_kernel<kFormat, kHalf, false, 128>
+                  : warps <= 16 ? rotate_quantize_kernel<kFormat, kHalf, true, 512>
+                                : rotate_quantize_kernel<kFormat, kHalf, true, 768>;
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
-    kernel<<<grid, kThreads, smem, stream>>>(a);
+    int per_sm = 0;
+    if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, warps * 32, smem)) return e;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows, a.num_sms * static_cast<int64_t>(std::max(1, per_sm))));
+    kernel<<<grid, warps * 32, smem, stream>>>(map, a);
     return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_quantize(const QuantArgs &a, const CUtensorMap &map, cudaStream_t stream) {
+    const bool half = a.dtype == CTU_DTYPE_FP16;
+    if (a.format == kNvfp4)
+        return half ? quantize_as<kNvfp4, true>(a, map, stream) : quantize_as<kNvfp4, false>(a, map, stream);
+    return half ? quantize_as<kMxfp4, true>(a, map, stream) : quantize_as<kMxfp4, false>(a, map, stream);
 }
 
 template <typename T>
 static cudaError_t dequantize_as(const DequantArgs &a, cudaStream_t stream) {
     const unsigned grid = static_cast<unsigned>(
-        std::min<int64_t>((a.rows * (a.k / 2) + 255) / 256, static_cast<int64_t>(a.num_sms) * 16));
+        std::min<int64_t>((a.rows * ((a.k + 255) / 256) + 7) / 8, static_cast<int64_t>(a.num_sms) * 8));
     if (a.format == kNvfp4)
         dequantize_kernel<kNvfp4, T><<<grid, 256, 0, stream>>>(a);
     else
@@ -221,15 +517,6 @@ cudaError_t launch_dequantize(const DequantArgs &a, cudaStream_t stream) {
     if (a.dtype == CTU_DTYPE_BF16) return dequantize_as<__nv_bfloat16>(a, stream);
     if (a.dtype == CTU_DTYPE_FP16) return dequantize_as<__half>(a, stream);
     return dequantize_as<float>(a, stream);
-}
-
-cudaError_t launch_decode_transposed(const DequantArgs &a, cudaStream_t stream) {
-    const dim3 grid((a.k + 31) / 32, static_cast<unsigned>((a.rows + 31) / 32));
-    if (a.format == kNvfp4)
-        decode_transposed_kernel<kNvfp4><<<grid, 256, 0, stream>>>(a);
-    else
-        decode_transposed_kernel<kMxfp4><<<grid, 256, 0, stream>>>(a);
-    return cudaGetLastError();
 }
 
 }  // namespace fp4

@@ -344,7 +344,8 @@ CTU_API int64_t ctu_fp4_block_scale_bytes(int64_t rows, int64_t k, int format);
 CTU_API int ctu_fp4_quantize(const void *x, int64_t rows, int64_t k, int dtype, int format, int rotation,
                              uint8_t *codes, uint8_t *block_scales, float *row_scales, void *stream);
 
-/* The values back, rounded once to dtype (CTU_DTYPE_*).  row_scales: one, or one per row. */
+/* The values back, (code * block scale) * row scale in fp32, rounded to dtype (CTU_DTYPE_*).
+ * row_scales: one, or one per row. */
 CTU_API int ctu_fp4_dequantize(const uint8_t *codes, const uint8_t *block_scales, const float *row_scales,
                                int64_t row_scale_count, int64_t rows, int64_t k, int format, int dtype, void *out,
                                void *stream);
@@ -364,11 +365,12 @@ CTU_API int ctu_debug_set_fp4_kernel(int which);
 
 /*
  * dx[m, k] = grad[m, n] w[n, k], rotated back when rotation is 256 (the rotation is its own inverse);
- * grad and dx bf16, n a multiple of 8.  The weights are decoded to bf16 in the workspace
- * (ctu_fp4_grad_workspace_bytes), which is exact for power-of-two channel scales and rounds once for
- * others; sums and the rotation are fp32.
+ * grad and dx bf16, n a multiple of 8.  The workspace
+ * (ctu_fp4_grad_workspace_bytes, 16-byte aligned) takes the weights decoded to bf16, exact for
+ * power-of-two channel scales and rounded for others, and, for few rows, fp32 partial sums; sums and the
+ * rotation are fp32.
  */
-CTU_API int64_t ctu_fp4_grad_workspace_bytes(int64_t n, int64_t k);
+CTU_API int64_t ctu_fp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k);
 CTU_API int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t *w_block_scales,
                                       const float *w_scale, int64_t w_scale_count, int rotation, void *workspace,
                                       void *dx, int64_t m, int64_t n, int64_t k, int format, void *stream);
