@@ -896,7 +896,7 @@ def _norm_vector(t, hidden, input, name):
         return None
     if t.device != input.device or t.numel() != hidden or t.dtype not in (input.dtype, torch.float32):
         raise RuntimeError(f"LayerNorm {name} must be [hidden] on the input's device, of its type or float32")
-    return t.contiguous()
+    return _dense(t)
 
 
 def _norm_checks(input, weight, bias):
@@ -917,7 +917,7 @@ def layer_norm(input, weight=None, bias=None, epsilon=1.0e-5):
     hidden, weight, bias, wtype = _norm_checks(input, weight, bias)
     if not (math.isfinite(epsilon) and epsilon > 0.0):
         raise RuntimeError("LayerNorm epsilon must be finite and positive")
-    x = input.contiguous()
+    x = _dense(input)
     rows = x.numel() // hidden
     out = torch.empty_like(x)
     mean = torch.empty(rows, dtype=torch.float32, device=x.device)
@@ -933,7 +933,7 @@ def layer_norm_backward(grad_output, input, mean, rstd, weight=None, bias=None, 
     hidden, weight, bias, wtype = _norm_checks(input, weight, bias)
     if grad_output.shape != input.shape or grad_output.dtype != input.dtype or grad_output.device != input.device:
         raise RuntimeError("LayerNorm gradient must match the input's shape, type and device")
-    x, g = input.contiguous(), grad_output.contiguous()
+    x, g = _dense(input), _dense(grad_output)
     rows = x.numel() // hidden
     for t in (mean, rstd):
         if t.dtype != torch.float32 or t.device != x.device or t.numel() != rows or not t.is_contiguous():

@@ -7,13 +7,23 @@
 //   dw   = sum over rows of dy * xhat,   db = sum over rows of dy
 //
 // Statistics, sums and gradients are fp32 whatever the storage type; each result is rounded once.
+//
+// All passes are bound by memory: a team of lanes (a warp, or several with a named barrier) keeps a row
+// in registers, as loaded, from its load to the result, so x (and dy) are read once; arithmetic is on
+// packed fp32 pairs.  In the backward pass a thread keeps the same columns for every row its team takes
+// and holds their sums of dw and db in registers; one CTA an SM leaves one partial sum per column, joined
+// in order by a second kernel (equal shapes add in equal order).  Rows wider than a team holds take the
+// looping kernels at the end.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cstdint>
+#include <type_traits>
 
 #include "../../include/ctu_b200.h"
 #include "layer_norm.cuh"
+#include "ptx.cuh"
 
 namespace ctu {
 namespace norm {
@@ -38,7 +48,296 @@ __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat
 template <>
 __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of the looping kernels
+constexpr int kSlices = 148;   // CTAs of the backward pass: one an SM of a B200
+constexpr int kForwardBlock = 512;
+constexpr int kBackwardBlock = 384;  // times 168 registers: an SM's register file
+
+// A thread's part of a row: kPieces loads of kVec elements (16 bytes), or of single elements where rows
+// do not start on 16 bytes.  Elements are handled in pairs; a group is the pairs that share a load (or
+// two single loads).
+template <typename T, int kVec, int kPieces>
+struct Part {
+    static constexpr bool kWide = kVec > 1;
+    static constexpr int kGroups = kWide ? kPieces : kPieces / 2;
+    static constexpr int kPairs = kWide ? kVec / 2 : 1;  // of a group
+    uint4 wide[kWide ? kPieces : 1];
+    T single[kWide ? 1 : kPieces];
+
+    static __device__ __forceinline__ int column(int piece) { return (threadIdx.x + piece * blockDim.x) * kVec; }
+    // Whether a group's first element (all of them, with wide loads) and second element exist.
+    static __device__ __forceinline__ bool first(int g, int h) { return column(kWide ? g : 2 * g) < h; }
+    static __device__ __forceinline__ bool second(int g, int h) { return column(kWide ? g : 2 * g + 1) < h; }
+
+    // What does not exist reads as zero.
+    __device__ __forceinline__ void load(const T *row, int h) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            const int c = column(p);
+            if constexpr (kWide)
+                wide[p] = c < h ? __ldcs(reinterpret_cast<const uint4 *>(row + c)) : make_uint4(0u, 0u, 0u, 0u);
+            else
+                single[p] = c < h ? row[c] : from_f<T>(0.0f);
+        }
+    }
+    __device__ __forceinline__ f32x2 pair(int g, int i) const {
+        if constexpr (!kWide) return pk2(to_f(single[2 * g]), to_f(single[2 * g + 1]));
+        const uint32_t w[4] = {wide[g].x, wide[g].y, wide[g].z, wide[g].w};
+        if constexpr (sizeof(T) == 4) return pk2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return pk2(bf16lo(w[i]), bf16hi(w[i]));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        return pk2(f.x, f.y);
+    }
+    // One group of results.
+    static __device__ __forceinline__ void store(T *row, int g, int h, const f32x2 (&v)[kPairs]) {
+        float e[2 * kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) unpk2(v[i], e[2 * i], e[2 * i + 1]);
+        if constexpr (kWide) {
+            alignas(16) T out[kVec];
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) out[i] = from_f<T>(e[i]);
+            *reinterpret_cast<uint4 *>(row + column(g)) = *reinterpret_cast<const uint4 *>(out);
+        } else {
+            row[column(2 * g)] = from_f<T>(e[0]);
+            if (second(g, h)) row[column(2 * g + 1)] = from_f<T>(e[1]);
+        }
+    }
+    // One group of weights (of the input's type or fp32), `fill` where there are none.
+    static __device__ __forceinline__ void weights(const void *p, bool fp32, int g, int h, float fill, f32x2 (&out)[kPairs]) {
+        if (p == nullptr) {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) out[i] = pk2(fill, fill);
+        } else if constexpr (!kWide) {
+            const int c0 = column(2 * g), c1 = column(2 * g + 1);
+            const bool two = second(g, h);
+            if (fp32)
+                out[0] = pk2(static_cast<const float *>(p)[c0], two ? static_cast<const float *>(p)[c1] : 0.0f);
+            else
+                out[0] = pk2(to_f(static_cast<const T *>(p)[c0]), two ? to_f(static_cast<const T *>(p)[c1]) : 0.0f);
+        } else if (fp32) {
+            const ulonglong2 *f = reinterpret_cast<const ulonglong2 *>(static_cast<const float *>(p) + column(g));
+#pragma unroll
+            for (int i = 0; i < kPairs / 2; ++i) {
+                const ulonglong2 u = __ldg(f + i);
+                out[2 * i] = u.x;
+                out[2 * i + 1] = u.y;
+            }
+        } else {
+            Part one;
+            one.wide[0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p) + column(g)));
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) out[i] = one.pair(0, i);
+        }
+    }
+};
+
+// Sum of two values over a team of `warps` warps, in every thread, in a fixed order.  Two buffers in
+// turn: a team's threads are past a buffer's last reads when its barrier after next is passed.
+struct TeamSum {
+    float2 (*part)[16];  // [2][16] of this team
+    int warps;
+    int barrier;
+    int flip = 0;
+
+    __device__ __forceinline__ float2 operator()(float2 v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        }
+        if (warps == 1) return v;
+        float2 *buf = part[flip];
+        flip ^= 1;
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0) buf[warp] = v;
+        asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+        v = buf[0];
+        for (int i = 1; i < warps; ++i) {
+            v.x += buf[i].x;
+            v.y += buf[i].y;
+        }
+        return v;
+    }
+};
+
+__device__ __forceinline__ float both(f32x2 v) {
+    float lo, hi;
+    unpk2(v, lo, hi);
+    return lo + hi;
+}
+
+// blockDim = (threads of a team, teams).
+template <typename T, int kVec, int kPieces>
+__global__ void __launch_bounds__(kForwardBlock) team_forward_kernel(const AffineArgs a) {
+    using P = Part<T, kVec, kPieces>;
+    __shared__ float2 part[15][2][16];
+    const int h = a.hidden;
+    const int team = threadIdx.y;
+    TeamSum sum{part[team], static_cast<int>(blockDim.x >> 5), 1 + team};
+    const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.y;
+    const float inv_h = 1.0f / static_cast<float>(h);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + team; r < a.rows; r += stride) {
+        P x;
+        x.load(static_cast<const T *>(a.x) + r * h, h);
+        f32x2 s = pk2(0.0f, 0.0f);
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g)
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) s = fadd2(s, x.pair(g, i));
+        const float mean = sum(make_float2(both(s), 0.0f)).x * inv_h;
+        const f32x2 mean2 = pk2(mean, mean);
+        f32x2 q = pk2(0.0f, 0.0f);
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, h)) continue;
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) {
+                f32x2 d = fsub2(x.pair(g, i), mean2);
+                if (!P::kWide && !P::second(g, h)) {
+                    float lo, hi;
+                    unpk2(d, lo, hi);
+                    d = pk2(lo, 0.0f);
+                }
+                q = ffma2(d, d, q);
+            }
+        }
+        const float var = sum(make_float2(both(q), 0.0f)).x * inv_h;
+        const float rstd = 1.0f / sqrtf(var + a.epsilon);
+        if (threadIdx.x == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        const f32x2 rstd2 = pk2(rstd, rstd);
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, h)) continue;
+            f32x2 w[P::kPairs], b[P::kPairs], y[P::kPairs];
+            P::weights(a.weight, fp32, g, h, 1.0f, w);
+            P::weights(a.bias, fp32, g, h, 0.0f, b);
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) y[i] = ffma2(fmul2(fsub2(x.pair(g, i), mean2), rstd2), w[i], b[i]);
+            P::store(static_cast<T *>(a.out) + r * h, g, h, y);
+        }
+    }
+}
+
+template <typename T, int kVec, int kPieces, bool kParams>
+__global__ void __launch_bounds__(kBackwardBlock) team_backward_kernel(const AffineArgs a) {
+    using P = Part<T, kVec, kPieces>;
+    __shared__ float2 part[15][2][16];
+    extern __shared__ float joined[];  // [teams - 1][2 sums][elements of a thread][threads of a team]
+    const int h = a.hidden;
+    const int team = threadIdx.y;
+    TeamSum sum{part[team], static_cast<int>(blockDim.x >> 5), 1 + team};
+    const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.y;
+    const float inv_h = 1.0f / static_cast<float>(h);
+    f32x2 dw[P::kGroups][P::kPairs], db[P::kGroups][P::kPairs];
+#pragma unroll
+    for (int g = 0; g < P::kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < P::kPairs; ++i) dw[g][i] = db[g][i] = pk2(0.0f, 0.0f);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + team; r < a.rows; r += stride) {
+        P x, dy;
+        x.load(static_cast<const T *>(a.x) + r * h, h);
+        dy.load(static_cast<const T *>(a.grad) + r * h, h);
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        const f32x2 mean2 = pk2(mean, mean), rstd2 = pk2(rstd, rstd);
+        f32x2 s = pk2(0.0f, 0.0f), t = s;
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, h)) continue;
+            f32x2 w[P::kPairs];
+            if (a.dx) P::weights(a.weight, fp32, g, h, 1.0f, w);
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) {
+                const f32x2 n = fmul2(fsub2(x.pair(g, i), mean2), rstd2);
+                const f32x2 d = dy.pair(g, i);
+                if (kParams) {
+                    dw[g][i] = ffma2(d, n, dw[g][i]);
+                    db[g][i] = fadd2(db[g][i], d);
+                }
+                if (a.dx) {
+                    const f32x2 gw = fmul2(d, w[i]);
+                    s = fadd2(s, gw);
+                    t = ffma2(gw, n, t);
+                }
+            }
+        }
+        if (a.dx == nullptr) continue;
+        const float2 st = sum(make_float2(both(s), both(t)));
+        const f32x2 minus_s = pk2(-st.x * inv_h, -st.x * inv_h), minus_t = pk2(-st.y * inv_h, -st.y * inv_h);
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, h)) continue;
+            f32x2 w[P::kPairs], out[P::kPairs];
+            P::weights(a.weight, fp32, g, h, 1.0f, w);
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) {
+                const f32x2 n = fmul2(fsub2(x.pair(g, i), mean2), rstd2);
+                out[i] = fmul2(rstd2, ffma2(n, minus_t, ffma2(dy.pair(g, i), w[i], minus_s)));
+            }
+            P::store(static_cast<T *>(a.dx) + r * h, g, h, out);
+        }
+    }
+    if (!kParams) return;
+    // The teams' sums, then the CTA's slice of the workspace.
+    constexpr int kEach = P::kGroups * P::kPairs * 2;
+    const int step = blockDim.x;
+    if (team > 0) {
+        float *mine = joined + static_cast<int64_t>(team - 1) * 2 * kEach * step + threadIdx.x;
+#pragma unroll
+        for (int e = 0; e < kEach; e += 2) {
+            unpk2(dw[e / 2 / P::kPairs][e / 2 % P::kPairs], mine[e * step], mine[(e + 1) * step]);
+            unpk2(db[e / 2 / P::kPairs][e / 2 % P::kPairs], mine[(kEach + e) * step], mine[(kEach + e + 1) * step]);
+        }
+    }
+    __syncthreads();
+    if (team > 0) return;
+    float *out = a.workspace + static_cast<int64_t>(blockIdx.x) * 2 * h;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        float lo, hi;
+        unpk2(dw[e / 2 / P::kPairs][e / 2 % P::kPairs], lo, hi);
+        float sw = e & 1 ? hi : lo;
+        unpk2(db[e / 2 / P::kPairs][e / 2 % P::kPairs], lo, hi);
+        float sb = e & 1 ? hi : lo;
+        for (int t = 0; t + 1 < static_cast<int>(blockDim.y); ++t) {
+            sw += joined[(t * 2 * kEach + e) * step + threadIdx.x];
+            sb += joined[((t * 2 + 1) * kEach + e) * step + threadIdx.x];
+        }
+        const int c = P::kWide ? P::column(e / kVec) + e % kVec : P::column(e);
+        if (c < h) {
+            out[c] = sw;
+            out[h + c] = sb;
+        }
+    }
+}
+
+// Slices of partial sums joined: 32 columns by 8 runs of slices a block.
+template <typename W>
+__global__ void __launch_bounds__(256) team_join_kernel(const AffineArgs a, int slices) {
+    __shared__ float part[8][33];
+    const int c = blockIdx.x * 32 + threadIdx.x;  // of 2 * hidden: dw, then db
+    const int total = 2 * a.hidden;
+    float s = 0.0f;
+    if (c < total) {
+        const int first = slices * threadIdx.y / 8, last = slices * (threadIdx.y + 1) / 8;
+#pragma unroll 4
+        for (int i = first; i < last; ++i) s += a.workspace[static_cast<int64_t>(i) * total + c];
+    }
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y != 0 || c >= total) return;
+    for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
+    if (c < a.hidden) {
+        if (a.dweight) static_cast<W *>(a.dweight)[c] = from_f<W>(s);
+    } else if (a.dbias) {
+        static_cast<W *>(a.dbias)[c - a.hidden] = from_f<W>(s);
+    }
+}
 
 // Sum of two values over the block, in every thread.
 __device__ __forceinline__ float2 block_sum(float2 v) {
@@ -141,20 +440,6 @@ __global__ void __launch_bounds__(256) parameter_partial_kernel(const AffineArgs
     }
 }
 
-template <typename W>
-__global__ void __launch_bounds__(256) parameter_join_kernel(const AffineArgs a, int slices) {
-    const int h = a.hidden;
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= h) return;
-    float dw = 0.0f, db = 0.0f;
-    for (int s = 0; s < slices; ++s) {
-        dw += a.workspace[(static_cast<int64_t>(s) * 2) * h + c];
-        db += a.workspace[(static_cast<int64_t>(s) * 2 + 1) * h + c];
-    }
-    if (a.dweight) static_cast<W *>(a.dweight)[c] = from_f<W>(dw);
-    if (a.dbias) static_cast<W *>(a.dbias)[c] = from_f<W>(db);
-}
-
 template <typename F>
 cudaError_t with_type(int dtype, F f) {
     switch (dtype) {
@@ -166,32 +451,144 @@ cudaError_t with_type(int dtype, F f) {
 
 }  // namespace
 
-int64_t backward_slices(int64_t rows, int64_t) { return std::max<int64_t>(1, std::min<int64_t>(64, (rows + 31) / 32)); }
+namespace {
+// Weights have the input's type or fp32.
+template <typename T, typename F>
+cudaError_t with_weight(const AffineArgs &a, F f) {
+    return a.weight_dtype == CTU_DTYPE_FP32 ? f(float()) : f(T());
+}
+}  // namespace
+
+// How a row is held: `vec` elements a piece, `pieces` pieces a thread (0: wider than a team holds),
+// `threads` of a team, `teams` a CTA.  Depends on the sizes and the alignment of rows alone.
+namespace {
+struct TeamPlan {
+    int vec, pieces, threads, teams;
+};
+
+// As few threads as hold a row in at most `most` pieces each, so that an SM works on several rows.
+TeamPlan team_plan(int64_t hidden, int bytes, bool aligned, bool backward) {
+    TeamPlan p{};
+    p.vec = aligned && hidden * bytes % 16 == 0 ? 16 / bytes : 1;
+    const int64_t count = hidden / p.vec;
+    // Forward: x alone.  Backward: x, dy and two fp32 sums an element, in 168 registers.
+    const int most = p.vec == 1 ? 16 : !backward || p.vec == 4 ? 8 : 5;
+    const int block = backward ? kBackwardBlock : kForwardBlock;
+    const int64_t threads = ((count + most - 1) / most + 31) / 32 * 32;
+    if (threads > block) return p;
+    p.pieces = static_cast<int>((count + threads - 1) / threads);
+    if (p.vec == 1) p.pieces = p.pieces <= 2 ? 2 : p.pieces <= 4 ? 4 : p.pieces <= 8 ? 8 : 16;
+    p.threads = static_cast<int>(threads);
+    // Forward CTAs are small (128 threads) and many; a backward CTA fills an SM.
+    p.teams = static_cast<int>(std::max<int64_t>(1, (backward ? block : 128) / threads));
+    return p;
+}
+
+bool row_aligned(const void *p) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <int kVec, bool kBackward, typename F>
+cudaError_t with_pieces(int pieces, F f) {
+    if constexpr (kVec == 1) {
+        switch (pieces) {
+        case 2: return f(std::integral_constant<int, 2>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 8: return f(std::integral_constant<int, 8>());
+        case 16: return f(std::integral_constant<int, 16>());
+        default: return cudaErrorInvalidValue;
+        }
+    } else {
+        switch (pieces) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 3: return f(std::integral_constant<int, 3>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 5: return f(std::integral_constant<int, 5>());
+        default: break;
+        }
+        if constexpr (!kBackward || kVec == 4) {
+            switch (pieces) {
+            case 6: return f(std::integral_constant<int, 6>());
+            case 7: return f(std::integral_constant<int, 7>());
+            case 8: return f(std::integral_constant<int, 8>());
+            default: break;
+            }
+        }
+        return cudaErrorInvalidValue;
+    }
+}
+
+template <typename T, bool kBackward, typename F>
+cudaError_t with_shape(const TeamPlan &p, F f) {
+    constexpr int kFull = 16 / sizeof(T);
+    if (p.vec == kFull)
+        return with_pieces<kFull, kBackward>(p.pieces, [&](auto n) { return f(std::integral_constant<int, kFull>(), n); });
+    return with_pieces<1, kBackward>(p.pieces, [&](auto n) { return f(std::integral_constant<int, 1>(), n); });
+}
+}  // namespace
+
+int64_t backward_slices(int64_t rows, int64_t) { return std::max<int64_t>(1, std::min<int64_t>(kSlices, rows)); }
 
 cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
+    const bool aligned = row_aligned(a.x) && row_aligned(a.out) && row_aligned(a.weight) && row_aligned(a.bias);
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_type(a.weight_dtype, [&](auto w) {
-            forward_kernel<T, decltype(w)><<<grid, kThreads, 0, stream>>>(a);
+        const TeamPlan plan = team_plan(a.hidden, sizeof(T), aligned, false);
+        if (plan.pieces == 0) {
+            const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
+            return with_weight<T>(a, [&](auto w) {
+                forward_kernel<T, decltype(w)><<<grid, kThreads, 0, stream>>>(a);
+                return cudaGetLastError();
+            });
+        }
+        const unsigned grid = static_cast<unsigned>(
+            std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, static_cast<int64_t>(a.num_sms) * 16));
+        return with_shape<T, false>(plan, [&](auto vec, auto pieces) {
+            team_forward_kernel<T, vec, pieces><<<grid, dim3(plan.threads, plan.teams), 0, stream>>>(a);
             return cudaGetLastError();
         });
     });
 }
 
 cudaError_t launch_layer_norm_backward(const AffineArgs &a, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
-    const int slices = static_cast<int>(backward_slices(a.rows, a.hidden));
+    const bool aligned = row_aligned(a.x) && row_aligned(a.grad) && row_aligned(a.dx) && row_aligned(a.weight);
+    const bool params = a.dweight || a.dbias;
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_type(a.weight_dtype, [&](auto w) {
-            using W = decltype(w);
-            if (a.dx && a.rows > 0) input_gradient_kernel<T, W><<<grid, kThreads, 0, stream>>>(a);
-            if (a.dweight || a.dbias) {
-                parameter_partial_kernel<T>
-                    <<<dim3((a.hidden + 31) / 32, slices), dim3(32, 8), 0, stream>>>(a, slices);
-                parameter_join_kernel<W><<<(a.hidden + 255) / 256, 256, 0, stream>>>(a, slices);
+        const TeamPlan plan = team_plan(a.hidden, sizeof(T), aligned, true);
+        if (plan.pieces == 0) {
+            const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
+            const int slices = static_cast<int>(std::min<int64_t>(64, backward_slices(a.rows, a.hidden)));
+            return with_weight<T>(a, [&](auto w) {
+                using W = decltype(w);
+                if (a.dx && a.rows > 0) input_gradient_kernel<T, W><<<grid, kThreads, 0, stream>>>(a);
+                if (params) {
+                    parameter_partial_kernel<T>
+                        <<<dim3((a.hidden + 31) / 32, slices), dim3(32, 8), 0, stream>>>(a, slices);
+                    team_join_kernel<W><<<(2 * a.hidden + 31) / 32, dim3(32, 8), 0, stream>>>(a, slices);
+                }
+                return cudaGetLastError();
+            });
+        }
+        const int64_t ctas = std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, kSlices);
+        const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, ctas));
+        const cudaError_t e = with_shape<T, true>(plan, [&](auto vec, auto pieces) {
+            const dim3 block(plan.threads, plan.teams);
+            if (!params) {
+                team_backward_kernel<T, vec, pieces, false><<<grid, block, 0, stream>>>(a);
+                return cudaGetLastError();
             }
+            auto kernel = team_backward_kernel<T, vec, pieces, true>;
+            const int smem = (plan.teams - 1) * 2 * vec * pieces * plan.threads * static_cast<int>(sizeof(float));
+            if (smem > 32768)
+                if (cudaError_t f = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+                    return f;
+            kernel<<<grid, block, smem, stream>>>(a);
+            return cudaGetLastError();
+        });
+        if (e != cudaSuccess || !params) return e;
+        return with_weight<T>(a, [&](auto w) {
+            team_join_kernel<decltype(w)>
+                <<<(2 * a.hidden + 31) / 32, dim3(32, 8), 0, stream>>>(a, static_cast<int>(grid));
             return cudaGetLastError();
         });
     });
