@@ -51,7 +51,7 @@ __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 constexpr int kThreads = 256;  // of the looping kernels
 constexpr int kSlices = 148;   // CTAs of the backward pass: one an SM of a B200
 constexpr int kForwardBlock = 512;
-constexpr int kBackwardBlock = 384;  // times 168 registers: an SM's register file
+constexpr int kBackwardBlock = 640;  // times 96 registers: an SM's register file
 
 // A thread's part of a row: kPieces loads of kVec elements (16 bytes), or of single elements where rows
 // do not start on 16 bytes.  Elements are handled in pairs; a group is the pairs that share a load (or
@@ -134,6 +134,9 @@ struct Part {
 
 // Sum of two values over a team of `warps` warps, in every thread, in a fixed order.  Two buffers in
 // turn: a team's threads are past a buffer's last reads when its barrier after next is passed.
+// kNamed: several teams of warps in a CTA meet at barriers of their own (which reserves all sixteen of a
+// CTA, so not where occupancy counts); otherwise the CTA is one team, or every team one warp.
+template <bool kNamed>
 struct TeamSum {
     float2 (*part)[16];  // [2][16] of this team
     int warps;
@@ -151,7 +154,10 @@ struct TeamSum {
         flip ^= 1;
         const int warp = threadIdx.x >> 5;
         if ((threadIdx.x & 31) == 0) buf[warp] = v;
-        asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+        if (kNamed)
+            asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+        else
+            __syncthreads();
         v = buf[0];
         for (int i = 1; i < warps; ++i) {
             v.x += buf[i].x;
@@ -169,12 +175,12 @@ __device__ __forceinline__ float both(f32x2 v) {
 
 // blockDim = (threads of a team, teams).
 template <typename T, int kVec, int kPieces>
-__global__ void __launch_bounds__(kForwardBlock) team_forward_kernel(const AffineArgs a) {
+__global__ void __maxnreg__(64) team_forward_kernel(const AffineArgs a) {
     using P = Part<T, kVec, kPieces>;
-    __shared__ float2 part[15][2][16];
+    __shared__ float2 part[2][16];
     const int h = a.hidden;
     const int team = threadIdx.y;
-    TeamSum sum{part[team], static_cast<int>(blockDim.x >> 5), 1 + team};
+    TeamSum<false> sum{part, static_cast<int>(blockDim.x >> 5), 1 + team};
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.y;
     const float inv_h = 1.0f / static_cast<float>(h);
@@ -230,7 +236,7 @@ __global__ void __launch_bounds__(kBackwardBlock) team_backward_kernel(const Aff
     extern __shared__ float joined[];  // [teams - 1][2 sums][elements of a thread][threads of a team]
     const int h = a.hidden;
     const int team = threadIdx.y;
-    TeamSum sum{part[team], static_cast<int>(blockDim.x >> 5), 1 + team};
+    TeamSum<true> sum{part[team], static_cast<int>(blockDim.x >> 5), 1 + team};
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.y;
     const float inv_h = 1.0f / static_cast<float>(h);
@@ -239,11 +245,23 @@ __global__ void __launch_bounds__(kBackwardBlock) team_backward_kernel(const Aff
     for (int g = 0; g < P::kGroups; ++g)
 #pragma unroll
         for (int i = 0; i < P::kPairs; ++i) dw[g][i] = db[g][i] = pk2(0.0f, 0.0f);
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + team; r < a.rows; r += stride) {
-        P x, dy;
-        x.load(static_cast<const T *>(a.x) + r * h, h);
-        dy.load(static_cast<const T *>(a.grad) + r * h, h);
-        const float mean = a.mean[r], rstd = a.rstd[r];
+    // The next row's loads in flight, where registers allow it.
+    constexpr bool kAhead = kPieces * kVec <= (sizeof(T) == 4 ? 8 : 16);
+    P next_x, next_dy;
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    auto load = [&](int64_t r) {
+        next_x.load(static_cast<const T *>(a.x) + r * h, h);
+        next_dy.load(static_cast<const T *>(a.grad) + r * h, h);
+        next_mean = a.mean[r];
+        next_rstd = a.rstd[r];
+    };
+    int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + team;
+    if (kAhead && r < a.rows) load(r);
+    for (; r < a.rows; r += stride) {
+        if (!kAhead) load(r);
+        const P x = next_x, dy = next_dy;
+        const float mean = next_mean, rstd = next_rstd;
+        if (kAhead && r + stride < a.rows) load(r + stride);
         const f32x2 mean2 = pk2(mean, mean), rstd2 = pk2(rstd, rstd);
         f32x2 s = pk2(0.0f, 0.0f), t = s;
 #pragma unroll
@@ -466,21 +484,24 @@ struct TeamPlan {
     int vec, pieces, threads, teams;
 };
 
-// As few threads as hold a row in at most `most` pieces each, so that an SM works on several rows.
 TeamPlan team_plan(int64_t hidden, int bytes, bool aligned, bool backward) {
     TeamPlan p{};
     p.vec = aligned && hidden * bytes % 16 == 0 ? 16 / bytes : 1;
     const int64_t count = hidden / p.vec;
-    // Forward: x alone.  Backward: x, dy and two fp32 sums an element, in 168 registers.
-    const int most = p.vec == 1 ? 16 : !backward || p.vec == 4 ? 8 : 5;
     const int block = backward ? kBackwardBlock : kForwardBlock;
+    // Pieces a thread, as many as its registers hold.  Forward (64): x alone.  Backward (96): two fp32 sums
+    // an element, x, dy and the next row's x and dy; more pieces, without the next row, only for rows that
+    // the CTA would not hold otherwise.
+    int most = p.vec == 1 ? (backward ? 8 : 16) : backward ? 2 : p.vec == 4 ? 8 : 5;
+    if (backward && (count + most - 1) / most > block) most = p.vec == 1 ? 16 : p.vec == 4 ? 4 : 3;
     const int64_t threads = ((count + most - 1) / most + 31) / 32 * 32;
     if (threads > block) return p;
     p.pieces = static_cast<int>((count + threads - 1) / threads);
     if (p.vec == 1) p.pieces = p.pieces <= 2 ? 2 : p.pieces <= 4 ? 4 : p.pieces <= 8 ? 8 : 16;
     p.threads = static_cast<int>(threads);
-    // Forward CTAs are small (128 threads) and many; a backward CTA fills an SM.
-    p.teams = static_cast<int>(std::max<int64_t>(1, (backward ? block : 128) / threads));
+    // Forward CTAs are small (a team, or four of a warp) and many; a backward CTA fills an SM, with at most
+    // fifteen teams (named barriers).
+    p.teams = static_cast<int>(backward ? std::min<int64_t>(15, block / threads) : threads == 32 ? 4 : 1);
     return p;
 }
 
@@ -501,11 +522,15 @@ cudaError_t with_pieces(int pieces, F f) {
         case 1: return f(std::integral_constant<int, 1>());
         case 2: return f(std::integral_constant<int, 2>());
         case 3: return f(std::integral_constant<int, 3>());
-        case 4: return f(std::integral_constant<int, 4>());
-        case 5: return f(std::integral_constant<int, 5>());
         default: break;
         }
         if constexpr (!kBackward || kVec == 4) {
+            if (pieces == 4) return f(std::integral_constant<int, 4>());
+        }
+        if constexpr (!kBackward) {
+            if (pieces == 5) return f(std::integral_constant<int, 5>());
+        }
+        if constexpr (!kBackward && kVec == 4) {
             switch (pieces) {
             case 6: return f(std::integral_constant<int, 6>());
             case 7: return f(std::integral_constant<int, 7>());
