@@ -43,7 +43,9 @@ struct QuantArgs {
     int dtype;     // CTU_DTYPE_BF16 / FP16
     int num_sms;
     uint32_t *err;
-    int rows_per_warp;  // short rows side by side in a warp: 8, 4 or 2 of them (K <= 256, 512, 1024), else 1
+    // Rows side by side: up to eight groups of 256 columns, in a warp (8, 4 or 2 of one, two or four groups,
+    // else 1); beyond, in a CTA.
+    int side_by_side;
     int load_groups;    // groups of 256 columns per tile load (rotation)
 };
 // `map` (rotation only): x as lines of 64 values, 4 * load_groups of them to a box, 128-byte swizzle.

@@ -187,12 +187,19 @@ int ctu_fp4_quantize(const void *x, int64_t rows, int64_t k, int dtype, int form
     if (int rc = kernel_device(&q, &err)) return rc;
     fp4::QuantArgs a{x, codes, block_scales, row_scales, rows, static_cast<int>(k), format, rotation, dtype, q.num_sms, err};
     const int groups = static_cast<int>((k + 255) / 256);
-    a.rows_per_warp = groups == 1 ? 8 : groups == 2 ? 4 : groups <= 4 ? 2 : 1;
+    a.side_by_side = groups == 1 ? 8 : groups == 2 ? 4 : groups <= 4 ? 2 : 1;
+    // A CTA's warps hold eight groups each: two rows where one would leave more than a tenth of the lanes
+    // idle and two leave fewer (20 groups: 2.5 warps a row, five for two).
+    if (groups > 8) {
+        auto idle = [&](int rows) { return static_cast<double>((groups * rows + 7) / 8 * 8) / (groups * rows) - 1.0; };
+        a.side_by_side = groups <= 64 && idle(1) > 0.1 && idle(2) < idle(1) ? 2 : 1;
+    }
     CUtensorMap map{};
     if (rotation != 0) {
         // Rows of three groups do not lie side by side: one to a warp.
-        if (groups == 3) a.rows_per_warp = 1;
-        a.load_groups = a.rows_per_warp > 1 || groups % 8 == 0 ? 8 : groups % 4 == 0 ? 4 : 2;
+        if (groups == 3) a.side_by_side = 1;
+        const int held = groups * a.side_by_side;
+        a.load_groups = held % 8 == 0 ? 8 : held % 4 == 0 ? 4 : 2;
         const uint64_t lines = static_cast<uint64_t>(rows) * static_cast<uint64_t>(k / 64);
         if (lines > INT32_MAX) return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 quantizer dimensions exceed the CUDA kernel range");
         const uint64_t dims[2] = {64, lines};
@@ -211,6 +218,8 @@ int ctu_fp4_dequantize(const uint8_t *codes, const uint8_t *block_scales, const 
     if (int rc = check_matrix("FP4 dequantizer", rows, k, format)) return rc;
     if (dtype < CTU_DTYPE_BF16 || dtype > CTU_DTYPE_FP32)
         return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 dequantizer output must be float16, bfloat16, or float32");
+    if (rows * ((k + 1023) / 1024) > INT32_MAX)
+        return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 dequantizer dimensions exceed the CUDA kernel range");
     if (row_scale_count != 1 && row_scale_count != rows)
         return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 dequantizer requires one row scale or one per row");
     if (rows == 0) return CTU_OK;
@@ -322,7 +331,7 @@ int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t 
     if (!aligned16(grad) || !aligned16(w) || !aligned16(w_block_scales) || !aligned16(workspace) || !aligned16(dx))
         return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 linear gradient tensors must be 16-byte aligned");
     const int64_t tiles = ((m + fp4::kPairRows - 1) / fp4::kPairRows) * ((k + fp4::kGradCols - 1) / fp4::kGradCols);
-    if (tiles > INT32_MAX / 2)
+    if (tiles > INT32_MAX / 16 || n * ((k + 1023) / 1024) > INT32_MAX)
         return fail(CTU_ERR_INVALID_ARGUMENT, "FP4 linear gradient dimensions exceed the CUDA kernel range");
     DeviceQuery q;
     uint32_t *err;

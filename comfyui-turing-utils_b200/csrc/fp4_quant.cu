@@ -71,7 +71,8 @@ __device__ __forceinline__ uint32_t e2m1x8(const f32x2 (&q)[4]) {
     return r;
 }
 
-// Where a lane's columns are.  A team of lanes owns a row: some lanes of a warp, a warp, or the CTA.
+// Where a lane's columns are.  A team of lanes owns a row: some lanes of a warp, a warp, or several warps
+// of a CTA, which may hold `rows_per_cta` rows side by side.
 struct Place {
     int64_t row;
     int group;    // of 256 columns in the row
@@ -79,27 +80,57 @@ struct Place {
     bool active;  // the row and the group exist
 };
 
-// Largest magnitude over a row's team.  `span` lanes of a warp hold a row, or (kMulti) all warps do.
+// Largest magnitude over a row.  Within a warp `span` lanes hold a row.  kMulti: a warp's lanes belong to
+// the CTA's row `first_row` and, from lane `border` on, to the next one; red[2 * warp] and the next are
+// their maxima, and a row's warps are those of its groups.
 template <bool kMulti>
-__device__ __forceinline__ float row_max(float amax, int span, float *red) {
-    if (kMulti) span = 32;
-    for (int o = 1; o < span; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (kMulti) {
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-        __syncthreads();
-        amax = red[0];
-        for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) amax = max_nan(amax, red[w]);
+__device__ __forceinline__ float row_max(float amax, int span, float *red, int groups, int slot) {
+    if (!kMulti) {
+        for (int o = 1; o < span; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        return amax;
     }
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    const int first_row = warp * 8 / groups;  // of the CTA
+    const bool later = slot != first_row;
+    float lo = later ? 0.0f : amax, hi = later ? amax : 0.0f;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    if (__any_sync(0xffffffffu, later)) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (lane == 0) *reinterpret_cast<float2 *>(red + 2 * warp) = make_float2(lo, hi);
+    __syncthreads();
+    const int from = slot * groups / 8, to = min((slot * groups + groups - 1) / 8, static_cast<int>(blockDim.x >> 5) - 1);
+    amax = 0.0f;
+    for (int w = from; w <= to; ++w) amax = max_nan(amax, red[2 * w + (slot != w * 8 / groups ? 1 : 0)]);
     return amax;
 }
 
+// t / 6 to nearest (a product with the reciprocal and one correction by its exact remainder, Markstein),
+// for t in the range where the e4m3 rounding that follows can tell.
+__device__ __forceinline__ float sixth(float t) {
+    const float c = 1.0f / 6.0f;
+    const float q = __fmul_rn(t, c);
+    return __fmaf_rn(__fmaf_rn(q, -6.0f, t), c, q);
+}
+
+// 1 / s of a block scale: the hardware's approximation and one Newton step.  With s of four significant
+// bits the result is the nearest fp32 value.
+__device__ __forceinline__ float scale_reciprocal(float s) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s));
+    return __fmaf_rn(y, __fmaf_rn(-s, y, 1.0f), y);
+}
+
 // Codes and scales of one lane's four blocks of 16; pair(j, p) is columns 2p, 2p + 1 of block j and
-// amax[j] its largest magnitude.
-template <int kFormat, bool kMulti, typename Pair>
+// amax[j] its largest magnitude.  kWhole: K is a multiple of 256, so a group has all its columns.
+template <int kFormat, bool kMulti, bool kWhole, typename Pair>
 __device__ __forceinline__ void finish(const QuantArgs &a, const Place &at, float (&amax)[4], int span, float *red,
-                                       Pair pair) {
+                                       int slot, Pair pair) {
     float row_amax = max_nan(max_nan(amax[0], amax[1]), max_nan(amax[2], amax[3]));
-    row_amax = row_max<kMulti>(at.active ? row_amax : 0.0f, span, red);
+    row_amax = row_max<kMulti>(at.active ? row_amax : 0.0f, span, red, (a.k + 255) / 256, slot);
     const bool bad = !(row_amax <= 3.402823466e38f);
     float row = 1.0f;
     if (kFormat == kNvfp4 && !bad) row = pow2_row_scale(row_amax);
@@ -107,53 +138,54 @@ __device__ __forceinline__ void finish(const QuantArgs &a, const Place &at, floa
 #pragma unroll
         for (int j = 0; j < 4; ++j) amax[j] = fmaxf(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], 1));
     }
-    const float inv_row = 1.0f / row;
+    // 1 / row: a power of two, whose exponent is negated (2^-126 has its reciprocal, 2^126, in range).
+    const float inv_row = __uint_as_float(0x7f000000u - __float_as_uint(row));
+    const f32x2 minus_row = pk2(-inv_row, -inv_row);
     if (at.active && at.group == 0 && at.q == 0) a.row_scales[at.row] = bad ? __uint_as_float(0x7fc00000u) : row;
+    uint8_t *codes = a.codes + at.row * (a.k / 2) + at.group * 128 + at.q * 8;
 
     uint32_t bytes = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int col = at.group * 256 + j * 64 + at.q * 16;
-        const bool in = at.active && col < a.k;
-        uint32_t byte = 0;
-        uint32_t word[2] = {0u, 0u};
-        if (!bad && in) {
-            if (kFormat == kNvfp4) {
-                byte = __nv_cvt_float_to_fp8(__fdiv_rn(amax[j] * inv_row, 6.0f), __NV_SATFINITE, __NV_E4M3);
-                const float s = block_scale_value(byte, kNvfp4);
-                // v / s rounded to nearest: a product with the reciprocal and one correction by its
-                // exact remainder (Markstein), so that ties of the code grid stay ties.  The signs are
-                // placed so that a zero keeps its own; a zero scale leaves such zeros.
-                const float inv = s == 0.0f ? 0.0f : __frcp_rn(s);
-                const f32x2 minus_inv = pk2(-inv, -inv), s2 = pk2(s, s), minus_row = pk2(-inv_row, -inv_row);
+        uint32_t byte;
+        uint32_t word[2];
+        if (kFormat == kNvfp4) {
+            byte = __nv_cvt_float_to_fp8(sixth(amax[j] * inv_row), __NV_SATFINITE, __NV_E4M3);
+            const float s = block_scale_value(byte, kNvfp4);
+            // v / s rounded to nearest by the same two steps, so that ties of the code grid stay ties.
+            // The signs are placed so that a zero keeps its own; a zero scale leaves such zeros.
+            const float inv = byte == 0 ? 0.0f : scale_reciprocal(s);
+            const f32x2 minus_inv = pk2(-inv, -inv), s2 = pk2(s, s);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    f32x2 q[4];
+            for (int h = 0; h < 2; ++h) {
+                f32x2 q[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x2 minus_v = fmul2(pair(j, 4 * h + i), minus_row);
-                        const f32x2 q0 = fmul2(minus_v, minus_inv);
-                        q[i] = ffma2(ffma2(q0, s2, minus_v), minus_inv, q0);
-                    }
-                    word[h] = e2m1x8(q);
+                for (int i = 0; i < 4; ++i) {
+                    const f32x2 minus_v = fmul2(pair(j, 4 * h + i), minus_row);
+                    const f32x2 q0 = fmul2(minus_v, minus_inv);
+                    q[i] = ffma2(ffma2(q0, s2, minus_v), minus_inv, q0);
                 }
-            } else {
-                const uint32_t e = __float_as_uint(amax[j]) >> 23;
-                byte = e > 2 ? e - 2 : 0;
-                const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte), exact
-                const f32x2 inv2 = pk2(inv, inv);
+                word[h] = e2m1x8(q);
+            }
+        } else {
+            const uint32_t e = __float_as_uint(amax[j]) >> 23;
+            byte = e > 2 ? e - 2 : 0;
+            const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte), exact
+            const f32x2 inv2 = pk2(inv, inv);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    f32x2 q[4];
+            for (int h = 0; h < 2; ++h) {
+                f32x2 q[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) q[i] = fmul2(pair(j, 4 * h + i), inv2);
-                    word[h] = e2m1x8(q);
-                }
+                for (int i = 0; i < 4; ++i) q[i] = fmul2(pair(j, 4 * h + i), inv2);
+                word[h] = e2m1x8(q);
             }
         }
-        bytes |= byte << (8 * j);
-        if (in) *reinterpret_cast<uint2 *>(a.codes + at.row * (a.k / 2) + col / 2) = make_uint2(word[0], word[1]);
+        const bool in = kWhole || at.group * 256 + j * 64 + at.q * 16 < a.k;
+        if (in) bytes |= byte << (8 * j);
+        if (in && at.active)
+            *reinterpret_cast<uint2 *>(codes + j * 32) = bad ? make_uint2(0u, 0u) : make_uint2(word[0], word[1]);
     }
+    if (bad) bytes = 0;
     // The group's scale bytes to whole words of its tiles: a byte transpose among the four lanes.
     const int64_t col_tiles = scale_col_tiles(a.k, kFormat);
     uint32_t word;
@@ -199,20 +231,23 @@ __device__ __forceinline__ float high_value(uint32_t w) {
 // where infinities and NaN rank above every finite value.
 template <int kFormat, bool kHalf, bool kMulti>
 __global__ void __launch_bounds__(kMulti ? 768 : 128) quantize_kernel(const QuantArgs a) {
-    __shared__ float red[2][24];
+    __shared__ float red[2][48];
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
-    const int slots = a.rows_per_warp;  // rows side by side in a warp
-    const int span = 32 / slots;
+    const int groups = (a.k + 255) / 256;
+    const int slots = a.side_by_side;  // rows of a warp, or (kMulti) of the CTA
+    const int span = kMulti ? 32 : 32 / slots;
     const int64_t teams = kMulti ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4;
     const int64_t team = kMulti ? blockIdx.x : blockIdx.x * 4ll + warp;
+    const int place = warp * 8 + (lane >> 2);  // kMulti: group of the CTA's rows
+    const int slot = kMulti ? place / groups : lane / span;
     Place at;
     at.q = lane & 3;
-    at.group = kMulti ? warp * 8 + (lane >> 2) : (lane % span) >> 2;
+    at.group = kMulti ? place - slot * groups : (lane % span) >> 2;
     int flip = 0;
     for (int64_t r0 = team * slots; r0 < a.rows; r0 += teams * slots, flip ^= 1) {
-        at.row = r0 + (kMulti ? 0 : lane / span);
-        at.active = at.row < a.rows && at.group * 256 < a.k;
+        at.row = r0 + slot;
+        at.active = slot < slots && at.row < a.rows && at.group < groups;
         uint4 w[4][2];
         float amax[4];
 #pragma unroll
@@ -237,7 +272,7 @@ __global__ void __launch_bounds__(kMulti ? 768 : 128) quantize_kernel(const Quan
             else
                 amax[j] = __uint_as_float(m << 16);
         }
-        finish<kFormat, kMulti>(a, at, amax, span, red[flip], [&](int j, int p) {
+        finish<kFormat, kMulti, false>(a, at, amax, span, red[flip], slot, [&](int j, int p) {
             const uint32_t v = (&w[j][0].x)[p];
             return pk2(low_value<kHalf>(v), high_value<kHalf>(v));
         });
@@ -264,7 +299,7 @@ __device__ __forceinline__ void radix4_pair(f32x2 &x0, f32x2 &x1, f32x2 &x2, f32
 template <int kFormat, bool kHalf, bool kMulti, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads)
     rotate_quantize_kernel(const __grid_constant__ CUtensorMap tmap, const QuantArgs a) {
-    __shared__ float red[2][24];
+    __shared__ float red[2][48];
     __shared__ uint64_t bars[24];
     extern __shared__ uint8_t smem_raw[];
     const int lane = threadIdx.x & 31;
@@ -272,16 +307,19 @@ __global__ void __launch_bounds__(kMaxThreads)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)) + warp * 8192;
     const uint32_t base = smem_u32(smem);
     uint64_t *bar = &bars[warp];
-    const int slots = a.rows_per_warp;
-    const int span = 32 / slots;
+    const int slots = a.side_by_side;
+    const int span = kMulti ? 32 : 32 / slots;
     const int groups = a.k / 256;
     const int64_t teams = kMulti ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4;
     const int64_t team = kMulti ? blockIdx.x : blockIdx.x * 4ll + warp;
+    const int place = warp * 8 + (lane >> 2);
+    const int slot = kMulti ? place / groups : lane / span;
     Place at;
     at.q = lane & 3;
-    at.group = kMulti ? warp * 8 + (lane >> 2) : (lane % span) >> 2;
-    // Copies of `load_groups` groups each: this warp's part of a row, or several whole rows.
-    const int mine = kMulti ? min(8, groups - warp * 8) : slots > 1 ? 8 : groups;
+    at.group = kMulti ? place - slot * groups : (lane % span) >> 2;
+    // Copies of `load_groups` groups each: this warp's part of the CTA's rows (they follow one another), or
+    // several whole rows.
+    const int mine = kMulti ? min(8, groups * slots - warp * 8) : slots > 1 ? 8 : groups;
     const int copies = (mine + a.load_groups - 1) / a.load_groups;
     auto load = [&](int64_t r0) {  // lane 0
         mbar_arrive_expect_tx(bar, static_cast<uint32_t>(copies * a.load_groups * 512));
@@ -306,8 +344,8 @@ __global__ void __launch_bounds__(kMaxThreads)
     uint32_t phase = 0;
     int flip = 0;
     for (int64_t r0 = team * slots; r0 < a.rows; r0 += teams * slots, flip ^= 1) {
-        at.row = r0 + (kMulti ? 0 : lane / span);
-        at.active = at.row < a.rows && at.group < groups;
+        at.row = r0 + slot;
+        at.active = slot < slots && at.row < a.rows && at.group < groups;
         mbar_wait(bar, phase, nullptr, a.err, kErrTimeoutFull);
         phase ^= 1u;
         __syncwarp();
@@ -384,7 +422,7 @@ __global__ void __launch_bounds__(kMaxThreads)
                 amax[j] = max_abs3_nan(amax[j], lo, hi);
             }
         }
-        finish<kFormat, kMulti>(a, at, amax, span, red[flip], [&](int j, int p) { return v[j][p]; });
+        finish<kFormat, kMulti, true>(a, at, amax, span, red[flip], slot, [&](int j, int p) { return v[j][p]; });
     }
     clear_padding(a, kFormat);
 }
@@ -413,50 +451,68 @@ __device__ __forceinline__ void decode8(uint32_t w, __half2 (&h)[4]) {
     for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2 *>(&r[i]);
 }
 
-// A warp takes 256 columns of a row at a time, eight to a lane, four such pieces in flight.  code * block
-// scale is exact in fp32; the row scale rounds there unless it is a power of two.
+// A warp takes up to 2048 columns of a row, eight to a lane and step, all steps' loads in flight.
+// code * block scale is exact (in fp16 for nvfp4: six significant bits, 2^-10 .. 2688); the product with
+// the row scale rounds to fp32 unless that is a power of two.
 template <int kFormat, typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantArgs a) {
-    constexpr int kPieces = 4;
+    constexpr int kSteps = sizeof(T) == 4 ? 4 : 8;
     const int lane = threadIdx.x & 31;
-    const int segs = (a.k + 255) / 256;
-    const int64_t total = a.rows * segs;
+    const int parts = (a.k + 256 * kSteps - 1) / (256 * kSteps);
+    const uint32_t total = static_cast<uint32_t>(a.rows) * parts;
     const int64_t col_tiles = scale_col_tiles(a.k, kFormat);
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-    for (int64_t i0 = blockIdx.x * 8ll + (threadIdx.x >> 5); i0 < total; i0 += warps * kPieces) {
-        uint32_t w[kPieces];
-        uint32_t byte[kPieces];
-        float row[kPieces];
-        int64_t at[kPieces];
+    for (uint32_t i = blockIdx.x * 8u + (threadIdx.x >> 5); i < total; i += gridDim.x * 8u) {
+        const uint32_t r = i / parts;
+        const int c0 = static_cast<int>(i - r * parts) * (256 * kSteps) + 8 * lane;
+        const int64_t at = static_cast<int64_t>(r) * a.k + c0;
+        const uint32_t *codes = reinterpret_cast<const uint32_t *>(a.codes + at / 2);
+        const uint8_t *scales = a.block_scales + scale_offset(r, c0 / block_of(kFormat), col_tiles);
+        constexpr int kScaleStep = 256 / (4 * block_of(kFormat)) * 512;  // tiles a step, in bytes
+        uint32_t w[kSteps], byte[kSteps];
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            const int64_t i = i0 + p * warps;
-            const int64_t r = i / segs;
-            const int c = static_cast<int>(i - r * segs) * 256 + 8 * lane;
-            const bool in = i < total && c < a.k;
-            at[p] = in ? r * a.k + c : -1;
-            if (in) {
-                w[p] = __ldcs(reinterpret_cast<const uint32_t *>(a.codes + at[p] / 2));
-                byte[p] = a.block_scales[scale_offset(r, c / block_of(kFormat), col_tiles)];
-                row[p] = a.row_scales[a.row_scale_count == 1 ? 0 : r];
+        for (int p = 0; p < kSteps; ++p) {
+            w[p] = byte[p] = 0;
+            if (c0 + 256 * p < a.k) {
+                w[p] = __ldcs(codes + 32 * p);
+                byte[p] = scales[p * kScaleStep];
             }
         }
+        const float row = a.row_scales[a.row_scale_count == 1 ? 0 : r];
+        const f32x2 row2 = pk2(row, row);
+        T *out = static_cast<T *>(a.out) + at;
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            if (at[p] < 0) continue;
-            const float s = block_scale_value(byte[p], kFormat);
+        for (int p = 0; p < kSteps; ++p) {
+            if (c0 + 256 * p >= a.k) break;
             __half2 h[4];
             decode8(w[p], h);
-            T out[8];
+            f32x2 v[4];
+            if (kFormat == kNvfp4) {
+                const __half s = __half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte[p]), __NV_E4M3));
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 f = __half22float2(__hmul2(h[q], __half2half2(s)));
+                    v[q] = fmul2(pk2(f.x, f.y), row2);
+                }
+            } else {
+                const float s = block_scale_value(byte[p], kMxfp4);
+                const f32x2 s2 = pk2(s, s);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 f = __half22float2(h[q]);
+                    v[q] = fmul2(fmul2(pk2(f.x, f.y), s2), row2);
+                }
+            }
+            alignas(16) T o[8];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float2 v = __half22float2(h[q]);
-                out[2 * q] = store_as<T>(v.x * s * row[p]);
-                out[2 * q + 1] = store_as<T>(v.y * s * row[p]);
+                float lo, hi;
+                unpk2(v[q], lo, hi);
+                o[2 * q] = store_as<T>(lo);
+                o[2 * q + 1] = store_as<T>(hi);
             }
-            uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + at[p]);
+            uint4 *dst = reinterpret_cast<uint4 *>(out + 256 * p);
 #pragma unroll
-            for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) dst[q] = reinterpret_cast<const uint4 *>(out)[q];
+            for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) dst[q] = reinterpret_cast<const uint4 *>(o)[q];
         }
     }
 }
@@ -469,8 +525,9 @@ template <int kFormat, bool kHalf>
 cudaError_t quantize_as(const QuantArgs &a, const CUtensorMap &map, cudaStream_t stream) {
     const int groups = (a.k + 255) / 256;
     const bool multi = groups > 8;
-    const int warps = multi ? (groups + 7) / 8 : 4;
-    int64_t rows = multi ? a.rows : (a.rows + 4 * a.rows_per_warp - 1) / (4 * a.rows_per_warp);
+    const int warps = multi ? (groups * a.side_by_side + 7) / 8 : 4;
+    const int per_cta = multi ? a.side_by_side : 4 * a.side_by_side;
+    int64_t rows = (a.rows + per_cta - 1) / per_cta;
     // Enough CTAs to clear the last tile's padding at once, however few rows there are.
     if (a.rows & 127) rows = std::max<int64_t>(rows, (scale_col_tiles(a.k, kFormat) * 128 + warps * 32 - 1) / (warps * 32));
     if (a.rotation == 0) {
@@ -505,7 +562,7 @@ cudaError_t launch_quantize(const QuantArgs &a, const CUtensorMap &map, cudaStre
 template <typename T>
 static cudaError_t dequantize_as(const DequantArgs &a, cudaStream_t stream) {
     const unsigned grid = static_cast<unsigned>(
-        std::min<int64_t>((a.rows * ((a.k + 255) / 256) + 7) / 8, static_cast<int64_t>(a.num_sms) * 8));
+        std::min<int64_t>((a.rows * ((a.k + 1023) / 1024) + 7) / 8, static_cast<int64_t>(a.num_sms) * 8));
     if (a.format == kNvfp4)
         dequantize_kernel<kNvfp4, T><<<grid, 256, 0, stream>>>(a);
     else
