@@ -90,7 +90,7 @@ SmallKernel linear_small_kernel(int format, int64_t m);
 
 // CTA-pair product (tcgen05 block-scaled MMA).
 constexpr int kPairRows = 256;  // output rows of a pair tile
-constexpr int kPairCols = 192;
+constexpr int kPairCols = 256;
 int linear_pair_smem();
 const void *linear_pair_kernel(int format);
 int linear_pair_threads();

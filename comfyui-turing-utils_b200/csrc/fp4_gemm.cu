@@ -3,11 +3,16 @@
 //   out[m, n] = bf16( fma( (sum_k A[m, k] B[n, k]) * a_scale[m], w_scale[n], bias[n] ) )
 //
 // A and B are e2m1 codes times their block scales; the tensor cores apply both and accumulate in
-// fp32.  A pair of CTAs owns a 256 x 192 tile: CTA r stages rows [128 r, 128 r + 128) of A and 96
-// rows of B, the scales of its own A rows and those of all 192 B rows; one M = 256, N = 192, K = 64
-// instruction of the leader reads both CTAs' halves.  192 columns, not 256, so that two accumulators
-// (2 x 192 columns of tensor memory) and two sets of scales (2 x 48) fit its 512 columns, and the
-// epilogue of one tile runs under the next one's MMAs.
+// fp32.  A pair of CTAs owns a 256 x 256 tile: CTA r stages rows [128 r, 128 r + 128) of A and as many of
+// B, the scales of its own A rows and those of all 256 B rows; one M = 256, N = 256, K = 64 instruction of
+// the leader reads both CTAs' halves.
+//
+// What bounds it is the L2: at 32760 x 13824 x 5120 stages of 256 x 128, 256 x 192 and 256 x 256 take the
+// same 600 cycles, 12.6 TB/s of tiles and scales whatever the tile, so the tile is as large as tensor
+// memory allows (951 us with 192 columns and two separate accumulators).  Two accumulators of 256 columns
+// and the scales need 560 of the 512 columns: the second accumulator starts 48 columns before the
+// first one's end, and the epilogue of a tile reads the shared columns first and then lets the next
+// tile's MMAs start.
 //
 // Roles: warp 0 loads (TMA), warp 1 of the leader copies scales into tensor memory and issues the
 // MMAs, warps 2..5 write the output.  Every wait is bounded.
@@ -24,7 +29,7 @@ namespace fp4 {
 
 namespace {
 
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kStageK = 256;  // values of K per stage: 128 bytes of codes
 constexpr int kChunks = 4;    // MMAs per stage
 constexpr int kABytes = 128 * 128;
@@ -43,14 +48,16 @@ constexpr int kOutBytes = 32 * 128;      // its 32 rows
 constexpr int kStructOffset = kStageOutOffset + kEpilogueWarps * kOutBytes;
 constexpr int kThreadCount = 32 * (2 + kEpilogueWarps);
 constexpr int kTmemCols = 512;
-constexpr int kScaleCol = 2 * kPairCols;  // first column of the scales
-constexpr int kScaleSet = 48;             // 4 chunks x (4 of A + 8 of B)
+constexpr int kScaleCols = 48;                             // 4 chunks x (4 of A + 8 of B)
+constexpr int kScaleCol = kTmemCols - kScaleCols;          // first of them
+constexpr int kSecondAcc = kScaleCol - kPairCols;          // first column of the second accumulator: 208
+static_assert(kPairCols - kSecondAcc <= kOutCols, "the shared columns are within the epilogue's first piece");
 
 struct Shared {
     uint64_t full[kStages];
     uint64_t empty[kStages];
     uint64_t acc_full[2];
-    uint64_t acc_empty[2];
+    uint64_t acc_free;  // a tile's shared columns have been read (leader)
     uint64_t drain;
     uint32_t tmem_base;
     int abort_flag;
@@ -91,10 +98,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             mbar_init(&S.full[s], 1);
             mbar_init(&S.empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&S.acc_full[b], 1);
-            mbar_init(&S.acc_empty[b], 2 * kEpilogueWarps);
-        }
+        for (int b = 0; b < 2; ++b) mbar_init(&S.acc_full[b], 1);
+        mbar_init(&S.acc_free, 2 * kEpilogueWarps);
         mbar_init(&S.drain, 1);
         S.abort_flag = 0;
         fence_mbar_init();
@@ -153,7 +158,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             // there first, which costs more than an MMA of this width takes).
             int s = 0;
             uint32_t ph = 0;
-            uint32_t set = 0;
             int local = 0;
             bool ok = true;
             const uint32_t a0 = smem_desc_low(smem_u32(smem + kAOffset));
@@ -163,19 +167,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const uint32_t empty0 = smem_u32(&S.empty[0]);
             for (int t = pair; t < num_tiles && ok; t += num_pairs, ++local) {
                 const uint32_t ab = local & 1;
-                ok = __all_sync(0xffffffffu, guard.wait_cluster(&S.acc_empty[ab], ((local >> 1) & 1) ^ 1u, kErrTimeoutAccumFree));
+                // The tile before last has been read entirely when the last one's shared columns have.
+                if (local > 0)
+                    ok = __all_sync(0xffffffffu, guard.wait_cluster(&S.acc_free, (local - 1) & 1, kErrTimeoutAccumFree));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + ab * kPairCols;
-                // The tile's first column may lie 64 rows into its first scale tile: two columns.
-                const uint32_t b_shift = static_cast<uint32_t>(((t % num_n) * kPairCols % 128) / 32);
+                const uint32_t d = tmem_base + ab * kSecondAcc;
                 for (int kb = 0; kb < nk; ++kb) {
                     ok = __all_sync(0xffffffffu, guard.wait(&S.full[s], ph, kErrTimeoutFull));
                     if (!ok) break;
                     tc_fence_after();
-                    // Scale sets alternate, so copies for one stage do not wait for the MMAs of the
-                    // stage before; copies and MMAs of one thread execute in order.
-                    const uint32_t sa = tmem_base + kScaleCol + set * kScaleSet;
+                    // Scale copies and MMAs of one thread execute in order, so one set of columns serves
+                    // every stage.
+                    const uint32_t sa = tmem_base + kScaleCol;
                     const uint32_t sb = sa + 16;
                     const uint32_t a = a0 + s * (kABytes >> 4);
                     const uint32_t b = b0 + s * (kBBytes >> 4);
@@ -195,13 +199,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                                                        ? idesc_fp4(kFormat, kPairRows, kPairCols, 0)
                                                        : idesc_fp4(kFormat, kPairRows, kPairCols, 2 * (c & 1));
                             mma_fp4_pair<kFormat>(d, desc64(a + 2 * c, kDescSw128High), desc64(b + 2 * c, kDescSw128High),
-                                                  idesc, sa + 4 * tile, sb + 8 * tile + b_shift, (kb | c) != 0 ? 1u : 0u);
+                                                  idesc, sa + 4 * tile, sb + 8 * tile, (kb | c) != 0 ? 1u : 0u);
                         }
                         mma_commit_pair_both_at(empty0 + 8 * s);
                         if (kb == nk - 1) mma_commit_pair_both(&S.acc_full[ab]);
                     }
                     __syncwarp();
-                    set ^= 1u;
                     if (++s == kStages) {
                         s = 0;
                         ph ^= 1u;
@@ -217,7 +220,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     } else {
         const int quad = warp & 3;
         const int ethread = threadIdx.x - 64;
-        const uint32_t leader_empty = mapa_shared(smem_u32(&S.acc_empty[0]), 0u);
+        const uint32_t leader_free = mapa_shared(smem_u32(&S.acc_free), 0u);
         const uint32_t staged = smem_u32(smem + kStageOutOffset + (warp - 2) * kOutBytes);
         const bool tma_out = (args.n & 7) == 0;  // rows of the output start on 16 bytes
         bool alive = true;
@@ -244,18 +247,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const int m_warp = m0 + quad * 32;
             const float a_s = m_warp + lane < args.m ? args.a_scale[m_warp + lane] : 0.0f;
 #pragma unroll 1
-            for (int c = 0; c < kPairCols / kOutCols; ++c) {
+            for (int i = 0; i < kPairCols / kOutCols; ++i) {
+                // The piece with the shared columns first: the last one of the first accumulator, the first
+                // one of the second.
+                const int c = ab == 0 ? (i + kPairCols / kOutCols - 1) % (kPairCols / kOutCols) : i;
                 const int n = n0 + c * kOutCols;
-                if (n >= args.n || m_warp >= args.m) break;
+                const bool inside = n < args.n && m_warp < args.m;
                 uint32_t acc[2][32];
-                const uint32_t src = tmem_base + static_cast<uint32_t>(ab * kPairCols + c * kOutCols) +
+                const uint32_t src = tmem_base + static_cast<uint32_t>(ab * kSecondAcc + c * kOutCols) +
                                      (static_cast<uint32_t>(quad * 32) << 16);
                 tmem_ld_32x32b_x32(src, acc[0]);
                 tmem_ld_32x32b_x32(src + 32, acc[1]);
                 // The staging rows are free once the last copy out of them has read them.
                 if (lane == 0) bulk_wait_read_all();
-                __syncwarp();
                 tmem_ld_wait();
+                if (i == 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_remote(leader_free);
+                }
+                __syncwarp();
+                if (!inside) continue;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -263,11 +275,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                         uint32_t p[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int i = 8 * q + 2 * j;
-                            const int col = c * kOutCols + 32 * h + i;
+                            const int e = 8 * q + 2 * j;
+                            const int col = c * kOutCols + 32 * h + e;
                             p[j] = pack_bf16x2(
-                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][i]), a_s), S.col_scale[col], S.col_bias[col]),
-                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][i + 1]), a_s), S.col_scale[col + 1],
+                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][e]), a_s), S.col_scale[col], S.col_bias[col]),
+                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][e + 1]), a_s), S.col_scale[col + 1],
                                           S.col_bias[col + 1]));
                         }
                         st_shared_v4(staged + 128u * lane + ((static_cast<uint32_t>(4 * h + q) ^ (lane & 7u)) << 4), p);
@@ -286,9 +298,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     __syncwarp();
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_remote(leader_empty + static_cast<uint32_t>(ab * sizeof(uint64_t)));
         }
         if (lane == 0) bulk_wait_all();  // the staged rows leave shared memory before the CTA does
     }
