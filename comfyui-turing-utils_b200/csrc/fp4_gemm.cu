@@ -223,6 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
         const uint32_t leader_free = mapa_shared(smem_u32(&S.acc_free), 0u);
         const uint32_t staged = smem_u32(smem + kStageOutOffset + (warp - 2) * kOutBytes);
         const bool tma_out = (args.n & 7) == 0;  // rows of the output start on 16 bytes
+        const uint64_t policy = evict_first_policy();
         bool alive = true;
         int local = 0;
         for (int t = pair; t < num_tiles; t += num_pairs, ++local) {
@@ -238,9 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             }
             named_barrier(1, 32 * kEpilogueWarps);
             if (alive) {
-                int ok = 1;
-                if (lane == 0) ok = guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum) ? 1 : 0;
-                alive = __shfl_sync(0xffffffffu, ok, 0) != 0;
+                alive = __all_sync(0xffffffffu, guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum));
             }
             if (!alive) continue;
             tc_fence_after();
@@ -289,7 +288,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_2d(&tmap_out, staged, n, m_warp);
+                        tma_store_2d(&tmap_out, staged, n, m_warp, policy);
                         bulk_commit();
                     }
                 } else {

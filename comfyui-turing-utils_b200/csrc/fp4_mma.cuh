@@ -116,10 +116,17 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
            | (static_cast<uint32_t>(m >> 4) << 24);   // M / 16
 }
 
-// 2D tile store from shared memory; what lies beyond the tensor is not written.
-__device__ __forceinline__ void tma_store_2d(const void *tmap, uint32_t smem_src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(tmap), "r"(x),
-                 "r"(y), "r"(smem_src)
+// 2D tile store from shared memory; what lies beyond the tensor is not written.  Output lines are the
+// first to leave the L2, which the operands' tiles are read from many times.
+__device__ __forceinline__ uint64_t evict_first_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void tma_store_2d(const void *tmap, uint32_t smem_src, int x, int y, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%1, %2}], [%3], %4;" ::"l"(
+                     tmap),
+                 "r"(x), "r"(y), "r"(smem_src), "l"(policy)
                  : "memory");
 }
 
