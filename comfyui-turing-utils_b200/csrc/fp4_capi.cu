@@ -132,6 +132,14 @@ int encode_scales(CUtensorMap *map, const void *scales, int64_t rows, int64_t k,
 // Forces a product kernel for tests: 0 by size, 1 the pair kernel, 2 the kernel for few rows.
 std::atomic<int> g_fp4_kernel{0};
 
+// The kernel for few rows up to 64 of them, and up to 128 where its strips leave half of the SMs to split
+// K over.  us, it against the pair kernel: 64 x 5120 x 5120 8.8 / 13.1, 64 x 13824 x 5120 14.0 / 13.5,
+// 128 x 5120 x 5120 11.1 / 13.7, 128 x 13824 x 5120 19.4 / 14.3, 128 x 512 x 512 11.0 / 8.2.
+bool few_rows(int64_t m, int64_t n, int64_t k, int num_sms) {
+    const int64_t strips = (n + fp4::kStripRows - 1) / fp4::kStripRows;
+    return m <= 64 || (m <= 128 && 2 * strips <= num_sms && k >= 1024);
+}
+
 SmemPlan g_small_plan[8];
 
 PairPlan g_linear_plan[2];
@@ -256,7 +264,7 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
     fp4::LinearArgs args{a_scale, w_scale, bias, out, err, static_cast<int>(m), static_cast<int>(n),
                          static_cast<int>(k), w_scale_count == 1 ? 1 : 0, format, 1};
     const int forced = g_fp4_kernel.load(std::memory_order_relaxed);
-    if (forced == 2 || (forced == 0 && m <= 128)) {
+    if (forced == 2 || (forced == 0 && few_rows(m, n, k, q.num_sms))) {
         const fp4::SmallKernel sk = fp4::linear_small_kernel(format, m);
         const int64_t strips =
             ((m + sk.tokens - 1) / sk.tokens) * ((n + fp4::kStripRows - 1) / fp4::kStripRows);

@@ -5,9 +5,8 @@
 //
 // K is split over the CTAs of a cluster, so that all SMs load at once however few strips there are.
 // Each CTA leaves its fp32 partial sums in its shared memory; after a cluster barrier the CTAs share
-// out the tokens, add the partials in rank order (equal calls give equal bits) and write the output.
-// TMEM lanes are output columns here: a warp's store of one token is 64 contiguous bytes, whatever
-// the output's alignment.
+// out the tokens, add the partials in rank order (equal calls give equal bits) and write the output, a
+// warp 256 contiguous bytes of a token.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -98,9 +97,12 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t *r) 
         : "r"(taddr));
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr)
+                 : "memory");
     return v;
 }
 
@@ -245,51 +247,66 @@ __global__ void __launch_bounds__(kThreadCount)
 
     const int valid = min(kTokens, args.m - m0);
     if (warp >= 2) {
-        const int row = (warp & 3) * 32 + lane;  // output column of the strip
-        const int n = n0 + row;
-        const bool in = n < args.n;
-        const float w_s = in ? args.w_scale[args.w_scale_count == 1 ? 0 : n] : 0.0f;
-        const float bias = in && args.bias != nullptr ? args.bias[n] : 0.0f;
-        __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(args.out);
+        // Partial sums to shared memory, [token][column of the strip]; the lanes are columns here.
         float *part = reinterpret_cast<float *>(smem);
+        const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
         for (int c = 0; c < valid && alive; c += 16) {
             uint32_t acc[16];
             tmem_ld_32x32b_x16(tmem_base + c + (static_cast<uint32_t>((warp & 3) * 32) << 16), acc);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                if (c + j >= valid) break;
-                if (split > 1) {
-                    part[(c + j) * kStrip + row] = __uint_as_float(acc[j]);
-                } else if (in) {
-                    const float v = __fmul_rn(__uint_as_float(acc[j]), args.a_scale[m0 + c + j]);
-                    out[static_cast<int64_t>(m0 + c + j) * args.n + n] = __float2bfloat16_rn(__fmaf_rn(v, w_s, bias));
-                }
-            }
+            for (int j = 0; j < 16; ++j)
+                if (c + j < valid) part[(c + j) * kStrip + row] = __uint_as_float(acc[j]);
         }
         tc_fence_before();
         __syncwarp();
-        if (split > 1) {
+        if (split > 1)
             cluster_sync();
-            if (in && alive) {
-                const uint32_t base = smem_u32(smem) + 4u * row;
-                for (int t = static_cast<int>(rank); t < valid; t += split) {
-                    float p[8];
+        else
+            named_barrier(1, 32 * kEpilogueWarps);
+        // A warp takes a token, a lane four columns of it.
+        const int n = n0 + 4 * lane;
+        if (n < args.n && alive) {
+            float w_s[4], bias[4];
 #pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        p[r] = r < split ? ld_cluster_f32(mapa_shared(base + 4u * kStrip * t, r)) : 0.0f;
-                    float sum = p[0];
+            for (int i = 0; i < 4; ++i) {
+                const bool in = n + i < args.n;
+                w_s[i] = in ? args.w_scale[args.w_scale_count == 1 ? 0 : n + i] : 0.0f;
+                bias[i] = in && args.bias != nullptr ? args.bias[n + i] : 0.0f;
+            }
+            const bool wide = (args.n & 3) == 0;
+            for (int t = static_cast<int>(rank) + split * (warp - 2); t < valid; t += split * kEpilogueWarps) {
+                const uint32_t src = smem_u32(smem) + 4u * (kStrip * t + 4 * lane);
+                float4 p[8];
 #pragma unroll
-                    for (int r = 1; r < 8; ++r)
-                        if (r < split) sum += p[r];
-                    const float v = __fmul_rn(sum, args.a_scale[m0 + t]);
-                    out[static_cast<int64_t>(m0 + t) * args.n + n] = __float2bfloat16_rn(__fmaf_rn(v, w_s, bias));
+                for (int r = 0; r < 8; ++r)
+                    if (r < split) p[r] = ld_cluster_f32x4(mapa_shared(src, r));
+                const float a_s = args.a_scale[m0 + t];
+                float4 sum = p[0];
+#pragma unroll
+                for (int r = 1; r < 8; ++r) {
+                    if (r < split) {
+                        sum.x += p[r].x;
+                        sum.y += p[r].y;
+                        sum.z += p[r].z;
+                        sum.w += p[r].w;
+                    }
+                }
+                const float v[4] = {__fmaf_rn(__fmul_rn(sum.x, a_s), w_s[0], bias[0]), __fmaf_rn(__fmul_rn(sum.y, a_s), w_s[1], bias[1]),
+                                    __fmaf_rn(__fmul_rn(sum.z, a_s), w_s[2], bias[2]), __fmaf_rn(__fmul_rn(sum.w, a_s), w_s[3], bias[3])};
+                __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(args.out) + static_cast<int64_t>(m0 + t) * args.n + n;
+                if (wide) {
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < args.n) dst[i] = __float2bfloat16_rn(v[i]);
                 }
             }
-            __syncwarp();
-            cluster_sync();  // no CTA leaves while another reads its partial sums
         }
+        __syncwarp();
+        if (split > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
     } else if (split > 1) {
         __syncwarp();
         cluster_sync();

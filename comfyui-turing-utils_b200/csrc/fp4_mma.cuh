@@ -142,31 +142,50 @@ __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
 }
 
 // 32 staged rows of 64 bf16 values (128-byte swizzle) to an output whose rows need not start on 16
-// bytes: a warp writes a row at a time in aligned pairs.  Where a row starts on an odd element, a lane
-// pairs its neighbour's second value with its own first, and the row's ends go out alone.
+// bytes: a warp writes a row in aligned pairs, eight rows' loads in flight.  Where a row starts on an odd
+// element, a lane pairs its neighbour's second value with its own first, and the row's ends go out alone.
 __device__ __forceinline__ void store_rows(__nv_bfloat16 *out, uint32_t staged, int m0, int n0, int rows, int cols,
                                            int lane) {
     const int valid = min(64, cols - n0);
     const int count = min(32, rows - m0);
-    for (int r = 0; r < count; ++r) {
-        const int64_t first = static_cast<int64_t>(m0 + r) * cols + n0;
-        const uint32_t own = ld_shared_u32(staged + 128u * r + (((static_cast<uint32_t>(lane) >> 2) ^ (r & 7u)) << 4) +
-                                           (lane & 3u) * 4u);
-        uint16_t *dst = reinterpret_cast<uint16_t *>(out) + first;
-        if ((first & 1) == 0) {
-            if (2 * lane + 1 < valid)
-                *reinterpret_cast<uint32_t *>(dst + 2 * lane) = own;
-            else if (2 * lane < valid)
-                dst[2 * lane] = static_cast<uint16_t>(own);
-        } else {
-            const uint32_t before = __shfl_up_sync(0xffffffffu, own, 1);
-            if (lane == 0)
-                dst[0] = static_cast<uint16_t>(own);
-            else if (2 * lane < valid)
-                *reinterpret_cast<uint32_t *>(dst + 2 * lane - 1) = __byte_perm(before, own, 0x5432);
-            else if (2 * lane - 1 < valid)
-                dst[2 * lane - 1] = static_cast<uint16_t>(before >> 16);
-            if (lane == 31 && valid == 64) dst[63] = static_cast<uint16_t>(own >> 16);
+    uint16_t *dst = reinterpret_cast<uint16_t *>(out) + static_cast<int64_t>(m0) * cols + n0;
+    bool odd = (static_cast<int64_t>(m0) * cols + n0) & 1;
+    for (int r0 = 0; r0 < count; r0 += 8) {
+        uint32_t own[8], before[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            own[i] = ld_shared_u32(staged + 128u * (r0 + i) + (((static_cast<uint32_t>(lane) >> 2) ^ static_cast<uint32_t>(i)) << 4) +
+                                   (lane & 3u) * 4u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) before[i] = __shfl_up_sync(0xffffffffu, own[i], 1);
+        if (valid == 64 && r0 + 8 <= count) {  // no lane leaves the others' path
+            const bool edge = lane == 0 || lane == 31;
+#pragma unroll
+            for (int i = 0; i < 8; ++i, dst += cols, odd ^= (cols & 1) != 0) {
+                const uint32_t word = odd ? __byte_perm(before[i], own[i], 0x5432) : own[i];
+                uint16_t *at = dst + 2 * lane - (odd ? 1 : 0);
+                if (!odd || lane > 0) *reinterpret_cast<uint32_t *>(at) = word;
+                if (odd && edge) dst[lane == 0 ? 0 : 63] = static_cast<uint16_t>(lane == 0 ? own[i] : own[i] >> 16);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i, dst += cols, odd ^= (cols & 1) != 0) {
+            if (r0 + i >= count) break;
+            if (!odd) {
+                if (2 * lane + 1 < valid)
+                    *reinterpret_cast<uint32_t *>(dst + 2 * lane) = own[i];
+                else if (2 * lane < valid)
+                    dst[2 * lane] = static_cast<uint16_t>(own[i]);
+            } else {
+                if (lane == 0)
+                    dst[0] = static_cast<uint16_t>(own[i]);
+                else if (2 * lane < valid)
+                    *reinterpret_cast<uint32_t *>(dst + 2 * lane - 1) = __byte_perm(before[i], own[i], 0x5432);
+                else if (2 * lane - 1 < valid)
+                    dst[2 * lane - 1] = static_cast<uint16_t>(before[i] >> 16);
+                if (lane == 31 && valid == 64) dst[63] = static_cast<uint16_t>(own[i] >> 16);
+            }
         }
     }
 }
