@@ -108,7 +108,7 @@ constexpr int kGradCols = 256;
 int grad_pair_smem();
 const void *grad_pair_kernel(int rotation);
 int grad_pair_threads();
-// Joins the partial sums of a split product: sum over parts in order, rotation, one rounding.
+// Joins the partial sums of a split product: sum over parts in order, one rounding.
 cudaError_t launch_grad_join(const GradArgs &a, int num_sms, cudaStream_t stream);
 
 }  // namespace fp4

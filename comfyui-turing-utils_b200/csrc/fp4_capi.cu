@@ -146,18 +146,19 @@ PairPlan g_linear_plan[2];
 PairPlan g_grad_plan[2];
 
 // Parts of the gradient's sum over n.  Tiles that do not fill the pairs of a B200 (74) are cut along n
-// until the rounds of pairs, counted in 64-row stages, are as few as they get; each further part costs a
-// pass of fp32 sums over dx (about four stages' worth a tile), so up to eight.  333 x 13824 x 5120: 40
-// tiles of 216 stages, three parts are two rounds of 72.  Depends on the sizes alone, so that the
-// workspace and the sums' order do.
+// while that lowers the rounds of pairs, counted in 64-row stages (0.28 us), plus the write and read of the
+// parts' fp32 sums at 5 TB/s.  333 x 13824 x 5120 is 40 tiles of 216 stages: three parts are two rounds of 72.
+// Depends on the sizes alone, so that the workspace and the sums' order do.
 int64_t grad_split(int64_t m, int64_t n, int64_t k) {
     constexpr int64_t kPairs = 74;
     const int64_t tiles = ((m + fp4::kPairRows - 1) / fp4::kPairRows) * ((k + fp4::kGradCols - 1) / fp4::kGradCols);
     const int64_t stages = (n + 63) / 64;
     if (tiles >= kPairs) return 1;
-    int64_t best = 1, cost = stages;
-    for (int64_t s = 2; s <= 8 && s <= stages; ++s) {
-        const int64_t c = (tiles * s + kPairs - 1) / kPairs * ((stages + s - 1) / s + 4) + 8;
+    int64_t best = 1;
+    double cost = static_cast<double>(stages);
+    for (int64_t s = 2; s <= 16 && 2 * s <= stages; ++s) {
+        const double rounds = static_cast<double>((tiles * s + kPairs - 1) / kPairs * ((stages + s - 1) / s));
+        const double c = rounds + 12.0 + static_cast<double>(s * m * k) * 5.7e-6;
         if (c < cost) {
             cost = c;
             best = s;

@@ -10,8 +10,8 @@
 // row and takes the strides 1, 4 and 16 in registers, 64 columns at a time, writes them back to
 // tensor memory, and takes stride 64 from there.  Rounded once, to bf16.
 //
-// With too few tiles to fill the GPU the sum over n is split; each part leaves fp32 sums, and a second
-// kernel adds them in order, rotates and rounds.
+// With too few tiles to fill the GPU the sum over n is split; each part leaves fp32 sums (rotated: the
+// rotation is linear), and a second kernel adds them in order and rounds.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -90,6 +90,11 @@ __device__ __forceinline__ void store_row16(__nv_bfloat16 *dst, const uint32_t *
             p[j] = pack_bf16x2(__uint_as_float(r[8 * q + 2 * j]), __uint_as_float(r[8 * q + 2 * j + 1]));
         reinterpret_cast<uint4 *>(dst)[q] = make_uint4(p[0], p[1], p[2], p[3]);
     }
+}
+
+__device__ __forceinline__ void store_sums16(float *dst, const uint32_t *r) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) reinterpret_cast<uint4 *>(dst)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
 }
 
 }  // namespace
@@ -250,20 +255,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const bool row_ok = m < args.m;
             const uint32_t acc = tmem_base + static_cast<uint32_t>(ab * kGradCols) + (static_cast<uint32_t>(quad * 32) << 16);
             __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(args.out) + static_cast<int64_t>(m) * args.k + n0;
-            if (args.split > 1) {
-                float *sums = args.partials + (static_cast<int64_t>(part) * args.m + m) * args.k + n0;
-#pragma unroll 1
-                for (int c = 0; c < 8; ++c) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(acc + c * 32, r);
-                    tmem_ld_wait();
-                    if (row_ok && n0 + c * 32 < args.k) {
-#pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            reinterpret_cast<uint4 *>(sums + c * 32)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-                    }
-                }
-            } else if constexpr (kRotate) {
+            float *sums = args.partials + (static_cast<int64_t>(part) * args.m + m) * args.k + n0;
+            const bool parts = args.split > 1;
+            if constexpr (kRotate) {
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t lo[32], hi[32];
@@ -304,7 +298,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     for (int i = 0; i < 16; ++i) radix4(r[0][i], r[1][i], r[2][i], r[3][i]);
                     if (row_ok) {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) store_row16(dst + q * 64 + c * 16, r[q]);
+                        for (int q = 0; q < 4; ++q) {
+                            if (parts)
+                                store_sums16(sums + q * 64 + c * 16, r[q]);
+                            else
+                                store_row16(dst + q * 64 + c * 16, r[q]);
+                        }
                     }
                 }
             } else {
@@ -313,7 +312,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     uint32_t r[16];
                     tmem_ld_32x32b_x16(acc + c * 16, r);
                     tmem_ld_wait();
-                    if (row_ok && n0 + c * 16 < args.k) store_row16(dst + c * 16, r);
+                    if (row_ok && n0 + c * 16 < args.k) {
+                        if (parts)
+                            store_sums16(sums + c * 16, r);
+                        else
+                            store_row16(dst + c * 16, r);
+                    }
                 }
             }
             tc_fence_before();
@@ -331,95 +335,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     }
 }
 
-// Four lanes to 256 columns (a rotation block): lane q holds columns 64 j + 16 q + i, so strides 1, 4 and
-// 64 are in registers and stride 16 is across the lanes.
-template <bool kRotate>
-__global__ void __launch_bounds__(128) grad_join_kernel(const GradArgs a) {
-    const int64_t quads = static_cast<int64_t>(a.m) * ((a.k + 255) / 256);
-    const int groups = (a.k + 255) / 256;
-    const int64_t part = static_cast<int64_t>(a.m) * a.k;
-    const int q = threadIdx.x & 3;
-    const int64_t total = (quads * 4 + 31) / 32 * 32;  // whole warps stay together
-    for (int64_t i = blockIdx.x * 128ll + threadIdx.x; i < total; i += gridDim.x * 128ll) {
-        const int64_t row = (i >> 2) / groups;
-        const int col = static_cast<int>((i >> 2) - row * groups) * 256;
-        const bool in = (i >> 2) < quads;
-        const float *src = a.partials + row * a.k + col;
-        __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + row * a.k + col;
-        if constexpr (kRotate) {
-            float v[4][16];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {  // columns 64 j + 16 q + i
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (in) {
-                        for (int p = 0; p < a.split; ++p) {
-                            const float4 x = __ldcs(reinterpret_cast<const float4 *>(src + p * part + 64 * j + 16 * q + 4 * c));
-                            sum.x += x.x;
-                            sum.y += x.y;
-                            sum.z += x.z;
-                            sum.w += x.w;
-                        }
-                    }
-                    v[j][4 * c] = sum.x * 0.0625f;
-                    v[j][4 * c + 1] = sum.y * 0.0625f;
-                    v[j][4 * c + 2] = sum.z * 0.0625f;
-                    v[j][4 * c + 3] = sum.w * 0.0625f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t(&u)[16] = reinterpret_cast<uint32_t(&)[16]>(v[j]);
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) radix4(u[i], u[i + 1], u[i + 2], u[i + 3]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) radix4(u[i], u[i + 4], u[i + 8], u[i + 12]);
-                // Stride 16: the four lanes hold the four digits; each computes its own output.
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int lead = (threadIdx.x & 31) & ~3;
-                    const float x0 = __shfl_sync(0xffffffffu, v[j][i], lead), x1 = __shfl_sync(0xffffffffu, v[j][i], lead + 1);
-                    const float x2 = __shfl_sync(0xffffffffu, v[j][i], lead + 2), x3 = __shfl_sync(0xffffffffu, v[j][i], lead + 3);
-                    const float t = x0 + x1, b = x0 - x1;
-                    v[j][i] = q == 0 ? (t + x2) - x3 : q == 1 ? (t - x2) + x3 : q == 2 ? (b + x2) + x3 : (x2 - b) + x3;
-                }
-            }
-            uint32_t(&u)[4][16] = reinterpret_cast<uint32_t(&)[4][16]>(v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) radix4(u[0][i], u[1][i], u[2][i], u[3][i]);
-            if (in) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) store_row16(dst + 64 * j + 16 * q, u[j]);
-            }
-        } else {
-#pragma unroll 1
-            for (int j = 0; j < 4; ++j) {
-                if (!in || col + 64 * j + 16 * q >= a.k) continue;
-                float4 sum[4] = {};
-                for (int p = 0; p < a.split; ++p) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float4 x = __ldcs(reinterpret_cast<const float4 *>(src + p * part + 64 * j + 16 * q + 4 * c));
-                        sum[c].x += x.x;
-                        sum[c].y += x.y;
-                        sum[c].z += x.z;
-                        sum[c].w += x.w;
-                    }
-                }
-                store_row16(dst + 64 * j + 16 * q, reinterpret_cast<const uint32_t *>(sum));
-            }
+// Sums of the parts, in order, rounded: eight columns a thread.
+__global__ void __launch_bounds__(256) grad_join_kernel(const GradArgs a) {
+    const int64_t total = static_cast<int64_t>(a.m) * a.k;
+    for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 8; i < total; i += gridDim.x * 2048ll) {
+        float4 lo = make_float4(0.0f, 0.0f, 0.0f, 0.0f), hi = lo;
+#pragma unroll 4
+        for (int p = 0; p < a.split; ++p) {
+            const float4 *src = reinterpret_cast<const float4 *>(a.partials + p * total + i);
+            const float4 x = __ldcs(src), y = __ldcs(src + 1);
+            lo.x += x.x;
+            lo.y += x.y;
+            lo.z += x.z;
+            lo.w += x.w;
+            hi.x += y.x;
+            hi.y += y.y;
+            hi.z += y.z;
+            hi.w += y.w;
         }
+        *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + i) =
+            make_uint4(pack_bf16x2(lo.x, lo.y), pack_bf16x2(lo.z, lo.w), pack_bf16x2(hi.x, hi.y), pack_bf16x2(hi.z, hi.w));
     }
 }
 
 cudaError_t launch_grad_join(const GradArgs &a, int num_sms, cudaStream_t stream) {
-    const int64_t threads = static_cast<int64_t>(a.m) * ((a.k + 255) / 256) * 4;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((threads + 127) / 128, num_sms * 16ll));
-    if (a.rotation)
-        grad_join_kernel<true><<<grid, 128, 0, stream>>>(a);
-    else
-        grad_join_kernel<false><<<grid, 128, 0, stream>>>(a);
+    const int64_t threads = static_cast<int64_t>(a.m) * a.k / 8;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((threads + 255) / 256, num_sms * 8ll));
+    grad_join_kernel<<<grid, 256, 0, stream>>>(a);
     return cudaGetLastError();
 }
 

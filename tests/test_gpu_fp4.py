@@ -248,15 +248,15 @@ def test_grad_input(k, fmt, m, n, width, rotation):
     dx = k.turing_fp4_linear_grad_input(g.cuda(), w, w_s, w_r, rotation)
     gd, wd = g.double().numpy(), wv * wr[:, None].astype(np.float64)
     exact = gd @ wd
-    # Sums: one truncation per K = 16 instruction and four levels inside; rotation: 8 fp32 additions
-    # of values bounded by the rotated magnitudes; then half a bf16 step.
+    # Sums: one truncation per K = 16 instruction and four levels inside; rotation: four stages of three
+    # fp32 additions, of values bounded by the rotated magnitudes; up to 16 parts added; then half a bf16 step.
     mags = np.abs(gd) @ np.abs(wd)
-    off = (-(-n // 16) + 4) * 2.0**-23 * mags
+    off = (-(-n // 16) + 4) * 2.0**-23 * mags + 16 * 2.0**-24 * mags
     if rotation:
         r = oracle.rotation_matrix()
         exact = (exact.reshape(-1, 256) @ r).reshape(m, width)
         mixed = (mags.reshape(-1, 256) @ np.abs(r)).reshape(m, width)
-        off = (off.reshape(-1, 256) @ np.abs(r)).reshape(m, width) + 12 * 2.0**-24 * mixed
+        off = (off.reshape(-1, 256) @ np.abs(r)).reshape(m, width) + (12 + 16) * 2.0**-24 * mixed
     assert dx.dtype == torch.bfloat16 and dx.shape == (m, width)
     got = dx.double().cpu().numpy()
     bound = HALF_BF16 * (np.abs(exact) + off) + off + 1e-37
