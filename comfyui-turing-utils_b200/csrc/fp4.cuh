@@ -98,18 +98,19 @@ int linear_pair_threads();
 // Gradient with respect to the input: dx[m, k] = grad[m, n] w[n, k], rotated back.
 struct GradArgs {
     void *out;        // bf16 [m, k]
-    float *partials;  // [split][m][k] where split > 1
+    float *partials;  // sums of the split tiles' parts: [tile][part][256 columns][256 rows]
     uint32_t *err;
     int m, n, k;
     int rotation;
-    int split;  // parts of the sum over n
+    int whole;  // tiles that are not split, the first ones
+    int split;  // parts of the others' sums over n
 };
 constexpr int kGradCols = 256;
 int grad_pair_smem();
 const void *grad_pair_kernel(int rotation);
 int grad_pair_threads();
 // Joins the partial sums of a split product: sum over parts in order, one rounding.
-cudaError_t launch_grad_join(const GradArgs &a, int num_sms, cudaStream_t stream);
+cudaError_t launch_grad_join(const GradArgs &a, cudaStream_t stream);
 
 }  // namespace fp4
 }  // namespace ctu

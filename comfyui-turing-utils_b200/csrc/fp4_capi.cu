@@ -145,26 +145,34 @@ SmemPlan g_small_plan[8];
 PairPlan g_linear_plan[2];
 PairPlan g_grad_plan[2];
 
-// Parts of the gradient's sum over n.  Tiles that do not fill the pairs of a B200 (74) are cut along n
-// while that lowers the rounds of pairs, counted in 64-row stages (0.28 us), plus the write and read of the
-// parts' fp32 sums at 5 TB/s.  333 x 13824 x 5120 is 40 tiles of 216 stages: three parts are two rounds of 72.
-// Depends on the sizes alone, so that the workspace and the sums' order do.
-int64_t grad_split(int64_t m, int64_t n, int64_t k) {
+// The gradient's tiles beyond the last full round of pairs (74 on a B200) are split along n, into as many
+// parts as lower the time of that round: stages of 64 rows (0.28 us) over the rounds that the parts need,
+// plus the write and read of their fp32 sums at 5 TB/s (256 KB a part) and of a launch.  4096 x 5120 x 5120
+// is 320 tiles, four rounds and 24 tiles in three parts each; 333 x 13824 x 5120 is 40 tiles of 216 stages in
+// three parts.  Depends on the sizes alone, so that the workspace and the sums' order do.
+struct GradPlan {
+    int64_t tiles, whole, split;
+};
+
+GradPlan grad_plan(int64_t m, int64_t n, int64_t k) {
     constexpr int64_t kPairs = 74;
-    const int64_t tiles = ((m + fp4::kPairRows - 1) / fp4::kPairRows) * ((k + fp4::kGradCols - 1) / fp4::kGradCols);
+    GradPlan p{};
+    p.tiles = ((m + fp4::kPairRows - 1) / fp4::kPairRows) * ((k + fp4::kGradCols - 1) / fp4::kGradCols);
     const int64_t stages = (n + 63) / 64;
-    if (tiles >= kPairs) return 1;
-    int64_t best = 1;
+    p.whole = p.tiles / kPairs * kPairs;
+    p.split = 1;
+    const int64_t tail = p.tiles - p.whole;
     double cost = static_cast<double>(stages);
-    for (int64_t s = 2; s <= 16 && 2 * s <= stages; ++s) {
-        const double rounds = static_cast<double>((tiles * s + kPairs - 1) / kPairs * ((stages + s - 1) / s));
-        const double c = rounds + 12.0 + static_cast<double>(s * m * k) * 5.7e-6;
+    for (int64_t s = 2; tail > 0 && s <= 16 && 2 * s <= stages; ++s) {
+        const double rounds = static_cast<double>((tail * s + kPairs - 1) / kPairs * ((stages + s - 1) / s));
+        const double c = rounds + 12.0 + 0.374 * static_cast<double>(s * tail);
         if (c < cost) {
             cost = c;
-            best = s;
+            p.split = s;
         }
     }
-    return best;
+    if (p.split == 1) p.whole = p.tiles;
+    return p;
 }
 
 }  // namespace
@@ -317,8 +325,8 @@ int ctu_debug_set_fp4_kernel(int which) {
 
 int64_t ctu_fp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    const int64_t split = grad_split(m, n, k);
-    return 2 * n * k + (split > 1 ? split * m * k * 4 : 0);
+    const GradPlan p = grad_plan(m, n, k);
+    return 2 * n * k + (p.tiles - p.whole) * p.split * fp4::kPairRows * fp4::kGradCols * 4;
 }
 
 int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t *w_block_scales, const float *w_scale,
@@ -348,7 +356,7 @@ int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     fp4::DequantArgs d{w, w_block_scales, w_scale, workspace, n, static_cast<int>(k), format, w_scale_count == 1 ? 1 : 0,
                        CTU_DTYPE_BF16, q.num_sms};
-    CUtensorMap map_a, map_b;
+    CUtensorMap map_a, map_b, map_out;
     const uint32_t box_a[2] = {64, 128}, box_b[2] = {64, 64};
     const uint64_t dims_a[2] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m)};
     const uint64_t dims_b[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)};
@@ -359,20 +367,26 @@ int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t 
     if (int rc = encode_tiled(&map_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, workspace, dims_b, stride_b, box_b,
                               CU_TENSOR_MAP_SWIZZLE_128B))
         return rc;
+    const uint32_t box_out[2] = {64, 32};
+    const uint64_t dims_out[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(m)};
+    if (int rc = encode_tiled(&map_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dx, dims_out, stride_b, box_out,
+                              CU_TENSOR_MAP_SWIZZLE_128B))
+        return rc;
     const void *kernel = fp4::grad_pair_kernel(rotation);
     int clusters = 0;
     if (int rc = pair_clusters(g_grad_plan[rotation ? 1 : 0], kernel, fp4::grad_pair_threads(), fp4::grad_pair_smem(), q,
                                &clusters))
         return rc;
     CTU_CUDA(fp4::launch_dequantize(d, s));
-    const int split = static_cast<int>(grad_split(m, n, k));
+    const GradPlan plan = grad_plan(m, n, k);
     fp4::GradArgs args{dx, reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + 2 * n * k), err,
-                       static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), rotation, split};
-    void *params[] = {&map_a, &map_b, &args};
+                       static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), rotation, static_cast<int>(plan.whole),
+                       static_cast<int>(plan.split)};
+    void *params[] = {&map_a, &map_b, &map_out, &args};
     if (int rc = launch_pairs(kernel, fp4::grad_pair_threads(), fp4::grad_pair_smem(),
-                              std::min<int64_t>(tiles * split, clusters), params, s))
+                              std::min<int64_t>(plan.whole + (plan.tiles - plan.whole) * plan.split, clusters), params, s))
         return rc;
-    if (split > 1) CTU_CUDA(fp4::launch_grad_join(args, q.num_sms, s));
+    if (plan.whole < plan.tiles) CTU_CUDA(fp4::launch_grad_join(args, s));
     return CTU_OK;
 }
 

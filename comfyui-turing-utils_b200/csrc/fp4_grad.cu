@@ -10,13 +10,13 @@
 // row and takes the strides 1, 4 and 16 in registers, 64 columns at a time, writes them back to
 // tensor memory, and takes stride 64 from there.  Rounded once, to bf16.
 //
-// With too few tiles to fill the GPU the sum over n is split; each part leaves fp32 sums (rotated: the
-// rotation is linear), and a second kernel adds them in order and rounds.
+// Tiles beyond the last full round of pairs are split along n; each part leaves its fp32 sums (rotated: the
+// rotation is linear), tile by tile and a column's rows together, so that a warp's store is 128 contiguous
+// bytes; a second kernel adds the parts in order, transposes and rounds.  Whole tiles go out through staged
+// tile stores.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
-
-#include <algorithm>
 
 #include "fp4.cuh"
 #include "fp4_mma.cuh"
@@ -27,13 +27,15 @@ namespace fp4 {
 
 namespace {
 
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kStageK = 64;  // bf16 values of the contraction per stage: 128 bytes
 constexpr int kABytes = 128 * 128;
 constexpr int kBBytes = 128 * 128;
 constexpr int kBOffset = kStages * kABytes;
-constexpr int kStructOffset = kBOffset + kStages * kBBytes;
+constexpr int kStageOutOffset = kBOffset + kStages * kBBytes;
 constexpr int kEpilogueWarps = 4;
+constexpr int kPieceBytes = 32 * 128;  // a warp's 32 rows of 64 output columns
+constexpr int kStructOffset = kStageOutOffset + kEpilogueWarps * 4 * kPieceBytes;
 constexpr int kThreadCount = 32 * (2 + kEpilogueWarps);
 constexpr int kTmemCols = 512;
 
@@ -81,20 +83,21 @@ __device__ __forceinline__ void radix4(uint32_t &r0, uint32_t &r1, uint32_t &r2,
     r3 = __float_as_uint((x2 - b) + x3);
 }
 
-__device__ __forceinline__ void store_row16(__nv_bfloat16 *dst, const uint32_t *r) {
+// 16 columns of a staged row (128-byte swizzle), `c` the quarter of the piece's 64.
+__device__ __forceinline__ void stage16(uint32_t piece, int c, uint32_t lane, const uint32_t *r) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (uint32_t q = 0; q < 2; ++q) {
         uint32_t p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             p[j] = pack_bf16x2(__uint_as_float(r[8 * q + 2 * j]), __uint_as_float(r[8 * q + 2 * j + 1]));
-        reinterpret_cast<uint4 *>(dst)[q] = make_uint4(p[0], p[1], p[2], p[3]);
+        st_shared_v4(piece + 128u * lane + (((2u * c + q) ^ (lane & 7u)) << 4), p);
     }
 }
-
+// 16 columns of a part's sums: a column's 256 rows lie together.
 __device__ __forceinline__ void store_sums16(float *dst, const uint32_t *r) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) reinterpret_cast<uint4 *>(dst)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+    for (int j = 0; j < 16; ++j) dst[j * 256] = __uint_as_float(r[j]);
 }
 
 }  // namespace
@@ -102,7 +105,7 @@ __device__ __forceinline__ void store_sums16(float *dst, const uint32_t *r) {
 template <bool kRotate>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     fp4_grad_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                         const GradArgs args) {
+                         const __grid_constant__ CUtensorMap tmap_out, const GradArgs args) {
     constexpr uint32_t kStageTx = 2 * (kABytes + kBBytes);
     // B: 64 rows of n by 128 columns of k, as two pieces of 64 columns; eight rows 1024 bytes apart.
     constexpr uint32_t kDescBHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -119,16 +122,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     const int num_pairs = gridDim.x >> 1;
     const int num_n = (args.k + kGradCols - 1) / kGradCols;
     const int num_m = (args.m + kPairRows - 1) / kPairRows;
-    const int num_tiles = num_m * num_n * args.split;
+    const int tiles = num_m * num_n;
+    const int num_tiles = args.whole + (tiles - args.whole) * args.split;  // work items
     const int nk_all = (args.n + kStageK - 1) / kStageK;
-    // Work item t: part t % split of the sum of tile t / split, over stages [first, last).
+    // Work items: the first `whole` tiles, then the parts of the others.  Item t sums stages [first, last) of
+    // its tile; `part` counts the parts' sums, -1 for a whole tile.
     auto work_item = [&](int t, int &m_tile, int &n_tile, int &part, int &first, int &last) {
-        part = t % args.split;
-        const int tile = t / args.split;
-        m_tile = tile / num_n;
-        n_tile = tile - m_tile * num_n;
-        first = static_cast<int>(static_cast<int64_t>(nk_all) * part / args.split);
-        last = static_cast<int>(static_cast<int64_t>(nk_all) * (part + 1) / args.split);
+        int tile = t;
+        part = -1;
+        first = 0;
+        last = nk_all;
+        if (t >= args.whole) {
+            part = t - args.whole;
+            tile = args.whole + part / args.split;
+            const int i = part % args.split;
+            first = static_cast<int>(static_cast<int64_t>(nk_all) * i / args.split);
+            last = static_cast<int>(static_cast<int64_t>(nk_all) * (i + 1) / args.split);
+        }
+        n_tile = tile / num_m;  // down the rows first: pairs at work share panels of the weights
+        m_tile = tile - n_tile * num_m;
     };
 
     if (threadIdx.x == 0) {
@@ -151,6 +163,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
+        prefetch_tmap(&tmap_out);
     }
     tc_fence_before();
     __syncthreads();
@@ -237,26 +250,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     } else {
         const int quad = warp & 3;
         const uint32_t leader_empty = mapa_shared(smem_u32(&S.acc_empty[0]), 0u);
+        const uint32_t staged = smem_u32(smem + kStageOutOffset + (warp - 2) * 4 * kPieceBytes);
+        const uint64_t policy = evict_first_policy();
         bool alive = true;
         int local = 0;
         for (int t = pair; t < num_tiles; t += num_pairs, ++local) {
             const int ab = local & 1;
-            if (alive) {
-                int ok = 1;
-                if (lane == 0) ok = guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum) ? 1 : 0;
-                alive = __shfl_sync(0xffffffffu, ok, 0) != 0;
-            }
+            if (alive) alive = __all_sync(0xffffffffu, guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum));
             if (!alive) continue;
             tc_fence_after();
             int m_tile, n_tile, part, first, last;
             work_item(t, m_tile, n_tile, part, first, last);
-            const int m = m_tile * kPairRows + static_cast<int>(rank) * 128 + quad * 32 + lane;
+            const int row = static_cast<int>(rank) * 128 + quad * 32;
+            const int m = m_tile * kPairRows + row;
             const int n0 = n_tile * kGradCols;
-            const bool row_ok = m < args.m;
             const uint32_t acc = tmem_base + static_cast<uint32_t>(ab * kGradCols) + (static_cast<uint32_t>(quad * 32) << 16);
-            __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(args.out) + static_cast<int64_t>(m) * args.k + n0;
-            float *sums = args.partials + (static_cast<int64_t>(part) * args.m + m) * args.k + n0;
-            const bool parts = args.split > 1;
+            float *sums = args.partials + static_cast<int64_t>(max(part, 0)) * (kPairRows * kGradCols) + row + lane;
+            if (part < 0) {  // the staged pieces are free once the last stores out of them have read them
+                if (lane == 0) bulk_wait_read_all();
+                __syncwarp();
+            }
             if constexpr (kRotate) {
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -288,42 +301,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     tmem_st_32x32b_x32(acc + c * 64 + 32, hi);
                 }
                 tmem_st_wait();
+            }
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t r[4][16];
+            for (int c = 0; c < 4; ++c) {  // 16 columns of each piece of 64
+                uint32_t r[4][16];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x16(acc + q * 64 + c * 16, r[q]);
-                    tmem_ld_wait();
+                for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x16(acc + q * 64 + c * 16, r[q]);
+                tmem_ld_wait();
+                if constexpr (kRotate) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) radix4(r[0][i], r[1][i], r[2][i], r[3][i]);
-                    if (row_ok) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            if (parts)
-                                store_sums16(sums + q * 64 + c * 16, r[q]);
-                            else
-                                store_row16(dst + q * 64 + c * 16, r[q]);
-                        }
-                    }
                 }
-            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (part < 0)
+                        stage16(staged + q * kPieceBytes, c, lane, r[q]);
+                    else
+                        store_sums16(sums + (q * 64 + c * 16) * kPairRows, r[q]);
+                }
+            }
+            if (part < 0) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0 && m < args.m) {
 #pragma unroll 1
-                for (int c = 0; c < 16; ++c) {
-                    uint32_t r[16];
-                    tmem_ld_32x32b_x16(acc + c * 16, r);
-                    tmem_ld_wait();
-                    if (row_ok && n0 + c * 16 < args.k) {
-                        if (parts)
-                            store_sums16(sums + c * 16, r);
-                        else
-                            store_row16(dst + c * 16, r);
-                    }
+                    for (int q = 0; q < 4; ++q)
+                        if (n0 + q * 64 < args.k) tma_store_2d(&tmap_out, staged + q * kPieceBytes, n0 + q * 64, m, policy);
+                    bulk_commit();
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(leader_empty + static_cast<uint32_t>(ab * sizeof(uint64_t)));
         }
+        if (lane == 0) bulk_wait_all();  // the staged rows leave shared memory before the CTA does
     }
 
     tc_fence_before();
@@ -335,33 +346,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     }
 }
 
-// Sums of the parts, in order, rounded: eight columns a thread.
+// Sums of a tile's parts, in order, rounded: 64 columns by 32 rows a block, through shared memory.
 __global__ void __launch_bounds__(256) grad_join_kernel(const GradArgs a) {
-    const int64_t total = static_cast<int64_t>(a.m) * a.k;
-    for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 8; i < total; i += gridDim.x * 2048ll) {
-        float4 lo = make_float4(0.0f, 0.0f, 0.0f, 0.0f), hi = lo;
-#pragma unroll 4
-        for (int p = 0; p < a.split; ++p) {
-            const float4 *src = reinterpret_cast<const float4 *>(a.partials + p * total + i);
-            const float4 x = __ldcs(src), y = __ldcs(src + 1);
-            lo.x += x.x;
-            lo.y += x.y;
-            lo.z += x.z;
-            lo.w += x.w;
-            hi.x += y.x;
-            hi.y += y.y;
-            hi.z += y.z;
-            hi.w += y.w;
-        }
-        *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + i) =
-            make_uint4(pack_bf16x2(lo.x, lo.y), pack_bf16x2(lo.z, lo.w), pack_bf16x2(hi.x, hi.y), pack_bf16x2(hi.z, hi.w));
+    __shared__ float block[64][33];
+    const int num_m = (a.m + kPairRows - 1) / kPairRows;
+    const int tile = blockIdx.x >> 5;  // of the split ones
+    const int col0 = (blockIdx.x & 3) * 64, row0 = (blockIdx.x >> 2 & 7) * 32;
+    const int m = (a.whole + tile) % num_m * kPairRows + row0;
+    const int k = (a.whole + tile) / num_m * kGradCols + col0;
+    if (m >= a.m || k >= a.k) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int64_t kTile = kPairRows * kGradCols;
+    const float *src = a.partials + tile * a.split * kTile + col0 * kPairRows + row0 + lane;
+    float sum[8] = {};
+#pragma unroll 2
+    for (int p = 0; p < a.split; ++p) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += __ldcs(src + p * kTile + (warp * 8 + i) * kPairRows);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) block[warp * 8 + i][lane] = sum[i];
+    __syncthreads();
+    const int c = 2 * lane;
+    if (k + c >= a.k) return;  // K is even
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = warp * 4 + i;
+        if (m + r < a.m)
+            *reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.out) + static_cast<int64_t>(m + r) * a.k + k + c) =
+                pack_bf16x2(block[c][r], block[c + 1][r]);
     }
 }
 
-cudaError_t launch_grad_join(const GradArgs &a, int num_sms, cudaStream_t stream) {
-    const int64_t threads = static_cast<int64_t>(a.m) * a.k / 8;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((threads + 255) / 256, num_sms * 8ll));
-    grad_join_kernel<<<grid, 256, 0, stream>>>(a);
+cudaError_t launch_grad_join(const GradArgs &a, cudaStream_t stream) {
+    const int tiles = ((a.m + kPairRows - 1) / kPairRows) * ((a.k + kGradCols - 1) / kGradCols) - a.whole;
+    grad_join_kernel<<<static_cast<unsigned>(tiles) * 32u, 256, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
