@@ -767,20 +767,26 @@ _FP4_BY_SCALE = {torch.float8_e4m3fn: (0, 16), torch.float8_e8m0fnu: (1, 32)}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+_FUNCTIONS: dict = {}  # C entries looked up once
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """One C-ABI call on `device`'s current stream (appended as the last argument)."""
-    fn = getattr(_lib.load(), name)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_lib.load(), name)
     index = device.index
     if index == torch.cuda.current_device():
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
-    _lib.check(rc)
+    if rc:
+        _lib.check(rc)
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    return _aligned(t.contiguous())
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else _aligned(t.contiguous())
 
 
 def _fp4_tiles(rows: int, k: int, block: int) -> tuple[int, int, int, int]:
@@ -789,22 +795,23 @@ def _fp4_tiles(rows: int, k: int, block: int) -> tuple[int, int, int, int]:
 
 def _fp4_operand(codes: torch.Tensor, block_scale: torch.Tensor, name: str):
     """(codes, scales, rows, k, format) of one quantized operand, checked."""
-    if not codes.is_cuda or codes.dim() != 2 or codes.dtype != torch.uint8:
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_cuda:
         raise RuntimeError(f"{name} must be a 2D uint8 CUDA tensor of packed FP4 codes")
     fmt = _FP4_BY_SCALE.get(block_scale.dtype)
     if fmt is None:
         raise RuntimeError(f"{name} block scales must be float8_e4m3fn (nvfp4) or float8_e8m0fnu (mxfp4)")
     rows, half = codes.shape
     k = 2 * half
-    if k <= 0 or k % 32:
+    if k <= 0 or k & 31:
         raise RuntimeError(f"{name} width must be positive and divisible by 32")
-    if block_scale.device != codes.device or block_scale.shape != _fp4_tiles(rows, k, fmt[1]):
+    if block_scale.shape != _fp4_tiles(rows, k, fmt[1]) or block_scale.get_device() != codes.get_device():
         raise RuntimeError(f"{name} block scales must be {list(_fp4_tiles(rows, k, fmt[1]))} tiles on the same device")
     return _dense(codes), _dense(block_scale), rows, k, fmt[0]
 
 
-def _fp4_vector(t: torch.Tensor, count: int, device: torch.device, name: str, scalar: bool) -> torch.Tensor:
-    if t.dtype != torch.float32 or t.device != device or not (t.numel() == count or (scalar and t.numel() == 1)):
+def _fp4_vector(t: torch.Tensor, count: int, device: int, name: str, scalar: bool) -> torch.Tensor:
+    n = t.numel()
+    if t.dtype != torch.float32 or t.get_device() != device or not (n == count or (scalar and n == 1)):
         raise RuntimeError(f"{name} must be float32 on the same device, {count} values" + (" or one" if scalar else ""))
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no gradient here: detach it")
@@ -840,7 +847,7 @@ def fp4_dequantize(codes, block_scale, scale, out_dtype=torch.bfloat16):
     codes, block_scale, rows, k, fmt = _fp4_operand(codes, block_scale, "codes")
     if out_dtype not in _NORM_TYPES:
         raise RuntimeError("FP4 dequantizer output must be float16, bfloat16, or float32")
-    scale = _fp4_vector(scale, rows, codes.device, "row scale", True)
+    scale = _fp4_vector(scale, rows, codes.get_device(), "row scale", True)
     out = torch.empty((rows, k), dtype=out_dtype, device=codes.device)
     _call(codes.device, "ctu_fp4_dequantize", codes.data_ptr(), block_scale.data_ptr(), scale.data_ptr(), scale.numel(),
           rows, k, fmt, _NORM_TYPES[out_dtype], out.data_ptr())
@@ -852,14 +859,15 @@ def fp4_linear(activation, weight, activation_block_scale, weight_block_scale, a
     a, a_bs, m, k, fmt = _fp4_operand(activation, activation_block_scale, "activation")
     w, w_bs, n, wk, wfmt = _fp4_operand(weight, weight_block_scale, "weight")
     dev = a.device
-    if w.device != dev:
+    index = dev.index
+    if w.get_device() != index:
         raise RuntimeError("all FP4 linear tensors must use the same CUDA device")
     if wk != k or wfmt != fmt:
         raise RuntimeError("activation and weight must have the same K and the same FP4 format")
-    a_s = _fp4_vector(activation_scale, m, dev, "activation scale", False)
-    w_s = _fp4_vector(weight_scale, n, dev, "weight scale", True)
+    a_s = _fp4_vector(activation_scale, m, index, "activation scale", False)
+    w_s = _fp4_vector(weight_scale, n, index, "weight scale", True)
     if bias is not None:
-        bias = _fp4_vector(bias, n, dev, "bias", False)
+        bias = _fp4_vector(bias, n, index, "bias", False)
     out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
     _call(dev, "ctu_fp4_linear", a.data_ptr(), w.data_ptr(), a_bs.data_ptr(), w_bs.data_ptr(), a_s.data_ptr(),
           w_s.data_ptr(), w_s.numel(), None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k, fmt)
@@ -878,7 +886,7 @@ def fp4_linear_grad_input(grad_output, weight, weight_block_scale, weight_scale,
         raise RuntimeError("FP4 linear gradient requires N divisible by 8")
     if rotation not in (0, 256) or k % (rotation or 32):
         raise RuntimeError("FP4 linear gradient rotation must be 0, or 256 with K divisible by it")
-    w_s = _fp4_vector(weight_scale, n, dev, "weight scale", True)
+    w_s = _fp4_vector(weight_scale, n, dev.index, "weight scale", True)
     g = _dense(grad_output)
     m = g.size(0)
     dx = torch.empty((m, k), dtype=torch.bfloat16, device=dev)
