@@ -56,7 +56,9 @@ constexpr int kBackwardBlock = 640;  // times 96 registers: an SM's register fil
 // A thread's part of a row: kPieces loads of kVec elements (16 bytes), or of single elements where rows
 // do not start on 16 bytes.  Elements are handled in pairs; a group is the pairs that share a load (or
 // two single loads).
-template <typename T, int kVec, int kPieces>
+// kThreads: of the team, 0 where only the launch knows.  A team is no larger than its row needs, so of wide
+// loads only the last one can lie beyond the row.
+template <typename T, int kVec, int kPieces, int kThreads>
 struct Part {
     static constexpr bool kWide = kVec > 1;
     static constexpr int kGroups = kWide ? kPieces : kPieces / 2;
@@ -64,10 +66,14 @@ struct Part {
     uint4 wide[kWide ? kPieces : 1];
     T single[kWide ? 1 : kPieces];
 
-    static __device__ __forceinline__ int column(int piece) { return (threadIdx.x + piece * blockDim.x) * kVec; }
+    static __device__ __forceinline__ int column(int piece) {
+        return threadIdx.x * kVec + piece * (kThreads ? kThreads : static_cast<int>(blockDim.x)) * kVec;
+    }
     // Whether a group's first element (all of them, with wide loads) and second element exist.
-    static __device__ __forceinline__ bool first(int g, int h) { return column(kWide ? g : 2 * g) < h; }
-    static __device__ __forceinline__ bool second(int g, int h) { return column(kWide ? g : 2 * g + 1) < h; }
+    static __device__ __forceinline__ bool first(int g, int h) {
+        return kWide ? g + 1 < kPieces || column(g) < h : column(2 * g) < h;
+    }
+    static __device__ __forceinline__ bool second(int g, int h) { return kWide ? first(g, h) : column(2 * g + 1) < h; }
 
     // What does not exist reads as zero.
     __device__ __forceinline__ void load(const T *row, int h) {
@@ -75,7 +81,7 @@ struct Part {
         for (int p = 0; p < kPieces; ++p) {
             const int c = column(p);
             if constexpr (kWide)
-                wide[p] = c < h ? __ldcs(reinterpret_cast<const uint4 *>(row + c)) : make_uint4(0u, 0u, 0u, 0u);
+                wide[p] = first(p, h) ? __ldcs(reinterpret_cast<const uint4 *>(row + c)) : make_uint4(0u, 0u, 0u, 0u);
             else
                 single[p] = c < h ? row[c] : from_f<T>(0.0f);
         }
@@ -138,7 +144,7 @@ struct Part {
 // CTA, so not where occupancy counts); otherwise the CTA is one team, or every team one warp.
 template <bool kNamed>
 struct TeamSum {
-    float2 (*part)[16];  // [2][16] of this team
+    float2 (*part)[20];  // [2][20] of this team
     int warps;
     int barrier;
     int flip = 0;
@@ -159,7 +165,9 @@ struct TeamSum {
         else
             __syncthreads();
         v = buf[0];
-        for (int i = 1; i < warps; ++i) {
+#pragma unroll
+        for (int i = 1; i < 20; ++i) {
+            if (i >= warps) break;
             v.x += buf[i].x;
             v.y += buf[i].y;
         }
@@ -174,17 +182,21 @@ __device__ __forceinline__ float both(f32x2 v) {
 }
 
 // blockDim = (threads of a team, teams).
-template <typename T, int kVec, int kPieces>
+// One team a CTA, or four teams of one warp.
+template <typename T, int kVec, int kPieces, int kThreads>
 __global__ void __maxnreg__(64) team_forward_kernel(const AffineArgs a) {
-    using P = Part<T, kVec, kPieces>;
-    __shared__ float2 part[2][16];
+    using P = Part<T, kVec, kPieces, kThreads>;
+    constexpr int kTeams = kThreads == 32 ? 4 : 1;
+    __shared__ float2 part[2][20];
     const int h = a.hidden;
-    const int team = threadIdx.y;
-    TeamSum<false> sum{part, static_cast<int>(blockDim.x >> 5), 1 + team};
+    const int team = kTeams > 1 ? threadIdx.y : 0;
+    TeamSum<false> sum{part, kThreads ? kThreads / 32 : static_cast<int>(blockDim.x >> 5), 0};
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.y;
+    const void *weight = a.weight, *bias = a.bias;
+    const float epsilon = a.epsilon;
+    const int64_t rows = a.rows, stride = static_cast<int64_t>(gridDim.x) * kTeams;
     const float inv_h = 1.0f / static_cast<float>(h);
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + team; r < a.rows; r += stride) {
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kTeams + team; r < rows; r += stride) {
         P x;
         x.load(static_cast<const T *>(a.x) + r * h, h);
         f32x2 s = pk2(0.0f, 0.0f);
@@ -210,7 +222,7 @@ __global__ void __maxnreg__(64) team_forward_kernel(const AffineArgs a) {
             }
         }
         const float var = sum(make_float2(both(q), 0.0f)).x * inv_h;
-        const float rstd = 1.0f / sqrtf(var + a.epsilon);
+        const float rstd = 1.0f / sqrtf(var + epsilon);
         if (threadIdx.x == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -220,8 +232,8 @@ __global__ void __maxnreg__(64) team_forward_kernel(const AffineArgs a) {
         for (int g = 0; g < P::kGroups; ++g) {
             if (!P::first(g, h)) continue;
             f32x2 w[P::kPairs], b[P::kPairs], y[P::kPairs];
-            P::weights(a.weight, fp32, g, h, 1.0f, w);
-            P::weights(a.bias, fp32, g, h, 0.0f, b);
+            P::weights(weight, fp32, g, h, 1.0f, w);
+            P::weights(bias, fp32, g, h, 0.0f, b);
 #pragma unroll
             for (int i = 0; i < P::kPairs; ++i) y[i] = ffma2(fmul2(fsub2(x.pair(g, i), mean2), rstd2), w[i], b[i]);
             P::store(static_cast<T *>(a.out) + r * h, g, h, y);
@@ -231,8 +243,8 @@ __global__ void __maxnreg__(64) team_forward_kernel(const AffineArgs a) {
 
 template <typename T, int kVec, int kPieces, bool kParams>
 __global__ void __launch_bounds__(kBackwardBlock) team_backward_kernel(const AffineArgs a) {
-    using P = Part<T, kVec, kPieces>;
-    __shared__ float2 part[15][2][16];
+    using P = Part<T, kVec, kPieces, 0>;
+    __shared__ float2 part[15][2][20];
     extern __shared__ float joined[];  // [teams - 1][2 sums][elements of a thread][threads of a team]
     const int h = a.hidden;
     const int team = threadIdx.y;
@@ -492,16 +504,21 @@ TeamPlan team_plan(int64_t hidden, int bytes, bool aligned, bool backward) {
     // Pieces a thread, as many as its registers hold.  Forward (64): x alone.  Backward (96): two fp32 sums
     // an element, x, dy and the next row's x and dy; more pieces, without the next row, only for rows that
     // the CTA would not hold otherwise.
-    int most = p.vec == 1 ? (backward ? 8 : 16) : backward ? 2 : p.vec == 4 ? 8 : 5;
+    int most = p.vec == 1 ? (backward ? 8 : 16) : backward ? 2 : 5;
     if (backward && (count + most - 1) / most > block) most = p.vec == 1 ? 16 : p.vec == 4 ? 4 : 3;
-    const int64_t threads = ((count + most - 1) / most + 31) / 32 * 32;
+    int64_t threads = ((count + most - 1) / most + 31) / 32 * 32;
     if (threads > block) return p;
+    if (!backward && p.vec > 1) {  // a power of two, which the kernels know
+        int64_t t = 32;
+        while (t < threads) t *= 2;
+        threads = t;
+    }
     p.pieces = static_cast<int>((count + threads - 1) / threads);
     if (p.vec == 1) p.pieces = p.pieces <= 2 ? 2 : p.pieces <= 4 ? 4 : p.pieces <= 8 ? 8 : 16;
     p.threads = static_cast<int>(threads);
     // Forward CTAs are small (a team, or four of a warp) and many; a backward CTA fills an SM, with at most
     // fifteen teams (named barriers).
-    p.teams = static_cast<int>(backward ? std::min<int64_t>(15, block / threads) : threads == 32 ? 4 : 1);
+    p.teams = static_cast<int>(backward ? std::min<int64_t>(15, block / threads) : p.vec > 1 && threads == 32 ? 4 : 1);
     return p;
 }
 
@@ -530,11 +547,24 @@ cudaError_t with_pieces(int pieces, F f) {
         if constexpr (!kBackward) {
             if (pieces == 5) return f(std::integral_constant<int, 5>());
         }
-        if constexpr (!kBackward && kVec == 4) {
-            switch (pieces) {
-            case 6: return f(std::integral_constant<int, 6>());
-            case 7: return f(std::integral_constant<int, 7>());
-            case 8: return f(std::integral_constant<int, 8>());
+        return cudaErrorInvalidValue;
+    }
+}
+
+// Forward teams of wide loads: 32 threads and one to five pieces, or 64 to 512 and what those do not hold,
+// three to five.
+template <int kVec, int kPieces, typename F>
+cudaError_t with_threads(int threads, F f) {
+    if constexpr (kVec == 1) {
+        return f(std::integral_constant<int, 0>());
+    } else {
+        if (threads == 32) return f(std::integral_constant<int, 32>());
+        if constexpr (kPieces >= 3) {
+            switch (threads) {
+            case 64: return f(std::integral_constant<int, 64>());
+            case 128: return f(std::integral_constant<int, 128>());
+            case 256: return f(std::integral_constant<int, 256>());
+            case 512: return f(std::integral_constant<int, 512>());
             default: break;
             }
         }
@@ -568,8 +598,11 @@ cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream) {
         const unsigned grid = static_cast<unsigned>(
             std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, static_cast<int64_t>(a.num_sms) * 16));
         return with_shape<T, false>(plan, [&](auto vec, auto pieces) {
-            team_forward_kernel<T, vec, pieces><<<grid, dim3(plan.threads, plan.teams), 0, stream>>>(a);
-            return cudaGetLastError();
+            return with_threads<vec, pieces>(plan.threads, [&](auto threads) {
+                team_forward_kernel<T, vec, pieces, threads>
+                    <<<grid, dim3(plan.threads, plan.teams), 0, stream>>>(a);
+                return cudaGetLastError();
+            });
         });
     });
 }
