@@ -176,6 +176,30 @@ def int8_linear(
     return output.reshape(*original_shape[:-1], weight.shape[0])
 
 
+def convrot_fp4_linear(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    weight_block_scale: torch.Tensor,
+    weight_scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+    convrot: bool = True,
+    convrot_groupsize: int = 256,
+) -> torch.Tensor:
+    """ConvRot linear over [..., K] activations with 4-bit floating point weights (no reference op):
+    codes, block scale tiles and channel scales as ``turing_fp4_quantize`` gives them for the weight
+    with the same rotation.  Differentiable in bf16 ``x``."""
+    if convrot:
+        _require(convrot_groupsize == CONVROT_GROUP, f"ConvRot group size {convrot_groupsize}")
+    output = ops.turing_convrot_fp4_linear(
+        x.reshape(-1, x.shape[-1]), weight, weight_block_scale,
+        weight_scale.to(device=x.device, dtype=torch.float32),
+        None if bias is None else bias.to(device=x.device, dtype=torch.float32), CONVROT_GROUP if convrot else 0)
+    dtype = out_dtype or x.dtype
+    output = output if dtype == output.dtype else output.to(dtype)
+    return output.reshape(*x.shape[:-1], weight.shape[0])
+
+
 def codebook_w4a8_linear(
     x: torch.Tensor,
     qdata: torch.Tensor,

@@ -141,3 +141,13 @@ def segmented_rms_adaln(norm, x: torch.Tensor, shift: torch.Tensor, scale: torch
     shift = shift.to(device=x.device, dtype=x.dtype)
     table = segment_table(segments, x.shape[0], scale.shape[0], x.device)
     return ops.turing_segmented_rms_adaln(x, weight, scale, shift, table, float(norm.eps))
+
+
+def affine_layer_norm(norm: torch.nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
+    """``norm(x)`` on the B200 layer norm kernel, differentiable in ``x`` and the norm's parameters
+    (kept in fp32, or in the input's type).  Only a norm over the last dimension is taken."""
+    import comfyui_turing_utils_kernel as ops
+
+    if tuple(norm.normalized_shape) != (x.shape[-1],):
+        raise RuntimeError(f"layer norm over {tuple(norm.normalized_shape)} does not fit input {tuple(x.shape)}")
+    return ops.turing_layer_norm(x, norm.weight, norm.bias, float(norm.eps))

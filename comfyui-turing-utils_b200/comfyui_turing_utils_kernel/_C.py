@@ -902,7 +902,7 @@ def fp4_linear_grad_input(grad_output, weight, weight_block_scale, weight_scale,
 def _norm_vector(t, hidden, input, name):
     if t is None:
         return None
-    if t.device != input.device or t.numel() != hidden or t.dtype not in (input.dtype, torch.float32):
+    if t.device != input.device or t.shape != (hidden,) or t.dtype not in (input.dtype, torch.float32):
         raise RuntimeError(f"LayerNorm {name} must be [hidden] on the input's device, of its type or float32")
     return _dense(t)
 

@@ -136,6 +136,22 @@ int get_encoder(EncodeTiledFn *out) {
     return CTU_OK;
 }
 
+// Encodes a map.  The encoder is a driver call and needs a current context, which a thread that has made
+// no runtime call yet lacks (an autograd thread whose tensors came from the caching allocator): the
+// device is then made current, and the call repeated.
+CUresult encode_in_context(EncodeTiledFn enc, CUtensorMap *map, CUtensorMapDataType type, cuuint32_t rank, void *base,
+                           const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                           const cuuint32_t *elem, CUtensorMapSwizzle swizzle) {
+    for (int attempt = 0;; ++attempt) {
+        const CUresult r = enc(map, type, rank, base, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        int dev = 0;
+        if (r != CUDA_ERROR_INVALID_CONTEXT || attempt > 0 || cudaGetDevice(&dev) != cudaSuccess ||
+            cudaSetDevice(dev) != cudaSuccess)
+            return r;
+    }
+}
+
 int encode_tiled(CUtensorMap *map, CUtensorMapDataType type, int rank, const void *base, const uint64_t *dims,
                  const uint64_t *strides, const uint32_t *box, CUtensorMapSwizzle swizzle) {
     EncodeTiledFn enc;
@@ -147,9 +163,8 @@ int encode_tiled(CUtensorMap *map, CUtensorMapDataType type, int rank, const voi
         b[i] = box[i];
         if (i > 0) st[i - 1] = strides[i - 1];
     }
-    const CUresult r = enc(map, type, static_cast<cuuint32_t>(rank), const_cast<void *>(base), d, st, b, es,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r =
+        encode_in_context(enc, map, type, static_cast<cuuint32_t>(rank), const_cast<void *>(base), d, st, b, es, swizzle);
     if (r != CUDA_SUCCESS) return fail(CTU_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
     return CTU_OK;
 }
@@ -164,9 +179,7 @@ int encode_2d(CUtensorMap *map, CUtensorMapDataType type, int elem_bytes, const 
     const cuuint64_t strides[1] = {inner * static_cast<uint64_t>(elem_bytes)};
     const cuuint32_t box[2] = {box_inner, box_outer};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = encode_in_context(enc, map, type, 2, const_cast<void *>(base), dims, strides, box, estr, swizzle);
     if (r != CUDA_SUCCESS) return fail(CTU_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
     return CTU_OK;
 }

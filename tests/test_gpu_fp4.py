@@ -386,3 +386,124 @@ def test_refusals_on_the_gpu(k):
     ):
         with pytest.raises(RuntimeError):
             call()
+
+
+# ---------------------------------------------------------------------------- together
+@pytest.mark.parametrize("m", (1, 70, 300))
+def test_norm_linear_and_their_gradients_together(k, m):
+    """An adapter-tuning step through frozen weights: affine norm, rotated 4-bit linear, gradients of the
+    norm's input and parameters, against the formulas in 64 bits from the values that the layers hold."""
+    from comfyui_turing_utils_b200 import dispatch, fusions
+
+    width, n = 768, 200
+    norm = torch.nn.LayerNorm(width).cuda()  # fp32 master parameters
+    with torch.no_grad():
+        norm.weight.add_(0.1 * torch.randn(width, device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+        norm.bias.add_(0.1 * torch.randn(width, device="cuda", generator=torch.Generator("cuda").manual_seed(2)))
+    x = rows_like(m, width, 3).cuda().view(1, m, width).requires_grad_(True)
+    (w, w_s, w_r), wv, wr = quantized(n, width, "nvfp4", 4, 256)
+    h = fusions.affine_layer_norm(norm, x)
+    h.retain_grad()
+    y = dispatch.convrot_fp4_linear(h, w, w_s, w_r)
+    g = torch.randn(1, m, n, device="cuda", generator=torch.Generator("cuda").manual_seed(5)).bfloat16()
+    y.backward(g)
+    # The product of what the quantizer holds of h.
+    codes, scales, row = oracle.quantize(h.detach().view(m, width).float().cpu().numpy(), "nvfp4", 256)
+    av, ar, wr = oracle.values(codes, scales, "nvfp4"), row.astype(np.float64), wr.astype(np.float64)
+    exact = (av @ wv.T) * ar[:, None] * wr[None, :]
+    off = np.abs(y.detach().view(m, n).double().cpu().numpy() - exact)
+    assert (off <= linear_bound(av, ar, wv, wr, exact)).all()
+    # Its input gradient, then the norm's backward pass from the bf16 gradient that reaches it.
+    gd, wd, r = g.view(m, n).double().cpu().numpy(), wv * wr[:, None], oracle.rotation_matrix()
+    mags = (np.abs(gd) @ np.abs(wd)).reshape(-1, 256) @ np.abs(r)
+    dh = ((gd @ wd).reshape(-1, 256) @ r).reshape(m, width)
+    got = h.grad.view(m, width).double().cpu().numpy()
+    slack = (-(-n // 16) + 32) * 2.0**-23 * mags.reshape(m, width)
+    assert (np.abs(got - dh) <= HALF_BF16 * (np.abs(dh) + slack) + slack).all()
+    xd = x.detach().view(m, width).double().cpu().numpy()
+    mean, var = xd.mean(1, keepdims=True), xd.var(1, keepdims=True)
+    rstd = 1 / np.sqrt(var + norm.eps)
+    n_ = (xd - mean) * rstd
+    gw = got * norm.weight.detach().double().cpu().numpy()
+    dx = rstd * (gw - gw.mean(1, keepdims=True) - n_ * (gw * n_).mean(1, keepdims=True))
+    # fp32 statistics: under 2^-18 of the terms' magnitudes (768 terms, sums at most 40 deep), and a bf16 step.
+    terms = rstd * (np.abs(gw) + np.abs(gw).mean(1, keepdims=True) + np.abs(n_) * (np.abs(gw * n_)).mean(1, keepdims=True))
+    assert (np.abs(x.grad.view(m, width).double().cpu().numpy() - dx) <= HALF_BF16 * np.abs(dx) + 2.0**-16 * terms).all()
+    for grad, want, size in ((norm.weight.grad, (got * n_).sum(0), np.abs(got * n_).sum(0)), (norm.bias.grad, got.sum(0), np.abs(got).sum(0))):
+        assert (np.abs(grad.double().cpu().numpy() - want) <= 2.0**-16 * size + 1e-30).all()
+
+
+def test_captured_training_step(k):
+    """Forward and backward captured together, replayed on other data."""
+    m, n, width = 64, 256, 512
+    (w, w_s, w_r), _, _ = quantized(n, width, "mxfp4", 6, 256)
+    weight, bias = (torch.randn(width, device="cuda").requires_grad_(True) for _ in range(2))
+    g = torch.randn(m, n, device="cuda").bfloat16()
+
+    def step(x):
+        h = k.turing_layer_norm(x, weight, bias)
+        y = k.turing_convrot_fp4_linear(h, w, w_s, w_r, None, 256)
+        return (y.detach(), *torch.autograd.grad(y, (x, weight, bias), g))
+
+    first, second = (rows_like(m, width, s).cuda() for s in (1, 2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(first.clone().requires_grad_(True))
+    torch.cuda.current_stream().wait_stream(side)
+    static = first.clone().requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for data in (second, first):
+        with torch.no_grad():
+            static.copy_(data)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(data.clone().requires_grad_(True))
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_long_offsets(k):
+    """Rows whose elements lie beyond 2^31: the last ones come out as they do alone."""
+    width, rows = 13824, 156000  # 2.16e9 values
+    x = torch.zeros((rows, width), dtype=torch.bfloat16, device="cuda")
+    tail = rows_like(200, width, 1).cuda()
+    x[-200:] = tail
+    codes, tiles, row = k.turing_fp4_quantize(x, "nvfp4", 256)
+    some, _, some_row = k.turing_fp4_quantize(tail, "nvfp4", 256)
+    assert torch.equal(codes[-200:], some) and torch.equal(row[-200:], some_row)
+    (w, w_s, w_r), _, _ = quantized(40, width, "nvfp4", 2, 256)
+    y = k.turing_convrot_fp4_linear(x, w, w_s, w_r)
+    # The reference takes the same product kernel, over enough rows of it.
+    assert torch.equal(y[-200:], k.turing_convrot_fp4_linear(x[-1000:], w, w_s, w_r)[-200:])
+    back = k.turing_fp4_dequantize(codes, tiles, row)
+    del x, codes, tiles
+    last = k.turing_fp4_quantize(tail, "nvfp4", 256)
+    assert torch.equal(back[-200:], k.turing_fp4_dequantize(*last))
+    del back
+    z = torch.zeros((rows, width), dtype=torch.bfloat16, device="cuda")
+    z[-200:] = tail
+    assert torch.equal(k.turing_layer_norm(z)[-200:], k.turing_layer_norm(tail))
+
+
+def test_calls_from_a_fresh_thread(k):
+    """A thread that has made no CUDA call yet, its outputs served from the allocator's cache."""
+    import threading
+
+    (a, a_s, a_r), _, _ = quantized(300, 512, "nvfp4", 1)
+    (w, w_s, w_r), _, _ = quantized(256, 512, "nvfp4", 2)
+    x = rows_like(300, 512, 3).cuda()
+    g = torch.randn(300, 256, device="cuda").bfloat16()
+    calls = [lambda: k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r), lambda: k.turing_fp4_linear(a[:3], w, a_s[:1], w_s, a_r[:3], w_r),
+             lambda: k.turing_fp4_quantize(x, "mxfp4", 256)[0], lambda: k.turing_fp4_linear_grad_input(g, w, w_s, w_r, 256)]
+    want = [f() for f in calls]
+    for f in calls:
+        f()  # leaves blocks of the sizes in the cache
+    torch.cuda.synchronize()
+    for f, y in zip(calls, want):
+        got = []
+        t = threading.Thread(target=lambda: got.append(f()))  # noqa: B023
+        t.start()
+        t.join()
+        assert len(got) == 1 and torch.equal(got[0], y)
