@@ -3,7 +3,8 @@
 Usage: python comfyui-turing-utils_b200/build.py [--force] [-v]
 
 The shared library lands next to the Python package that loads it
-(comfyui_turing_utils_kernel/libctu_b200.so), so it travels with the source tree.
+(comfyui_turing_utils_kernel/libctu_b200.so), so it travels with the source tree; so do the
+torch bindings of the ops that are registered from C++ (libctu_torch.so).
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 OUT_DIR = HERE / "comfyui_turing_utils_kernel"
 LIB = OUT_DIR / "libctu_b200.so"
+TORCH_LIB = OUT_DIR / "libctu_torch.so"
 OBJ_DIR = HERE / "_build"
 
 SOURCES = ["capi.cu", "convrot_quant.cu", "convrot_quant_reg.cu", "convrot_quant_t4.cu", "convrot_quant_k8.cu", "gemm_i8.cu", "gemm_pair.cu", "gemm_grouped.cu", "dequant.cu", "noalloc.cu", "codebook.cu", "unpack_s4.cu", "norm_adaln.cu",
@@ -32,6 +34,19 @@ NVCC_FLAGS = [
     # Kernel templates are declared in headers and instantiated in their own .cu files.
     "-diag-suppress", "20281",
 ]
+
+
+def _torch_command(out: Path) -> list[str]:
+    """g++ line of the torch bindings, which call the C ABI of the library next to them."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda}/include",
+            str(CSRC / "torch_ops.cpp"), "-o", str(out), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+            f"-L{OUT_DIR}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
 
 
 def _nvcc() -> str:
@@ -73,6 +88,13 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link failed")
         os.replace(tmp, LIB)
+    if force or _stale(TORCH_LIB, [CSRC / "torch_ops.cpp", INCLUDE / "ctu_b200.h"]):
+        tmp = TORCH_LIB.with_suffix(f".so.{os.getpid()}.tmp")
+        res = subprocess.run(_torch_command(tmp), capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("g++ failed on the torch bindings")
+        os.replace(tmp, TORCH_LIB)
     return LIB
 
 

@@ -756,205 +756,3 @@ def int8_gemm_s32(activation, weight, out=None):
             _ptr(_aligned(activation)), _ptr(_aligned(weight)), _ptr(out), out.stride(0), m, n, k,
             _stream(activation.device)))
     return out
-
-
-# ----------------------------------------------------------------------------- 4-bit floating point
-# No reference counterpart: e2m1 codes with a scale per block (layouts in include/ctu_b200.h).  The
-# block scales' dtype names the format: float8_e4m3fn is nvfp4 (blocks of 16), float8_e8m0fnu mxfp4
-# (blocks of 32).
-_FP4_FORMATS = {"nvfp4": (0, 16, torch.float8_e4m3fn), "mxfp4": (1, 32, torch.float8_e8m0fnu)}
-_FP4_BY_SCALE = {torch.float8_e4m3fn: (0, 16), torch.float8_e8m0fnu: (1, 32)}
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-_FUNCTIONS: dict = {}  # C entries looked up once
-
-
-def _call(device: torch.device, name: str, *args) -> None:
-    """One C-ABI call on `device`'s current stream (appended as the last argument)."""
-    fn = _FUNCTIONS.get(name)
-    if fn is None:
-        fn = _FUNCTIONS[name] = getattr(_lib.load(), name)
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        _lib.check(rc)
-
-
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_contiguous() and not t.data_ptr() & 15 else _aligned(t.contiguous())
-
-
-def _fp4_tiles(rows: int, k: int, block: int) -> tuple[int, int, int, int]:
-    return ((rows + 127) // 128, (k // block + 3) // 4, 32, 16)
-
-
-def _fp4_operand(codes: torch.Tensor, block_scale: torch.Tensor, name: str):
-    """(codes, scales, rows, k, format) of one quantized operand, checked."""
-    if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_cuda:
-        raise RuntimeError(f"{name} must be a 2D uint8 CUDA tensor of packed FP4 codes")
-    fmt = _FP4_BY_SCALE.get(block_scale.dtype)
-    if fmt is None:
-        raise RuntimeError(f"{name} block scales must be float8_e4m3fn (nvfp4) or float8_e8m0fnu (mxfp4)")
-    rows, half = codes.shape
-    k = 2 * half
-    if k <= 0 or k & 31:
-        raise RuntimeError(f"{name} width must be positive and divisible by 32")
-    if block_scale.shape != _fp4_tiles(rows, k, fmt[1]) or block_scale.get_device() != codes.get_device():
-        raise RuntimeError(f"{name} block scales must be {list(_fp4_tiles(rows, k, fmt[1]))} tiles on the same device")
-    return _dense(codes), _dense(block_scale), rows, k, fmt[0]
-
-
-def _fp4_vector(t: torch.Tensor, count: int, device: int, name: str, scalar: bool) -> torch.Tensor:
-    n = t.numel()
-    if t.dtype != torch.float32 or t.get_device() != device or not (n == count or (scalar and n == 1)):
-        raise RuntimeError(f"{name} must be float32 on the same device, {count} values" + (" or one" if scalar else ""))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} has no gradient here: detach it")
-    return t.contiguous()
-
-
-def fp4_quantize(input, format="nvfp4", rotation=0):
-    """bf16 or fp16 rows [m, k] -> (codes uint8 [m, k/2], block scale tiles, row scales fp32 [m, 1])."""
-    if format not in _FP4_FORMATS:
-        raise RuntimeError("FP4 format must be 'nvfp4' or 'mxfp4'")
-    fmt, block, scale_dtype = _FP4_FORMATS[format]
-    if not input.is_cuda or input.dim() != 2:
-        raise RuntimeError("FP4 quantizer input must be a 2D CUDA tensor")
-    if input.dtype not in (torch.bfloat16, torch.float16):
-        raise RuntimeError("FP4 quantizer input must be float16 or bfloat16")
-    if rotation not in (0, 256):
-        raise RuntimeError("FP4 quantizer rotation must be 0 or 256")
-    rows, k = input.shape
-    if k <= 0 or k % (rotation or 32):
-        raise RuntimeError(f"FP4 quantizer width must be positive and divisible by {rotation or 32}")
-    x = _dense(input)
-    dev = x.device
-    codes = torch.empty((rows, k // 2), dtype=torch.uint8, device=dev)
-    scales = torch.empty(_fp4_tiles(rows, k, block), dtype=scale_dtype, device=dev)
-    row = torch.empty((rows, 1), dtype=torch.float32, device=dev)
-    _call(dev, "ctu_fp4_quantize", x.data_ptr(), rows, k, _NORM_TYPES[x.dtype], fmt, rotation, codes.data_ptr(),
-          scales.data_ptr(), row.data_ptr())
-    return codes, scales, row
-
-
-def fp4_dequantize(codes, block_scale, scale, out_dtype=torch.bfloat16):
-    """The values [m, k] that codes and scales stand for; `scale` fp32, one or one per row."""
-    codes, block_scale, rows, k, fmt = _fp4_operand(codes, block_scale, "codes")
-    if out_dtype not in _NORM_TYPES:
-        raise RuntimeError("FP4 dequantizer output must be float16, bfloat16, or float32")
-    scale = _fp4_vector(scale, rows, codes.get_device(), "row scale", True)
-    out = torch.empty((rows, k), dtype=out_dtype, device=codes.device)
-    _call(codes.device, "ctu_fp4_dequantize", codes.data_ptr(), block_scale.data_ptr(), scale.data_ptr(), scale.numel(),
-          rows, k, fmt, _NORM_TYPES[out_dtype], out.data_ptr())
-    return out
-
-
-def fp4_linear(activation, weight, activation_block_scale, weight_block_scale, activation_scale, weight_scale, bias=None):
-    """bf16 [m, n] from two quantized operands; see ctu_fp4_linear."""
-    a, a_bs, m, k, fmt = _fp4_operand(activation, activation_block_scale, "activation")
-    w, w_bs, n, wk, wfmt = _fp4_operand(weight, weight_block_scale, "weight")
-    dev = a.device
-    index = dev.index
-    if w.get_device() != index:
-        raise RuntimeError("all FP4 linear tensors must use the same CUDA device")
-    if wk != k or wfmt != fmt:
-        raise RuntimeError("activation and weight must have the same K and the same FP4 format")
-    a_s = _fp4_vector(activation_scale, m, index, "activation scale", False)
-    w_s = _fp4_vector(weight_scale, n, index, "weight scale", True)
-    if bias is not None:
-        bias = _fp4_vector(bias, n, index, "bias", False)
-    out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
-    _call(dev, "ctu_fp4_linear", a.data_ptr(), w.data_ptr(), a_bs.data_ptr(), w_bs.data_ptr(), a_s.data_ptr(),
-          w_s.data_ptr(), w_s.numel(), None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k, fmt)
-    return out
-
-
-def fp4_linear_grad_input(grad_output, weight, weight_block_scale, weight_scale, rotation=0):
-    """bf16 [m, k]: the gradient that fp4_linear's input receives through the frozen weights."""
-    w, w_bs, n, k, fmt = _fp4_operand(weight, weight_block_scale, "weight")
-    dev = w.device
-    if grad_output.device != dev or grad_output.dtype != torch.bfloat16 or grad_output.dim() != 2:
-        raise RuntimeError("grad_output must be a 2D bfloat16 tensor on the weight's device")
-    if grad_output.size(1) != n:
-        raise RuntimeError("grad_output must be [M, N] with the weight's N")
-    if n <= 0 or n % 8:
-        raise RuntimeError("FP4 linear gradient requires N divisible by 8")
-    if rotation not in (0, 256) or k % (rotation or 32):
-        raise RuntimeError("FP4 linear gradient rotation must be 0, or 256 with K divisible by it")
-    w_s = _fp4_vector(weight_scale, n, dev.index, "weight scale", True)
-    g = _dense(grad_output)
-    m = g.size(0)
-    dx = torch.empty((m, k), dtype=torch.bfloat16, device=dev)
-    if m == 0:
-        return dx
-    workspace = torch.empty(_lib.load().ctu_fp4_grad_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
-    _call(dev, "ctu_fp4_linear_grad_input", g.data_ptr(), w.data_ptr(), w_bs.data_ptr(), w_s.data_ptr(), w_s.numel(),
-          rotation, workspace.data_ptr(), dx.data_ptr(), m, n, k, fmt)
-    return dx
-
-
-# ----------------------------------------------------------------------------- affine layer norm
-def _norm_vector(t, hidden, input, name):
-    if t is None:
-        return None
-    if t.device != input.device or t.shape != (hidden,) or t.dtype not in (input.dtype, torch.float32):
-        raise RuntimeError(f"LayerNorm {name} must be [hidden] on the input's device, of its type or float32")
-    return _dense(t)
-
-
-def _norm_checks(input, weight, bias):
-    if not input.is_cuda or input.dim() < 1:
-        raise RuntimeError("LayerNorm input must be a CUDA tensor")
-    _check_float_like(input, "LayerNorm input")
-    hidden = input.size(-1)
-    if hidden <= 0:
-        raise RuntimeError("LayerNorm dimensions must be positive")
-    weight, bias = _norm_vector(weight, hidden, input, "weight"), _norm_vector(bias, hidden, input, "bias")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise RuntimeError("LayerNorm weight and bias must have the same type")
-    return hidden, weight, bias, (weight if weight is not None else bias if bias is not None else input).dtype
-
-
-def layer_norm(input, weight=None, bias=None, epsilon=1.0e-5):
-    """(output, mean, rstd) of the affine layer norm over the last dimension."""
-    hidden, weight, bias, wtype = _norm_checks(input, weight, bias)
-    if not (math.isfinite(epsilon) and epsilon > 0.0):
-        raise RuntimeError("LayerNorm epsilon must be finite and positive")
-    x = _dense(input)
-    rows = x.numel() // hidden
-    out = torch.empty_like(x)
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _call(x.device, "ctu_layer_norm", x.data_ptr(), None if weight is None else weight.data_ptr(),
-          None if bias is None else bias.data_ptr(), out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, hidden,
-          float(epsilon), _NORM_TYPES[x.dtype], _NORM_TYPES[wtype])
-    return out, mean, rstd
-
-
-def layer_norm_backward(grad_output, input, mean, rstd, weight=None, bias=None, needs=(True, True, True)):
-    """(dx, dweight, dbias), None where not needed (or where there is no such parameter)."""
-    hidden, weight, bias, wtype = _norm_checks(input, weight, bias)
-    if grad_output.shape != input.shape or grad_output.dtype != input.dtype or grad_output.device != input.device:
-        raise RuntimeError("LayerNorm gradient must match the input's shape, type and device")
-    x, g = _dense(input), _dense(grad_output)
-    rows = x.numel() // hidden
-    for t in (mean, rstd):
-        if t.dtype != torch.float32 or t.device != x.device or t.numel() != rows or not t.is_contiguous():
-            raise RuntimeError("LayerNorm statistics must be contiguous float32 [rows] on the input's device")
-    dev = x.device
-    dx = torch.empty_like(x) if needs[0] else None
-    dw = torch.empty(hidden, dtype=wtype, device=dev) if needs[1] and weight is not None else None
-    db = torch.empty(hidden, dtype=wtype, device=dev) if needs[2] and bias is not None else None
-    workspace = None
-    if dw is not None or db is not None:
-        workspace = torch.empty(_lib.load().ctu_layer_norm_backward_workspace_bytes(rows, hidden), dtype=torch.uint8,
-                                device=dev)
-    _call(dev, "ctu_layer_norm_backward", g.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(),
-          mean.data_ptr(), rstd.data_ptr(), *(None if t is None else t.data_ptr() for t in (dx, dw, db, workspace)),
-          rows, hidden, _NORM_TYPES[x.dtype], _NORM_TYPES[wtype])
-    return dx, dw, db

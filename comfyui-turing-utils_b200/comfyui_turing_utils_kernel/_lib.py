@@ -101,6 +101,20 @@ def load():
     return _lib
 
 
+def load_torch_ops() -> None:
+    """Register the ops of libctu_torch.so, the torch bindings next to the CUDA library."""
+    import torch
+
+    load()
+    path = _LIB_PATH.with_name("libctu_torch.so")
+    if not path.exists():
+        raise KernelUnavailable(f"{path} is not built; run comfyui-turing-utils_b200/build.py")
+    try:
+        torch.ops.load_library(str(path))
+    except OSError as exc:
+        raise KernelUnavailable(str(exc)) from exc
+
+
 def check(rc: int) -> None:
     """Map a C-ABI status to the exception the reference's pybind layer raises."""
     if rc == CTU_OK:

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _C
+from . import _C, _lib
 
 
 def _require_cuda(t: torch.Tensor, what: str) -> None:
@@ -469,29 +469,20 @@ def _turing_w4a4_g128_linear_fake(activation, weight, activation_scale, weight_s
 
 
 # 4-bit floating point linear and affine layer norm (no reference ops; arithmetic and layouts in
-# ctu_b200.h).  A single token's call is bound by host time, so these are defined on a
-# torch.library.Library, whose call costs a third of a torch.library.custom_op's (8 us against 22 us
-# for an empty op of five arguments); schema, fake kernels and autograd are the same.
-_LIBRARY = torch.library.Library("turing_utils", "FRAGMENT")
+# ctu_b200.h).  A single token's call is bound by host time, so these ops, their checks and their
+# gradients are registered from C++ (csrc/torch_ops.cpp): 1 x 5120 x 5120 costs 17 us of host time as a
+# Python op over ctypes.  Their fake kernels are here.
+_lib.load_torch_ops()
 
-
-def _define(name: str, schema: str, impl) -> None:
-    _LIBRARY.define(name + schema)
-    _LIBRARY.impl(name, impl, "CompositeExplicitAutograd")
-
-
-def _fp4_block(block_scale: torch.Tensor) -> int:
-    return 16 if block_scale.dtype == torch.float8_e4m3fn else 32
-
-
-_define("fp4_quantize", "(Tensor x, str format='nvfp4', int rotation=0) -> (Tensor, Tensor, Tensor)", _C.fp4_quantize)
+_FP4_FORMATS = {"nvfp4": (16, torch.float8_e4m3fn), "mxfp4": (32, torch.float8_e8m0fnu)}
 
 
 @torch.library.register_fake("turing_utils::fp4_quantize")
 def _fp4_quantize_fake(x, format="nvfp4", rotation=0):
-    _, block, dtype = _C._FP4_FORMATS[format]
+    block, dtype = _FP4_FORMATS[format]
     rows, k = x.shape
-    return (x.new_empty((rows, k // 2), dtype=torch.uint8), x.new_empty(_C._fp4_tiles(rows, k, block), dtype=dtype),
+    return (x.new_empty((rows, k // 2), dtype=torch.uint8),
+            x.new_empty(((rows + 127) // 128, (k // block + 3) // 4, 32, 16), dtype=dtype),
             x.new_empty((rows, 1), dtype=torch.float32))
 
 
@@ -503,10 +494,6 @@ def turing_fp4_quantize(x: torch.Tensor, format: str = "nvfp4", rotation: int = 
     return torch.ops.turing_utils.fp4_quantize.default(x, format, rotation)
 
 
-_define("fp4_dequantize", "(Tensor codes, Tensor block_scale, Tensor scale, ScalarType out_dtype=bfloat16) -> Tensor",
-        _C.fp4_dequantize)
-
-
 @torch.library.register_fake("turing_utils::fp4_dequantize")
 def _fp4_dequantize_fake(codes, block_scale, scale, out_dtype=torch.bfloat16):
     return codes.new_empty((codes.size(0), codes.size(1) * 2), dtype=out_dtype)
@@ -514,12 +501,9 @@ def _fp4_dequantize_fake(codes, block_scale, scale, out_dtype=torch.bfloat16):
 
 def turing_fp4_dequantize(codes: torch.Tensor, block_scale: torch.Tensor, scale: torch.Tensor,
                           out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that FP4 codes and scales stand for (rotated values stay rotated)."""
+    """The values that FP4 codes and scales stand for (rotated values stay rotated); ``scale`` is one
+    fp32 value or one per row."""
     return torch.ops.turing_utils.fp4_dequantize.default(codes, block_scale, scale, out_dtype)
-
-
-_define("fp4_linear", "(Tensor activation, Tensor weight, Tensor activation_block_scale, Tensor weight_block_scale, "
-        "Tensor activation_scale, Tensor weight_scale, Tensor? bias=None) -> Tensor", _C.fp4_linear)
 
 
 @torch.library.register_fake("turing_utils::fp4_linear")
@@ -536,10 +520,6 @@ def turing_fp4_linear(activation: torch.Tensor, weight: torch.Tensor, activation
                                                      activation_scale, weight_scale, bias)
 
 
-_define("fp4_linear_grad_input", "(Tensor grad_output, Tensor weight, Tensor weight_block_scale, Tensor weight_scale, "
-        "int rotation=0) -> Tensor", _C.fp4_linear_grad_input)
-
-
 @torch.library.register_fake("turing_utils::fp4_linear_grad_input")
 def _fp4_linear_grad_input_fake(grad_output, weight, weight_block_scale, weight_scale, rotation=0):
     return grad_output.new_empty((grad_output.size(0), weight.size(1) * 2))
@@ -552,49 +532,9 @@ def turing_fp4_linear_grad_input(grad_output: torch.Tensor, weight: torch.Tensor
                                                                 rotation)
 
 
-# Gradients go through a torch.autograd.Function around the ops: an op with registered autograd costs
-# twice as much host time in both directions (layer norm: 45 and 91 us).
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _no_second_derivative(what: str) -> None:
-    if torch.is_grad_enabled():  # create_graph=True
-        raise RuntimeError(f"{what} has no second derivative")
-
-
-def _convrot_fp4_linear(x, weight, weight_block_scale, weight_scale, bias=None, rotation=256):
-    fmt = "nvfp4" if weight_block_scale.dtype == torch.float8_e4m3fn else "mxfp4"
-    codes, block_scale, scale = _C.fp4_quantize(x, fmt, rotation)
-    return _C.fp4_linear(codes, weight, block_scale, weight_block_scale, scale, weight_scale, bias)
-
-
-_define("convrot_fp4_linear", "(Tensor x, Tensor weight, Tensor weight_block_scale, Tensor weight_scale, "
-        "Tensor? bias=None, int rotation=256) -> Tensor", _convrot_fp4_linear)
-
-
 @torch.library.register_fake("turing_utils::convrot_fp4_linear")
 def _convrot_fp4_linear_fake(x, weight, weight_block_scale, weight_scale, bias=None, rotation=256):
     return x.new_empty((x.size(0), weight.size(0)), dtype=torch.bfloat16)
-
-
-class _ConvrotFp4Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, weight_block_scale, weight_scale, bias, rotation):
-        if ctx.needs_input_grad[3] or ctx.needs_input_grad[4]:
-            raise RuntimeError("the FP4 linear's weight scale and bias are frozen: detach them")
-        if x.dtype != torch.bfloat16 or weight.size(0) % 8:
-            raise RuntimeError("the FP4 linear's gradient takes bfloat16 input and N divisible by 8")
-        ctx.save_for_backward(weight, weight_block_scale, weight_scale)
-        ctx.rotation = rotation
-        return torch.ops.turing_utils.convrot_fp4_linear.default(x, weight, weight_block_scale, weight_scale, bias,
-                                                                 rotation)
-
-    @staticmethod
-    def backward(ctx, grad):
-        _no_second_derivative("the FP4 linear")
-        dx = torch.ops.turing_utils.fp4_linear_grad_input.default(grad, *ctx.saved_tensors, ctx.rotation)
-        return dx, None, None, None, None, None
 
 
 def turing_convrot_fp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_block_scale: torch.Tensor,
@@ -603,28 +543,14 @@ def turing_convrot_fp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_bloc
     """Linear of bf16/fp16 rows with FP4 weights: the rows are rotated and quantized to the weights'
     format, then multiplied.  Differentiable in ``x`` (bf16): the quantization passes the gradient
     straight through, the weights are frozen."""
-    if _wants_grad(x, weight_scale, bias):
-        return _ConvrotFp4Linear.apply(x, weight, weight_block_scale, weight_scale, bias, rotation)
     return torch.ops.turing_utils.convrot_fp4_linear.default(x, weight, weight_block_scale, weight_scale, bias, rotation)
-
-
-_define("layer_norm", "(Tensor x, Tensor? weight=None, Tensor? bias=None, float epsilon=1e-5) -> "
-        "(Tensor, Tensor, Tensor)", _C.layer_norm)
 
 
 @torch.library.register_fake("turing_utils::layer_norm")
 def _layer_norm_fake(x, weight=None, bias=None, epsilon=1.0e-5):
     rows = x.numel() // x.size(-1)
-    return torch.empty_like(x, memory_format=torch.contiguous_format), *(x.new_empty(rows, dtype=torch.float32) for _ in "mr")
-
-
-def _layer_norm_backward(grad, x, mean, rstd, weight=None, bias=None, needs=7):
-    grads = _C.layer_norm_backward(grad, x, mean, rstd, weight, bias, [bool(needs & b) for b in (1, 2, 4)])
-    return tuple(x.new_empty(0) if g is None else g for g in grads)
-
-
-_define("layer_norm_backward", "(Tensor grad, Tensor x, Tensor mean, Tensor rstd, Tensor? weight=None, "
-        "Tensor? bias=None, int needs=7) -> (Tensor, Tensor, Tensor)", _layer_norm_backward)
+    return (torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(rows, dtype=torch.float32),
+            x.new_empty(rows, dtype=torch.float32))
 
 
 @torch.library.register_fake("turing_utils::layer_norm_backward")
@@ -635,36 +561,18 @@ def _layer_norm_backward_fake(grad, x, mean, rstd, weight=None, bias=None, needs
             torch.empty_like(bias) if needs & 4 and bias is not None else none)
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, epsilon):
-        y, mean, rstd = torch.ops.turing_utils.layer_norm.default(x, weight, bias, epsilon)
-        ctx.save_for_backward(x, mean, rstd, weight, bias)
-        return y
-
-    @staticmethod
-    def backward(ctx, grad):
-        _no_second_derivative("LayerNorm")
-        wanted = ctx.needs_input_grad
-        needs = wanted[0] + 2 * wanted[1] + 4 * wanted[2]
-        dx, dw, db = torch.ops.turing_utils.layer_norm_backward.default(grad, *ctx.saved_tensors, needs)
-        return dx if wanted[0] else None, dw if wanted[1] else None, db if wanted[2] else None, None
-
-
 def turing_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                       epsilon: float = 1.0e-5) -> torch.Tensor:
     """Affine layer norm over the last dimension, differentiable in x, weight and bias.
 
     x is bf16, fp16 or fp32; weight and bias have its type or are fp32."""
-    if _wants_grad(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, epsilon)
     return torch.ops.turing_utils.layer_norm.default(x, weight, bias, epsilon)[0]
 
 
 def turing_fp4_block_scale_tiles(block_scale: torch.Tensor) -> torch.Tensor:
     """Plain block scales [rows, k / block] (float8_e4m3fn or float8_e8m0fnu), as checkpoints store them,
     in the tiles that the FP4 ops read: once, when a layer is loaded."""
-    if block_scale.dim() != 2 or block_scale.dtype not in _C._FP4_BY_SCALE:
+    if block_scale.dim() != 2 or block_scale.dtype not in (torch.float8_e4m3fn, torch.float8_e8m0fnu):
         raise RuntimeError("block scales must be 2D float8_e4m3fn or float8_e8m0fnu")
     rows, blocks = block_scale.shape
     mt, kt = (rows + 127) // 128, (blocks + 3) // 4

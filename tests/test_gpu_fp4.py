@@ -228,11 +228,12 @@ def test_linear_repeats_bits_and_leaves_neighbours(k, fmt):
         for _ in range(3):
             assert torch.equal(first, k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r))
         # The C entry into a buffer with a margin on both sides.
-        from comfyui_turing_utils_kernel import _C
+        from comfyui_turing_utils_kernel import _lib
 
         buf = torch.full((m * n + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
-        _C._call(buf.device, "ctu_fp4_linear", a.data_ptr(), w.data_ptr(), a_s.data_ptr(), w_s.data_ptr(), a_r.data_ptr(),
-                 w_r.data_ptr(), n, None, buf.data_ptr() + 64, m, n, width, 0 if fmt == "nvfp4" else 1)
+        _lib.check(_lib.load().ctu_fp4_linear(
+            a.data_ptr(), w.data_ptr(), a_s.data_ptr(), w_s.data_ptr(), a_r.data_ptr(), w_r.data_ptr(), n, None,
+            buf.data_ptr() + 64, m, n, width, 0 if fmt == "nvfp4" else 1, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(buf[32 : 32 + m * n].view(m, n), first)
         assert (buf[:32] == 7).all() and (buf[32 + m * n :] == 7).all()
 
