@@ -15,7 +15,7 @@
 // tile's MMAs start.
 //
 // Roles: warp 0 loads (TMA), warp 1 of the leader copies scales into tensor memory and issues the
-// MMAs, warps 2..5 write the output.  Every wait is bounded.
+// MMAs, warps 2..9 write the output.  Every wait is bounded.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -42,7 +42,7 @@ constexpr int kBOffset = kStages * kABytes;
 constexpr int kAScaleOffset = kBOffset + kStages * kBBytes;
 constexpr int kBScaleOffset = kAScaleOffset + kStages * kAScaleBytes;
 constexpr int kStageOutOffset = kBScaleOffset + kStages * kBScaleBytes;
-constexpr int kEpilogueWarps = 4;
+constexpr int kEpilogueWarps = 8;         // at most; the launch chooses 4 or 8
 constexpr int kOutCols = 64;             // columns a warp stages at a time: 128 bytes a row
 constexpr int kOutBytes = 32 * 128;      // its 32 rows
 constexpr int kStructOffset = kStageOutOffset + kEpilogueWarps * kOutBytes;
@@ -82,6 +82,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Shared &S = *reinterpret_cast<Shared *>(smem + kStructOffset);
 
+    const int epilogue_warps = static_cast<int>(blockDim.x >> 5) - 2;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const int warp = threadIdx.x >> 5;
@@ -99,7 +100,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             mbar_init(&S.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) mbar_init(&S.acc_full[b], 1);
-        mbar_init(&S.acc_free, 2 * kEpilogueWarps);
+        mbar_init(&S.acc_free, 2 * epilogue_warps);
         mbar_init(&S.drain, 1);
         S.abort_flag = 0;
         fence_mbar_init();
@@ -167,7 +168,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const uint32_t empty0 = smem_u32(&S.empty[0]);
             for (int t = pair; t < num_tiles && ok; t += num_pairs, ++local) {
                 const uint32_t ab = local & 1;
-                // The tile before last has been read entirely when the last one's shared columns have.
+                // A warp's first piece of a tile read: its part of the tile before is, and the shared columns.
                 if (local > 0)
                     ok = __all_sync(0xffffffffu, guard.wait_cluster(&S.acc_free, (local - 1) & 1, kErrTimeoutAccumFree));
                 if (!ok) break;
@@ -219,6 +220,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
         }
     } else {
         const int quad = warp & 3;
+        const int sharers = epilogue_warps >> 2;  // warps to each 32 rows, and this one's place among them
+        const int share = (warp - 2) >> 2;
         const int ethread = threadIdx.x - 64;
         const uint32_t leader_free = mapa_shared(smem_u32(&S.acc_free), 0u);
         const uint32_t staged = smem_u32(smem + kStageOutOffset + (warp - 2) * kOutBytes);
@@ -230,14 +233,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const int ab = local & 1;
             const int m0 = (t / num_n) * kPairRows + static_cast<int>(rank) * 128;
             const int n0 = (t % num_n) * kPairCols;
-            named_barrier(1, 32 * kEpilogueWarps);
-            for (int c = ethread; c < kPairCols; c += 32 * kEpilogueWarps) {
+            named_barrier(1, 32 * epilogue_warps);
+            for (int c = ethread; c < kPairCols; c += 32 * epilogue_warps) {
                 const int n = n0 + c;
                 const bool in = n < args.n;
                 S.col_scale[c] = in ? args.w_scale[args.w_scale_count == 1 ? 0 : n] : 0.0f;
                 S.col_bias[c] = in && args.bias != nullptr ? args.bias[n] : 0.0f;
             }
-            named_barrier(1, 32 * kEpilogueWarps);
+            named_barrier(1, 32 * epilogue_warps);
             if (alive) {
                 alive = __all_sync(0xffffffffu, guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum));
             }
@@ -246,7 +249,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const int m_warp = m0 + quad * 32;
             const float a_s = m_warp + lane < args.m ? args.a_scale[m_warp + lane] : 0.0f;
 #pragma unroll 1
-            for (int i = 0; i < kPairCols / kOutCols; ++i) {
+            for (int i = share; i < kPairCols / kOutCols; i += sharers) {
                 // The piece with the shared columns first: the last one of the first accumulator, the first
                 // one of the second.
                 const int c = ab == 0 ? (i + kPairCols / kOutCols - 1) % (kPairCols / kOutCols) : i;
@@ -260,7 +263,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                 // The staging rows are free once the last copy out of them has read them.
                 if (lane == 0) bulk_wait_read_all();
                 tmem_ld_wait();
-                if (i == 0) {
+                if (i == share) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_remote(leader_free);
@@ -311,7 +314,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
 }
 
 int linear_pair_smem() { return kSmem; }
-int linear_pair_threads() { return kThreadCount; }
+// Eight epilogue warps shorten the way from a tile's last MMA to its output, which is what few tiles wait
+// for (1025 x 1537 x 1568: 12.7 us against 14.8 with four); four leave more to the MMAs where tiles follow
+// one another.
+int linear_pair_threads(bool few_tiles) { return few_tiles ? kThreadCount : 32 * (2 + 4); }
 const void *linear_pair_kernel(int format) {
     return format == kNvfp4 ? reinterpret_cast<const void *>(&fp4_linear_pair_kernel<kNvfp4>)
                             : reinterpret_cast<const void *>(&fp4_linear_pair_kernel<kMxfp4>);
