@@ -25,7 +25,8 @@ TORCH_LIB = OUT_DIR / "libctu_torch.so"
 OBJ_DIR = HERE / "_build"
 
 SOURCES = ["capi.cu", "convrot_quant.cu", "convrot_quant_reg.cu", "convrot_quant_t4.cu", "convrot_quant_k8.cu", "gemm_i8.cu", "gemm_pair.cu", "gemm_grouped.cu", "dequant.cu", "noalloc.cu", "codebook.cu", "unpack_s4.cu", "norm_adaln.cu",
-           "layer_norm.cu", "fp4_quant.cu", "fp4_gemm.cu", "fp4_gemm_small.cu", "fp4_grad.cu", "fp4_capi.cu"]
+           "layer_norm.cu", "layer_norm_backward_bf16.cu", "layer_norm_backward_fp16.cu",
+           "layer_norm_backward_fp32.cu", "fp4_quant.cu", "fp4_gemm.cu", "fp4_gemm_small.cu", "fp4_grad.cu", "fp4_capi.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",

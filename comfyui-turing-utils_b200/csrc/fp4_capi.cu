@@ -460,6 +460,7 @@ int ctu_layer_norm_backward(const void *grad, const void *x, const void *weight,
     a.dtype = dtype;
     a.weight_dtype = weight_dtype;
     a.num_sms = q.num_sms;
+    a.err = err;
     CTU_CUDA(ctu::norm::launch_layer_norm_backward(a, static_cast<cudaStream_t>(stream)));
     return CTU_OK;
 }

@@ -26,12 +26,18 @@ struct AffineArgs {
     int dtype;         // CTU_DTYPE_* of x, out, grad, dx
     int weight_dtype;  // CTU_DTYPE_* of weight, bias and their gradients
     int num_sms;
+    uint32_t *err;     // the device's error word (bounded waits)
 };
 
 // Row slices whose partial sums of the weight's and bias's gradients are joined at the end.
 int64_t backward_slices(int64_t rows, int64_t hidden);
 
 cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream);
+// One storage type's backward pass (layer_norm_backward_*.cu).
+template <typename T>
+cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream);
+constexpr int kSlices = 148;  // backward CTAs that leave partial sums: one an SM of a B200
+
 cudaError_t launch_layer_norm_backward(const AffineArgs &a, cudaStream_t stream);
 
 }  // namespace norm

@@ -1,0 +1,383 @@
+// Affine layer norm, backward pass (xhat as in the forward pass):
+//
+//   g  = dy * w,  dx = rstd * (g - mean(g) - xhat * mean(g * xhat))
+//   dw = sum over rows of dy * xhat,  db = sum over rows of dy
+//
+// A thread keeps the same columns for every row its team takes and holds their sums of dw and db in
+// registers; one CTA an SM leaves one partial sum per column, joined in order by a second kernel (equal
+// shapes add in equal order).  Sums are fp32; each result is rounded once.
+//
+// Bytes in flight bound it: where rows start on 16 bytes, a team's next rows of x and dy are copied into
+// shared memory (bulk copies, two rows deep) while it works on one, and the weights are there as fp32, so
+// registers hold the sums alone.  Other rows are kept in registers as loaded; rows wider than a team holds
+// take the looping kernels.
+#pragma once
+
+#include "layer_norm_parts.cuh"
+
+namespace ctu {
+namespace norm {
+
+namespace {
+
+constexpr int kBackwardBlock = 512;  // times 128 registers: an SM's register file
+constexpr int kMaxSmem = 220 * 1024;
+
+// The teams' sums to the CTA's slice of the workspace: through shared memory ([teams][dw, db][hidden]),
+// added over the teams in order, written 128 bytes a warp (one team gathering the others' by element took 5 us
+// longer at 5120 columns).  Every team has left its last row when this is called.
+template <typename P>
+__device__ __forceinline__ void leave_sums(const AffineArgs &a, const f32x2 (&dw)[P::kGroups][P::kPairs],
+                                           const f32x2 (&db)[P::kGroups][P::kPairs], float *sums) {
+    if (!a.dweight && !a.dbias) return;
+    const int h = a.hidden;
+    __syncthreads();
+    float *mine = sums + static_cast<int64_t>(threadIdx.y) * 2 * h;
+#pragma unroll
+    for (int g = 0; g < P::kGroups; ++g) {
+        if (!P::first(g, h)) continue;
+        const int c0 = P::column(P::kWide ? g : 2 * g);
+        const int c1 = P::kWide ? c0 + 1 : P::column(2 * g + 1);
+        const bool two = P::second(g, h);
+#pragma unroll
+        for (int i = 0; i < P::kPairs; ++i) {
+            float lo, hi;
+            unpk2(dw[g][i], lo, hi);
+            mine[c0 + 2 * i] = lo;
+            if (two) mine[c1 + 2 * i] = hi;
+            unpk2(db[g][i], lo, hi);
+            mine[h + c0 + 2 * i] = lo;
+            if (two) mine[h + c1 + 2 * i] = hi;
+        }
+    }
+    __syncthreads();
+    float *out = a.workspace + static_cast<int64_t>(blockIdx.x) * 2 * h;
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < 2 * h; c += blockDim.x * blockDim.y) {
+        float v = sums[c];
+        for (int t = 1; t < static_cast<int>(blockDim.y); ++t) v += sums[t * 2 * h + c];
+        out[c] = v;
+    }
+}
+
+// Rows of single elements, in registers.  blockDim = (threads of a team, teams).
+template <typename T, int kPieces>
+__global__ void __launch_bounds__(kBackwardBlock) team_backward_kernel(const AffineArgs a) {
+    using P = Part<T, 1, kPieces, 0>;
+    __shared__ float2 part[15][2][20];
+    extern __shared__ float joined[];
+    const int h = a.hidden;
+    const int team = threadIdx.y;
+    TeamSum<true> sum{part[team], static_cast<int>(blockDim.x >> 5), 1 + team};
+    const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.y;
+    const float inv_h = 1.0f / static_cast<float>(h);
+    f32x2 dw[P::kGroups][P::kPairs], db[P::kGroups][P::kPairs];
+#pragma unroll
+    for (int g = 0; g < P::kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < P::kPairs; ++i) dw[g][i] = db[g][i] = pk2(0.0f, 0.0f);
+    const void *weight = a.weight;
+    T *const dx = static_cast<T *>(a.dx);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + team; r < a.rows; r += stride) {
+        P x, dy;
+        x.load(static_cast<const T *>(a.x) + r * h, h);
+        dy.load(static_cast<const T *>(a.grad) + r * h, h);
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        const f32x2 mean2 = pk2(mean, mean), rstd2 = pk2(rstd, rstd);
+        f32x2 s = pk2(0.0f, 0.0f), t = s;
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, h)) continue;
+            f32x2 w[P::kPairs];
+            if (dx) P::weights(weight, fp32, g, h, 1.0f, w);
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) {
+                const f32x2 n = fmul2(fsub2(x.pair(g, i), mean2), rstd2);
+                const f32x2 d = dy.pair(g, i);
+                dw[g][i] = ffma2(d, n, dw[g][i]);
+                db[g][i] = fadd2(db[g][i], d);
+                if (dx) {
+                    const f32x2 gw = fmul2(d, w[i]);
+                    s = fadd2(s, gw);
+                    t = ffma2(gw, n, t);
+                }
+            }
+        }
+        if (dx == nullptr) continue;
+        const float2 st = sum(make_float2(both(s), both(t)));
+        const f32x2 minus_s = pk2(-st.x * inv_h, -st.x * inv_h), minus_t = pk2(-st.y * inv_h, -st.y * inv_h);
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, h)) continue;
+            f32x2 w[P::kPairs], out[P::kPairs];
+            P::weights(weight, fp32, g, h, 1.0f, w);
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) {
+                const f32x2 n = fmul2(fsub2(x.pair(g, i), mean2), rstd2);
+                out[i] = fmul2(rstd2, ffma2(n, minus_t, ffma2(dy.pair(g, i), w[i], minus_s)));
+            }
+            P::store(dx + r * h, g, h, out);
+        }
+    }
+    leave_sums<P>(a, dw, db, joined);
+}
+
+// Wide rows through shared memory.  blockDim = (kTeam, teams); dynamic shared memory holds the weights as
+// fp32, then [teams][2 buffers][x, dy] rows, and the teams' sums at the end.
+template <typename T, int kPieces, int kTeam>
+__global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const AffineArgs a) {
+    constexpr int kVec = 16 / sizeof(T);
+    using P = Part<T, kVec, kPieces, kTeam>;
+    constexpr int kTeams = kBackwardBlock / kTeam;
+    constexpr bool kNamed = kTeam > 32 && kTeams > 1;
+    __shared__ float2 part[kTeams][2][20];
+    __shared__ uint64_t bars[kTeams][2];
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int h = a.hidden;
+    const int team = threadIdx.y;
+    const uint32_t row_bytes = static_cast<uint32_t>(h) * sizeof(T);
+    float *const weights = reinterpret_cast<float *>(smem);
+    uint8_t *const rows = smem + ((h * 4 + 15) & ~15) + team * 4 * row_bytes;
+    TeamSum<kNamed> sum{part[team], kTeam / 32, 1 + team};
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kTeams;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+    const float inv_h = 1.0f / static_cast<float>(h);
+    T *const dx = static_cast<T *>(a.dx);
+
+    auto load = [&](int64_t r, int buf) {  // one thread of the team
+        uint8_t *dst = rows + buf * 2 * row_bytes;
+        mbar_arrive_expect_tx(&bars[team][buf], 2 * row_bytes);
+        bulk_load(dst, static_cast<const T *>(a.x) + r * h, row_bytes, &bars[team][buf]);
+        bulk_load(dst + row_bytes, static_cast<const T *>(a.grad) + r * h, row_bytes, &bars[team][buf]);
+    };
+    if (threadIdx.x == 0) {
+        mbar_init(&bars[team][0], 1);
+        mbar_init(&bars[team][1], 1);
+        fence_mbar_init();
+        if (first < a.rows) load(first, 0);
+        if (first + stride < a.rows) load(first + stride, 1);
+    }
+    const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
+    for (int c = threadIdx.y * kTeam + threadIdx.x; c < h; c += kBackwardBlock)
+        weights[c] = a.weight == nullptr ? 1.0f
+                     : fp32              ? static_cast<const float *>(a.weight)[c]
+                                         : to_f(static_cast<const T *>(a.weight)[c]);
+    __syncthreads();
+
+    f32x2 dw[P::kGroups][P::kPairs], db[P::kGroups][P::kPairs];
+#pragma unroll
+    for (int g = 0; g < P::kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < P::kPairs; ++i) dw[g][i] = db[g][i] = pk2(0.0f, 0.0f);
+    // One piece of x, dy and the weights.
+    auto piece = [&](const uint8_t *row, int g, Part<T, kVec, 1, kTeam> &x, Part<T, kVec, 1, kTeam> &dy,
+                     f32x2 (&w)[P::kPairs]) {
+        const int c = P::column(g);
+        x.wide[0] = *reinterpret_cast<const uint4 *>(row + c * sizeof(T));
+        dy.wide[0] = *reinterpret_cast<const uint4 *>(row + row_bytes + c * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < P::kPairs; i += 2) {
+            const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(weights + c + 2 * i);
+            w[i] = u.x;
+            w[i + 1] = u.y;
+        }
+    };
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    if (first < a.rows) {
+        next_mean = a.mean[first];
+        next_rstd = a.rstd[first];
+    }
+    int buf = 0;
+    uint32_t phase = 0;
+    for (int64_t r = first; r < a.rows; r += stride) {
+        const f32x2 mean2 = pk2(next_mean, next_mean), rstd2 = pk2(next_rstd, next_rstd);
+        if (r + stride < a.rows) {
+            next_mean = a.mean[r + stride];
+            next_rstd = a.rstd[r + stride];
+        }
+        mbar_wait(&bars[team][buf], phase, nullptr, a.err, kErrTimeoutFull);
+        const uint8_t *row = rows + buf * 2 * row_bytes;
+        f32x2 s = pk2(0.0f, 0.0f), t = s;
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, h)) continue;
+            Part<T, kVec, 1, kTeam> x, dy;
+            f32x2 w[P::kPairs];
+            piece(row, g, x, dy, w);
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) {
+                const f32x2 n = fmul2(fsub2(x.pair(0, i), mean2), rstd2);
+                const f32x2 d = dy.pair(0, i);
+                dw[g][i] = ffma2(d, n, dw[g][i]);
+                db[g][i] = fadd2(db[g][i], d);
+                const f32x2 gw = fmul2(d, w[i]);
+                s = fadd2(s, gw);
+                t = ffma2(gw, n, t);
+            }
+        }
+        const float2 st = sum(make_float2(both(s), both(t)));
+        // Every thread of the team is past the row before: its buffer takes the row after the next.
+        if (kTeam == 32) __syncwarp();
+        if (threadIdx.x == 0 && r != first && r + stride < a.rows) {
+            fence_proxy_async_smem();
+            load(r + stride, buf ^ 1);
+        }
+        const f32x2 minus_s = pk2(-st.x * inv_h, -st.x * inv_h), minus_t = pk2(-st.y * inv_h, -st.y * inv_h);
+        if (dx != nullptr) {
+#pragma unroll
+            for (int g = 0; g < P::kGroups; ++g) {
+                if (!P::first(g, h)) continue;
+                Part<T, kVec, 1, kTeam> x, dy;
+                f32x2 w[P::kPairs], out[P::kPairs];
+                piece(row, g, x, dy, w);
+#pragma unroll
+                for (int i = 0; i < P::kPairs; ++i) {
+                    const f32x2 n = fmul2(fsub2(x.pair(0, i), mean2), rstd2);
+                    out[i] = fmul2(rstd2, ffma2(n, minus_t, ffma2(dy.pair(0, i), w[i], minus_s)));
+                }
+                P::store(dx + r * h, g, h, out);
+            }
+        }
+        buf ^= 1;
+        if (buf == 0) phase ^= 1u;
+    }
+    leave_sums<P>(a, dw, db, reinterpret_cast<float *>(smem));
+}
+
+// Slices of partial sums joined: 32 columns by 8 runs of slices a block.
+template <typename W>
+__global__ void __launch_bounds__(256) team_join_kernel(const AffineArgs a, int slices) {
+    __shared__ float part[8][33];
+    const int c = blockIdx.x * 32 + threadIdx.x;  // of 2 * hidden: dw, then db
+    const int total = 2 * a.hidden;
+    float s = 0.0f;
+    if (c < total) {
+        const int first = slices * threadIdx.y / 8, last = slices * (threadIdx.y + 1) / 8;
+#pragma unroll 10
+        for (int i = first; i < last; ++i) s += a.workspace[static_cast<int64_t>(i) * total + c];
+    }
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y != 0 || c >= total) return;
+    for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
+    if (c < a.hidden) {
+        if (a.dweight) static_cast<W *>(a.dweight)[c] = from_f<W>(s);
+    } else if (a.dbias) {
+        static_cast<W *>(a.dbias)[c - a.hidden] = from_f<W>(s);
+    }
+}
+
+template <typename T, typename W>
+__global__ void __launch_bounds__(kThreads) input_gradient_kernel(const AffineArgs a) {
+    const int h = a.hidden;
+    const W *w = static_cast<const W *>(a.weight);
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *x = static_cast<const T *>(a.x) + r * h;
+        const T *dy = static_cast<const T *>(a.grad) + r * h;
+        T *dx = static_cast<T *>(a.dx) + r * h;
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float2 s = make_float2(0.0f, 0.0f);
+        for (int c = threadIdx.x; c < h; c += kThreads) {
+            const float n = (to_f(x[c]) - mean) * rstd;
+            const float g = to_f(dy[c]) * (w ? to_f(w[c]) : 1.0f);
+            s.x += g;
+            s.y += g * n;
+        }
+        s = block_sum(s);
+        s.x /= static_cast<float>(h);
+        s.y /= static_cast<float>(h);
+        for (int c = threadIdx.x; c < h; c += kThreads) {
+            const float n = (to_f(x[c]) - mean) * rstd;
+            const float g = to_f(dy[c]) * (w ? to_f(w[c]) : 1.0f);
+            dx[c] = from_f<T>(rstd * (g - s.x - n * s.y));
+        }
+    }
+}
+
+// Partial sums of one slice of rows: workspace [slice][0: dw, 1: db][hidden].
+template <typename T>
+__global__ void __launch_bounds__(256) parameter_partial_kernel(const AffineArgs a, int slices) {
+    __shared__ float2 part[8][33];
+    const int h = a.hidden;
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    const int slice = blockIdx.y;
+    float2 s = make_float2(0.0f, 0.0f);
+    if (c < h) {
+        for (int64_t r = slice * 8 + threadIdx.y; r < a.rows; r += static_cast<int64_t>(slices) * 8) {
+            const float dy = to_f(static_cast<const T *>(a.grad)[r * h + c]);
+            s.x += dy * ((to_f(static_cast<const T *>(a.x)[r * h + c]) - a.mean[r]) * a.rstd[r]);
+            s.y += dy;
+        }
+    }
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < h) {
+        for (int i = 1; i < 8; ++i) {
+            s.x += part[i][threadIdx.x].x;
+            s.y += part[i][threadIdx.x].y;
+        }
+        a.workspace[(static_cast<int64_t>(slice) * 2) * h + c] = s.x;
+        a.workspace[(static_cast<int64_t>(slice) * 2 + 1) * h + c] = s.y;
+    }
+}
+
+}  // namespace
+
+namespace {
+int staged_smem(int hidden, int bytes, int teams) { return ((hidden * 4 + 15) & ~15) + teams * 4 * hidden * bytes; }
+
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes) {
+    return bytes <= 32768 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+}  // namespace
+
+template <typename T>
+cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
+    const bool aligned = row_aligned(a.x) && row_aligned(a.grad) && row_aligned(a.dx) && row_aligned(a.weight);
+    const bool params = a.dweight || a.dbias;
+    TeamPlan plan = team_plan(a.hidden, sizeof(T), aligned, kBackwardBlock);
+    if (plan.pieces != 0 && plan.vec > 1 && staged_smem(a.hidden, sizeof(T), kBackwardBlock / plan.threads) > kMaxSmem)
+        plan.pieces = 0;
+    if (plan.pieces == 0) {
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
+        const int slices = static_cast<int>(std::min<int64_t>(64, backward_slices(a.rows, a.hidden)));
+        return with_weight<T>(a, [&](auto w) {
+            using W = decltype(w);
+            if (a.dx && a.rows > 0) input_gradient_kernel<T, W><<<grid, kThreads, 0, stream>>>(a);
+            if (params) {
+                parameter_partial_kernel<T>
+                    <<<dim3((a.hidden + 31) / 32, slices), dim3(32, 8), 0, stream>>>(a, slices);
+                team_join_kernel<W><<<(2 * a.hidden + 31) / 32, dim3(32, 8), 0, stream>>>(a, slices);
+            }
+            return cudaGetLastError();
+        });
+    }
+    plan.teams = plan.vec > 1 ? kBackwardBlock / plan.threads : std::min(15, kBackwardBlock / plan.threads);
+    const int64_t ctas = std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, kSlices);
+    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, ctas));
+    const cudaError_t e = with_shape<T, kBackwardBlock>(plan, [&](auto vec, auto pieces, auto threads) {
+        const dim3 block(plan.threads, plan.teams);
+        const int sums = params ? plan.teams * 2 * a.hidden * static_cast<int>(sizeof(float)) : 0;
+        if constexpr (vec == 1) {
+            auto kernel = team_backward_kernel<T, pieces>;
+            if (cudaError_t f = allow_smem(kernel, sums)) return f;
+            kernel<<<grid, block, sums, stream>>>(a);
+        } else {
+            const int smem = std::max(sums, staged_smem(a.hidden, sizeof(T), plan.teams));
+            auto kernel = staged_backward_kernel<T, pieces, threads>;
+            if (cudaError_t f = allow_smem(kernel, smem)) return f;
+            kernel<<<grid, block, smem, stream>>>(a);
+        }
+        return cudaGetLastError();
+    });
+    if (e != cudaSuccess || !params) return e;
+    return with_weight<T>(a, [&](auto w) {
+        team_join_kernel<decltype(w)>
+            <<<(2 * a.hidden + 31) / 32, dim3(32, 8), 0, stream>>>(a, static_cast<int>(grid));
+        return cudaGetLastError();
+    });
+}
+
+}  // namespace norm
+}  // namespace ctu

@@ -1,0 +1,11 @@
+// Affine layer norm, backward pass for bf16 rows (a translation unit of its own: the shapes' kernels take a
+// minute to compile for each type).
+#include "layer_norm_backward.cuh"
+
+namespace ctu {
+namespace norm {
+
+template cudaError_t backward_as<__nv_bfloat16>(const AffineArgs &, cudaStream_t);
+
+}  // namespace norm
+}  // namespace ctu

@@ -1,0 +1,281 @@
+// What the affine layer norm's forward and backward kernels share: a thread's part of a row, sums over a
+// team, and the choice of a kernel by shape.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/ctu_b200.h"
+#include "layer_norm.cuh"
+#include "ptx.cuh"
+
+namespace ctu {
+namespace norm {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+
+
+constexpr int kThreads = 256;  // of the looping kernels, for rows wider than a team holds
+
+// Sum of two values over the block, in every thread.
+__device__ __forceinline__ float2 block_sum(float2 v) {
+    __shared__ float2 part[kThreads / 32];
+    for (int o = 16; o > 0; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < kThreads / 32; ++i) {
+        s.x += part[i].x;
+        s.y += part[i].y;
+    }
+    return s;
+}
+
+// A thread's part of a row: kPieces loads of kVec elements (16 bytes), or of single elements where rows
+// do not start on 16 bytes.  Elements are handled in pairs; a group is the pairs that share a load (or
+// two single loads).
+// kThreads: of the team, 0 where only the launch knows.  A team is no larger than its row needs, so of wide
+// loads only the last one can lie beyond the row.
+template <typename T, int kVec, int kPieces, int kThreads>
+struct Part {
+    static constexpr bool kWide = kVec > 1;
+    static constexpr int kGroups = kWide ? kPieces : kPieces / 2;
+    static constexpr int kPairs = kWide ? kVec / 2 : 1;  // of a group
+    uint4 wide[kWide ? kPieces : 1];
+    T single[kWide ? 1 : kPieces];
+
+    static __device__ __forceinline__ int column(int piece) {
+        return threadIdx.x * kVec + piece * (kThreads ? kThreads : static_cast<int>(blockDim.x)) * kVec;
+    }
+    // Whether a group's first element (all of them, with wide loads) and second element exist.
+    static __device__ __forceinline__ bool first(int g, int h) {
+        return kWide ? g + 1 < kPieces || column(g) < h : column(2 * g) < h;
+    }
+    static __device__ __forceinline__ bool second(int g, int h) { return kWide ? first(g, h) : column(2 * g + 1) < h; }
+
+    // What does not exist reads as zero.
+    __device__ __forceinline__ void load(const T *row, int h) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            const int c = column(p);
+            if constexpr (kWide)
+                wide[p] = first(p, h) ? __ldcs(reinterpret_cast<const uint4 *>(row + c)) : make_uint4(0u, 0u, 0u, 0u);
+            else
+                single[p] = c < h ? row[c] : from_f<T>(0.0f);
+        }
+    }
+    __device__ __forceinline__ f32x2 pair(int g, int i) const {
+        if constexpr (!kWide) return pk2(to_f(single[2 * g]), to_f(single[2 * g + 1]));
+        const uint32_t w[4] = {wide[g].x, wide[g].y, wide[g].z, wide[g].w};
+        if constexpr (sizeof(T) == 4) return pk2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return pk2(bf16lo(w[i]), bf16hi(w[i]));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        return pk2(f.x, f.y);
+    }
+    // One group of results.
+    static __device__ __forceinline__ void store(T *row, int g, int h, const f32x2 (&v)[kPairs]) {
+        float e[2 * kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) unpk2(v[i], e[2 * i], e[2 * i + 1]);
+        if constexpr (kWide) {
+            alignas(16) T out[kVec];
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) out[i] = from_f<T>(e[i]);
+            *reinterpret_cast<uint4 *>(row + column(g)) = *reinterpret_cast<const uint4 *>(out);
+        } else {
+            row[column(2 * g)] = from_f<T>(e[0]);
+            if (second(g, h)) row[column(2 * g + 1)] = from_f<T>(e[1]);
+        }
+    }
+    // One group of weights (of the input's type or fp32), `fill` where there are none.
+    static __device__ __forceinline__ void weights(const void *p, bool fp32, int g, int h, float fill, f32x2 (&out)[kPairs]) {
+        if (p == nullptr) {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) out[i] = pk2(fill, fill);
+        } else if constexpr (!kWide) {
+            const int c0 = column(2 * g), c1 = column(2 * g + 1);
+            const bool two = second(g, h);
+            if (fp32)
+                out[0] = pk2(static_cast<const float *>(p)[c0], two ? static_cast<const float *>(p)[c1] : 0.0f);
+            else
+                out[0] = pk2(to_f(static_cast<const T *>(p)[c0]), two ? to_f(static_cast<const T *>(p)[c1]) : 0.0f);
+        } else if (fp32) {
+            const ulonglong2 *f = reinterpret_cast<const ulonglong2 *>(static_cast<const float *>(p) + column(g));
+#pragma unroll
+            for (int i = 0; i < kPairs / 2; ++i) {
+                const ulonglong2 u = __ldg(f + i);
+                out[2 * i] = u.x;
+                out[2 * i + 1] = u.y;
+            }
+        } else {
+            Part one;
+            one.wide[0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p) + column(g)));
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) out[i] = one.pair(0, i);
+        }
+    }
+};
+
+// Sum of two values over a team of `warps` warps, in every thread, in a fixed order.  Two buffers in
+// turn: a team's threads are past a buffer's last reads when its barrier after next is passed.
+// kNamed: several teams of warps in a CTA meet at barriers of their own (which reserves all sixteen of a
+// CTA, so not where occupancy counts); otherwise the CTA is one team, or every team one warp.
+template <bool kNamed>
+struct TeamSum {
+    float2 (*part)[20];  // [2][20] of this team
+    int warps;
+    int barrier;
+    int flip = 0;
+
+    __device__ __forceinline__ float2 operator()(float2 v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        }
+        if (warps == 1) return v;
+        float2 *buf = part[flip];
+        flip ^= 1;
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0) buf[warp] = v;
+        if (kNamed)
+            asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+        else
+            __syncthreads();
+        v = buf[0];
+#pragma unroll
+        for (int i = 1; i < 20; ++i) {
+            if (i >= warps) break;
+            v.x += buf[i].x;
+            v.y += buf[i].y;
+        }
+        return v;
+    }
+};
+
+__device__ __forceinline__ float both(f32x2 v) {
+    float lo, hi;
+    unpk2(v, lo, hi);
+    return lo + hi;
+}
+
+// blockDim = (threads of a team, teams).
+
+template <typename F>
+cudaError_t with_type(int dtype, F f) {
+    switch (dtype) {
+    case CTU_DTYPE_BF16: return f(__nv_bfloat16());
+    case CTU_DTYPE_FP16: return f(__half());
+    default: return f(float());
+    }
+}
+
+// Weights have the input's type or fp32.
+template <typename T, typename F>
+cudaError_t with_weight(const AffineArgs &a, F f) {
+    return a.weight_dtype == CTU_DTYPE_FP32 ? f(float()) : f(T());
+}
+
+// How a row is held: `vec` elements a piece, `pieces` pieces a thread (0: wider than a team holds),
+// `threads` of a team, `teams` a CTA.  Depends on the sizes and the alignment of rows alone.
+struct TeamPlan {
+    int vec, pieces, threads, teams;
+};
+
+// Five wide pieces (sixteen single elements) a thread at most, and as few threads as hold the row that way:
+// more rows are in flight, and what a row costs a warp besides its elements is spread over more of them.
+// With wide pieces the kernels know the team's size: a power of two up to `block`, or `block`.
+inline TeamPlan team_plan(int64_t hidden, int bytes, bool aligned, int block) {
+    TeamPlan p{};
+    p.vec = aligned && hidden * bytes % 16 == 0 ? 16 / bytes : 1;
+    const int64_t count = hidden / p.vec;
+    const int most = p.vec == 1 ? 16 : 5;
+    int64_t threads = ((count + most - 1) / most + 31) / 32 * 32;
+    if (threads > block) return p;
+    if (p.vec > 1) {
+        int64_t t = 32;
+        while (t < threads) t *= 2;
+        threads = std::min<int64_t>(t, block);
+    }
+    p.pieces = static_cast<int>((count + threads - 1) / threads);
+    if (p.vec == 1) p.pieces = p.pieces <= 2 ? 2 : p.pieces <= 4 ? 4 : p.pieces <= 8 ? 8 : 16;
+    p.threads = static_cast<int>(threads);
+    p.teams = 1;
+    return p;
+}
+
+inline bool row_aligned(const void *p) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Calls f(vec, pieces, threads) with the plan's values as constants (threads 0 with single elements).  With
+// wide loads that is 32 threads and one to five pieces, or more threads and what fewer do not hold: three to
+// five.
+template <int kBlock, int kVec, int kPieces, typename F>
+cudaError_t with_threads(int threads, F f) {
+    using std::integral_constant;
+    constexpr integral_constant<int, kVec> vec{};
+    constexpr integral_constant<int, kPieces> pieces{};
+    if constexpr (kVec == 1) {
+        return f(vec, pieces, integral_constant<int, 0>());
+    } else {
+        if (threads == 32) return f(vec, pieces, integral_constant<int, 32>());
+        if constexpr (kPieces >= 3) {
+            switch (threads) {
+            case 64: return f(vec, pieces, integral_constant<int, 64>());
+            case 128: return f(vec, pieces, integral_constant<int, 128>());
+            case 256: return f(vec, pieces, integral_constant<int, 256>());
+            case kBlock: return f(vec, pieces, integral_constant<int, kBlock>());
+            default: break;
+            }
+        }
+        return cudaErrorInvalidValue;
+    }
+}
+
+template <typename T, int kBlock, typename F>
+cudaError_t with_shape(const TeamPlan &p, F f) {
+    constexpr int kFull = 16 / sizeof(T);
+    if (p.vec == 1) {
+        switch (p.pieces) {
+        case 2: return with_threads<kBlock, 1, 2>(p.threads, f);
+        case 4: return with_threads<kBlock, 1, 4>(p.threads, f);
+        case 8: return with_threads<kBlock, 1, 8>(p.threads, f);
+        default: return with_threads<kBlock, 1, 16>(p.threads, f);
+        }
+    }
+    switch (p.pieces) {
+    case 1: return with_threads<kBlock, kFull, 1>(p.threads, f);
+    case 2: return with_threads<kBlock, kFull, 2>(p.threads, f);
+    case 3: return with_threads<kBlock, kFull, 3>(p.threads, f);
+    case 4: return with_threads<kBlock, kFull, 4>(p.threads, f);
+    default: return with_threads<kBlock, kFull, 5>(p.threads, f);
+    }
+}
+
+}  // namespace
+}  // namespace norm
+}  // namespace ctu
