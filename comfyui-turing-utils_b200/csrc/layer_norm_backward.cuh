@@ -158,10 +158,15 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         if (first + stride < a.rows) load(first + stride, 1);
     }
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
-    for (int c = threadIdx.y * kTeam + threadIdx.x; c < h; c += kBackwardBlock)
-        weights[c] = a.weight == nullptr ? 1.0f
-                     : fp32              ? static_cast<const float *>(a.weight)[c]
-                                         : to_f(static_cast<const T *>(a.weight)[c]);
+    // The weights of a piece of eight as two fours, the first ones of all pieces together and the second ones:
+    // lanes then read 16 bytes 16 bytes apart, without bank conflicts.
+    const int second_half = kVec == 8 ? h / 2 : 0;
+    for (int c = threadIdx.y * kTeam + threadIdx.x; c < h; c += kBackwardBlock) {
+        const int at = kVec == 8 ? (c & 4 ? second_half : 0) + (c >> 3) * 4 + (c & 3) : c;
+        weights[at] = a.weight == nullptr ? 1.0f
+                      : fp32              ? static_cast<const float *>(a.weight)[c]
+                                          : to_f(static_cast<const T *>(a.weight)[c]);
+    }
     __syncthreads();
 
     f32x2 dw[P::kGroups][P::kPairs], db[P::kGroups][P::kPairs];
@@ -177,7 +182,8 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         dy.wide[0] = *reinterpret_cast<const uint4 *>(row + row_bytes + c * sizeof(T));
 #pragma unroll
         for (int i = 0; i < P::kPairs; i += 2) {
-            const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(weights + c + 2 * i);
+            const float *from = kVec == 8 ? weights + (i ? second_half : 0) + c / 2 : weights + c + 2 * i;
+            const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(from);
             w[i] = u.x;
             w[i + 1] = u.y;
         }
