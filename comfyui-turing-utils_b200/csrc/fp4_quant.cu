@@ -20,6 +20,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/ctu_b200.h"
 #include "fp4.cuh"
@@ -543,13 +544,23 @@ cudaError_t quantize_as(const QuantArgs &a, const CUtensorMap &map, cudaStream_t
         return cudaGetLastError();
     }
     const int smem = warps * 8192 + 1024;
-    auto kernel = !multi        ? rotate_quantize_kernel<kFormat, kHalf, false, 128>
-                  : warps <= 16 ? rotate_quantize_kernel<kFormat, kHalf, true, 512>
-                                : rotate_quantize_kernel<kFormat, kHalf, true, 768>;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
-    int per_sm = 0;
-    if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, warps * 32, smem)) return e;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows, a.num_sms * static_cast<int64_t>(std::max(1, per_sm))));
+    const int variant = !multi ? 0 : warps <= 16 ? 1 : 2;
+    auto kernel = variant == 0   ? rotate_quantize_kernel<kFormat, kHalf, false, 128>
+                  : variant == 1 ? rotate_quantize_kernel<kFormat, kHalf, true, 512>
+                                 : rotate_quantize_kernel<kFormat, kHalf, true, 768>;
+    // CTAs an SM by warps a CTA, asked once a device (a call's host time is most of a small call's).
+    static std::atomic<int> resident[64][3][25];
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    std::atomic<int> &known = resident[dev][variant][warps];
+    int per_sm = known.load(std::memory_order_acquire);
+    if (per_sm == 0) {
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 24 * 8192 + 1024)) return e;
+        if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, warps * 32, smem)) return e;
+        per_sm = std::max(1, per_sm);
+        known.store(per_sm, std::memory_order_release);
+    }
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows, a.num_sms * static_cast<int64_t>(per_sm)));
     kernel<<<grid, warps * 32, smem, stream>>>(map, a);
     return cudaGetLastError();
 }

@@ -16,6 +16,8 @@
 // what its bytes take at 5.7 TB/s.
 #pragma once
 
+#include <atomic>
+
 #include "layer_norm_parts.cuh"
 
 namespace ctu {
@@ -335,9 +337,15 @@ __global__ void __launch_bounds__(256) parameter_partial_kernel(const AffineArgs
 namespace {
 int staged_smem(int hidden, int bytes, int teams) { return ((hidden * 4 + 15) & ~15) + teams * 4 * hidden * bytes; }
 
+// Opts a kernel in to the most it may ask for, once a device.
 template <typename K>
-cudaError_t allow_smem(K kernel, int bytes) {
-    return bytes <= 32768 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+cudaError_t allow_smem(K kernel, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) return e;
+    done[dev].store(true, std::memory_order_release);
+    return cudaSuccess;
 }
 }  // namespace
 
@@ -370,12 +378,14 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
         const int sums = params ? plan.teams * 2 * a.hidden * static_cast<int>(sizeof(float)) : 0;
         if constexpr (vec == 1) {
             auto kernel = team_backward_kernel<T, pieces>;
-            if (cudaError_t f = allow_smem(kernel, sums)) return f;
+            static std::atomic<bool> done[64];
+                if (cudaError_t f = allow_smem(kernel, done)) return f;
             kernel<<<grid, block, sums, stream>>>(a);
         } else {
             const int smem = std::max(sums, staged_smem(a.hidden, sizeof(T), plan.teams));
             auto kernel = staged_backward_kernel<T, pieces, threads>;
-            if (cudaError_t f = allow_smem(kernel, smem)) return f;
+            static std::atomic<bool> done[64];
+                if (cudaError_t f = allow_smem(kernel, done)) return f;
             kernel<<<grid, block, smem, stream>>>(a);
         }
         return cudaGetLastError();
