@@ -508,3 +508,54 @@ def test_calls_from_a_fresh_thread(k):
         t.start()
         t.join()
         assert len(got) == 1 and torch.equal(got[0], y)
+
+
+def test_ops_trace_and_compile(k):
+    """Fake kernels, autograd registration and traced gradients agree with the ops; a compiled layer gives
+    the eager one's bits."""
+    from torch.library import opcheck
+
+    ops = torch.ops.turing_utils
+    (w, w_s, w_r), _, _ = quantized(64, 512, "nvfp4", 1, 256)
+    x = rows_like(40, 512, 2).cuda()
+    codes, scale, row = k.turing_fp4_quantize(x, "nvfp4", 256)
+    leaf = x.clone().requires_grad_(True)
+    weight, bias = (torch.randn(512, device="cuda").requires_grad_(True) for _ in range(2))
+    stats = torch.zeros(40, device="cuda"), torch.ones(40, device="cuda")
+    checks = ("test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+    for op, args in ((ops.fp4_quantize, (x, "nvfp4", 256)), (ops.fp4_dequantize, (codes, scale, row)),
+                     (ops.fp4_linear, (codes, w, scale, w_s, row, w_r)),
+                     (ops.fp4_linear_grad_input, (torch.randn(40, 64, device="cuda").bfloat16(), w, w_s, w_r, 256)),
+                     (ops.convrot_fp4_linear, (leaf, w, w_s, w_r)), (ops.layer_norm, (leaf, weight, bias)),
+                     (ops.layer_norm, (leaf, None, bias)),
+                     (ops.layer_norm_backward, (x, x, *stats, weight.detach(), bias.detach(), 7))):
+        opcheck(op.default, args, test_utils=checks)
+
+    def layer(x, weight, bias):
+        return k.turing_convrot_fp4_linear(k.turing_layer_norm(x, weight, bias), w, w_s, w_r).float().square().sum()
+
+    leaves = (leaf, weight, bias)
+    eager = torch.autograd.grad(layer(*leaves), leaves)
+    compiled = torch.autograd.grad(torch.compile(layer, backend="aot_eager", fullgraph=True)(*leaves), leaves)
+    assert all(torch.equal(p, q) for p, q in zip(eager, compiled))
+
+
+@pytest.mark.parametrize("m,n,width,rotation", [(16, 2048, 512, 256), (333, 4096, 768, 0), (1300, 1024, 4096, 256)])
+def test_gradient_repeats_bits(k, m, n, width, rotation):
+    """Split sums are joined in a fixed order; rows beyond the gradient's stay as they were."""
+    from comfyui_turing_utils_kernel import _lib
+
+    (w, w_s, w_r), _, _ = quantized(n, width, "mxfp4", 3, rotation)
+    g = torch.randn(m, n, device="cuda").bfloat16()
+    first = k.turing_fp4_linear_grad_input(g, w, w_s, w_r, rotation)
+    for _ in range(3):
+        assert torch.equal(first, k.turing_fp4_linear_grad_input(g, w, w_s, w_r, rotation))
+    lib = _lib.load()
+    buf = torch.full((m + 2, width), 7.0, dtype=torch.bfloat16, device="cuda")
+    room = lib.ctu_fp4_grad_workspace_bytes(m, n, width)
+    work = torch.full((room + 256,), 9, dtype=torch.uint8, device="cuda")
+    _lib.check(lib.ctu_fp4_linear_grad_input(
+        g.data_ptr(), w.data_ptr(), w_s.data_ptr(), w_r.data_ptr(), n, rotation, work.data_ptr(), buf[1:].data_ptr(), m, n,
+        width, 1, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(buf[1 : 1 + m], first) and (buf[0] == 7).all() and (buf[-1] == 7).all()
+    assert (work[room:] == 9).all()
