@@ -5,8 +5,8 @@
 // Statistics and sums are fp32 whatever the storage type; each result is rounded once.  Bound by memory:
 // a team of lanes (a warp, or a CTA of several) keeps a row in registers, as loaded, so x is read once;
 // arithmetic is on packed fp32 pairs.  32760 x 5120 bf16: 115 us, 5.84 TB/s (0.90 of a copy's rate); with the
-// team's size a launch parameter, so that each access computed its address and bounds, 154 us.  Rows wider
-// than a team holds take the looping kernel.
+// team's size a launch parameter, so that each access computed its address and bounds, 154 us.  Rows that do not
+// start on 16 bytes: RAGGED_FIGURES.  Rows wider than a team holds take the looping kernel.
 #include "layer_norm_parts.cuh"
 
 namespace ctu {
@@ -75,6 +75,82 @@ __global__ void __maxnreg__(64) team_forward_kernel(const AffineArgs a) {
     }
 }
 
+// Rows that do not start on 16 bytes.  Neither do their weights, so those are in shared memory, shifted as the
+// CTA's rows are; CTAs are large, so that they are copied there once for many rows.  blockDim = (threads of a
+// team, teams).
+template <typename T, int kPieces, int kThreads>
+__global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const AffineArgs a) {
+    constexpr int kVec = 16 / sizeof(T);
+    using P = Part<T, kVec, kPieces, kThreads>;
+    __shared__ float2 part[kThreads > 32 ? kForwardBlock / kThreads : 1][2][20];
+    extern __shared__ __align__(16) float weights[];
+    const int h = a.hidden;
+    const int team = threadIdx.y;
+    const TeamRows<kVec> mine(blockDim.y, team);
+    const T *const from = static_cast<const T *>(a.x);
+    const Ragged<kVec> at(from + mine.first * h, h);
+    const int inner = at.inner;
+    TeamSum<true> sum{part[kThreads > 32 ? team : 0], kThreads / 32, 1 + team};
+    const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
+    const float inv_h = 1.0f / static_cast<float>(h);
+    P x;
+    float own = 0.0f, own_w = 0.0f, own_b = 0.0f;
+    auto load = [&](int64_t r) {
+        const T *row = from + r * h;
+        x.load(row + at.head, inner);
+        if (at.own) own = to_f(row[at.column]);
+    };
+    if (mine.first < a.rows) load(mine.first);
+    stage_weights<T, kVec>(weights, a.weight, fp32, 1.0f, at.head, inner);
+    stage_weights<T, kVec>(weights + inner, a.bias, fp32, 0.0f, at.head, inner);
+    if (at.own) {
+        own_w = weight_at<T>(a.weight, fp32, at.column, 1.0f);
+        own_b = weight_at<T>(a.bias, fp32, at.column, 0.0f);
+    }
+    __syncthreads();
+    for (int64_t r = mine.first; r < a.rows;) {
+        f32x2 s = pk2(own, 0.0f);
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g)
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) s = fadd2(s, x.pair(g, i));
+        const float mean = sum(make_float2(both(s), 0.0f)).x * inv_h;
+        const f32x2 mean2 = pk2(mean, mean);
+        const float own_d = at.own ? own - mean : 0.0f;
+        f32x2 q = pk2(own_d * own_d, 0.0f);
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, inner)) continue;
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) {
+                const f32x2 d = fsub2(x.pair(g, i), mean2);
+                q = ffma2(d, d, q);
+            }
+        }
+        const float var = sum(make_float2(both(q), 0.0f)).x * inv_h;
+        const float rstd = 1.0f / sqrtf(var + a.epsilon);
+        if (threadIdx.x == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        const f32x2 rstd2 = pk2(rstd, rstd);
+        T *const out = static_cast<T *>(a.out) + r * h;
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g) {
+            if (!P::first(g, inner)) continue;
+            f32x2 w[P::kPairs], b[P::kPairs], y[P::kPairs];
+            staged_weights<kVec>(weights, inner, P::column(g), w);
+            staged_weights<kVec>(weights + inner, inner, P::column(g), b);
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) y[i] = ffma2(fmul2(fsub2(x.pair(g, i), mean2), rstd2), w[i], b[i]);
+            P::store(out + at.head, g, inner, y);
+        }
+        if (at.own) out[at.column] = from_f<T>(fmaf(own_d * rstd, own_w, own_b));
+        r += mine.stride;
+        if (r < a.rows) load(r);
+    }
+}
+
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const AffineArgs a) {
     const int h = a.hidden;
@@ -110,7 +186,9 @@ cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream) {
     const bool aligned = row_aligned(a.x) && row_aligned(a.out) && row_aligned(a.weight) && row_aligned(a.bias);
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        TeamPlan plan = team_plan(a.hidden, sizeof(T), aligned, kForwardBlock);
+        const bool whole = aligned && a.hidden * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+        const bool ragged = !whole && start_alike(a.x, a.out) && ragged_length(a.hidden, sizeof(T));
+        TeamPlan plan = team_plan(a.hidden, sizeof(T), whole || ragged, kForwardBlock);
         if (plan.pieces == 0) {
             const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
             return with_weight<T>(a, [&](auto w) {
@@ -123,6 +201,22 @@ cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream) {
         const unsigned grid = static_cast<unsigned>(
             std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, static_cast<int64_t>(a.num_sms) * 16));
         return with_shape<T, kForwardBlock>(plan, [&](auto vec, auto pieces, auto threads) {
+            if constexpr (vec > 1) {
+                if (ragged) {
+                    // As many teams as the rows give every SM two CTAs of, and as many CTAs as run at once.
+                    const int smem = 2 * a.hidden * static_cast<int>(sizeof(float));
+                    const int each = smem + 4096 <= 114 * 1024 ? 2 : 1;
+                    plan.teams = static_cast<int>(std::min<int64_t>(
+                        kForwardBlock / threads, (a.rows + each * a.num_sms - 1) / (each * a.num_sms)));
+                    auto kernel = ragged_forward_kernel<T, pieces, threads>;
+                    static std::atomic<bool> done[64];
+                    if (cudaError_t e = allow_smem(kernel, done)) return e;
+                    const int64_t ctas = (a.rows + plan.teams - 1) / plan.teams;
+                    const int64_t some = ragged_grid(a.rows, std::min<int64_t>(ctas + vec - 1, a.num_sms * each), vec);
+                    kernel<<<static_cast<unsigned>(some), dim3(plan.threads, plan.teams), smem, stream>>>(a);
+                    return cudaGetLastError();
+                }
+            }
             team_forward_kernel<T, vec, pieces, threads><<<grid, dim3(plan.threads, plan.teams), 0, stream>>>(a);
             return cudaGetLastError();
         });

@@ -16,8 +16,6 @@
 // what its bytes take at 5.7 TB/s.
 #pragma once
 
-#include <atomic>
-
 #include "layer_norm_parts.cuh"
 
 namespace ctu {
@@ -26,24 +24,35 @@ namespace norm {
 namespace {
 
 constexpr int kBackwardBlock = 512;  // times 128 registers: an SM's register file
-constexpr int kMaxSmem = 220 * 1024;
+
+// Sums of an element of its own that a thread may have, and where the inner part starts: see Ragged.
+struct OwnSums {
+    int head, inner, column;
+    bool own;
+    float dw, db;
+};
 
 // The teams' sums to the CTA's slice of the workspace: through shared memory ([teams][dw, db][hidden]),
 // added over the teams in order, written 128 bytes a warp (one team gathering the others' by element took 5 us
 // longer at 5120 columns).  Every team has left its last row when this is called.
 template <typename P>
 __device__ __forceinline__ void leave_sums(const AffineArgs &a, const f32x2 (&dw)[P::kGroups][P::kPairs],
-                                           const f32x2 (&db)[P::kGroups][P::kPairs], float *sums) {
+                                           const f32x2 (&db)[P::kGroups][P::kPairs], const OwnSums &own,
+                                           float *sums) {
     if (!a.dweight && !a.dbias) return;
     const int h = a.hidden;
     __syncthreads();
     float *mine = sums + static_cast<int64_t>(threadIdx.y) * 2 * h;
+    if (own.own) {
+        mine[own.column] = own.dw;
+        mine[h + own.column] = own.db;
+    }
 #pragma unroll
     for (int g = 0; g < P::kGroups; ++g) {
-        if (!P::first(g, h)) continue;
-        const int c0 = P::column(P::kWide ? g : 2 * g);
+        if (!P::first(g, own.inner)) continue;
+        const int c0 = own.head + P::column(P::kWide ? g : 2 * g);
         const int c1 = P::kWide ? c0 + 1 : P::column(2 * g + 1);
-        const bool two = P::second(g, h);
+        const bool two = P::second(g, own.inner);
 #pragma unroll
         for (int i = 0; i < P::kPairs; ++i) {
             float lo, hi;
@@ -124,12 +133,12 @@ __global__ void __launch_bounds__(kBackwardBlock) team_backward_kernel(const Aff
             P::store(dx + r * h, g, h, out);
         }
     }
-    leave_sums<P>(a, dw, db, joined);
+    leave_sums<P>(a, dw, db, OwnSums{0, h, 0, false, 0.0f, 0.0f}, joined);
 }
 
 // Wide rows through shared memory.  blockDim = (kTeam, teams); dynamic shared memory holds the weights as
 // fp32, then [teams][2 buffers][x, dy] rows, and the teams' sums at the end.
-template <typename T, int kPieces, int kTeam>
+template <typename T, int kPieces, int kTeam, bool kRagged>
 __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const AffineArgs a) {
     constexpr int kVec = 16 / sizeof(T);
     using P = Part<T, kVec, kPieces, kTeam>;
@@ -138,22 +147,25 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
     __shared__ float2 part[kTeams][2][20];
     __shared__ uint64_t bars[kTeams][2];
     extern __shared__ __align__(16) uint8_t smem[];
-    const int h = a.hidden;
     const int team = threadIdx.y;
+    const TeamRows<kRagged ? kVec : 1> mine(kTeams, team);
+    const int64_t stride = mine.stride, first = mine.first;
+    const Ragged<kVec> at(static_cast<const T *>(a.x) + first * a.hidden, a.hidden);
+    const int head = kRagged ? at.head : 0;
+    const int h = kRagged ? at.inner : a.hidden;  // of a row's part on 16 bytes
+    const bool has_own = kRagged && at.own;
     const uint32_t row_bytes = static_cast<uint32_t>(h) * sizeof(T);
     float *const weights = reinterpret_cast<float *>(smem);
-    uint8_t *const rows = smem + ((h * 4 + 15) & ~15) + team * 4 * row_bytes;
+    uint8_t *const rows = smem + h * 4 + team * 4 * row_bytes;
     TeamSum<kNamed> sum{part[team], kTeam / 32, 1 + team};
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * kTeams;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTeams + team;
-    const float inv_h = 1.0f / static_cast<float>(h);
+    const float inv_h = 1.0f / static_cast<float>(a.hidden);
     T *const dx = static_cast<T *>(a.dx);
 
     auto load = [&](int64_t r, int buf) {  // one thread of the team
         uint8_t *dst = rows + buf * 2 * row_bytes;
         mbar_arrive_expect_tx(&bars[team][buf], 2 * row_bytes);
-        bulk_load(dst, static_cast<const T *>(a.x) + r * h, row_bytes, &bars[team][buf]);
-        bulk_load(dst + row_bytes, static_cast<const T *>(a.grad) + r * h, row_bytes, &bars[team][buf]);
+        bulk_load(dst, static_cast<const T *>(a.x) + r * a.hidden + head, row_bytes, &bars[team][buf]);
+        bulk_load(dst + row_bytes, static_cast<const T *>(a.grad) + r * a.hidden + head, row_bytes, &bars[team][buf]);
     };
     if (threadIdx.x == 0) {
         mbar_init(&bars[team][0], 1);
@@ -163,14 +175,15 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         if (first + stride < a.rows) load(first + stride, 1);
     }
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
-    // The weights of a piece of eight as two fours, the first ones of all pieces together and the second ones:
-    // lanes then read 16 bytes 16 bytes apart, without bank conflicts.
-    const int second_half = kVec == 8 ? h / 2 : 0;
-    for (int c = threadIdx.y * kTeam + threadIdx.x; c < h; c += kBackwardBlock) {
-        const int at = kVec == 8 ? (c & 4 ? second_half : 0) + (c >> 3) * 4 + (c & 3) : c;
-        weights[at] = a.weight == nullptr ? 1.0f
-                      : fp32              ? static_cast<const float *>(a.weight)[c]
-                                          : to_f(static_cast<const T *>(a.weight)[c]);
+    stage_weights<T, kVec>(weights, a.weight, fp32, 1.0f, head, h);
+    float own_x = 0.0f, own_dy = 0.0f, own_w = 0.0f, own_dw = 0.0f, own_db = 0.0f;
+    auto load_own = [&](int64_t r) {
+        own_x = to_f(static_cast<const T *>(a.x)[r * a.hidden + at.column]);
+        own_dy = to_f(static_cast<const T *>(a.grad)[r * a.hidden + at.column]);
+    };
+    if (has_own) {
+        own_w = weight_at<T>(a.weight, fp32, at.column, 1.0f);
+        if (first < a.rows) load_own(first);
     }
     __syncthreads();
 
@@ -185,13 +198,7 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         const int c = P::column(g);
         x.wide[0] = *reinterpret_cast<const uint4 *>(row + c * sizeof(T));
         dy.wide[0] = *reinterpret_cast<const uint4 *>(row + row_bytes + c * sizeof(T));
-#pragma unroll
-        for (int i = 0; i < P::kPairs; i += 2) {
-            const float *from = kVec == 8 ? weights + (i ? second_half : 0) + c / 2 : weights + c + 2 * i;
-            const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(from);
-            w[i] = u.x;
-            w[i + 1] = u.y;
-        }
+        staged_weights<kVec>(weights, h, c, w);
     };
     float next_mean = 0.0f, next_rstd = 0.0f;
     if (first < a.rows) {
@@ -201,7 +208,8 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
     int buf = 0;
     uint32_t phase = 0;
     for (int64_t r = first; r < a.rows; r += stride) {
-        const f32x2 mean2 = pk2(next_mean, next_mean), rstd2 = pk2(next_rstd, next_rstd);
+        const float mean = next_mean, rstd = next_rstd;
+        const f32x2 mean2 = pk2(mean, mean), rstd2 = pk2(rstd, rstd);
         if (r + stride < a.rows) {
             next_mean = a.mean[r + stride];
             next_rstd = a.rstd[r + stride];
@@ -209,6 +217,16 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         mbar_wait(&bars[team][buf], phase, nullptr, a.err, kErrTimeoutFull);
         const uint8_t *row = rows + buf * 2 * row_bytes;
         f32x2 s = pk2(0.0f, 0.0f), t = s;
+        float own_n = 0.0f, own_gw = 0.0f;
+        if (has_own) {
+            own_n = (own_x - mean) * rstd;
+            own_gw = own_dy * own_w;
+            own_dw = fmaf(own_dy, own_n, own_dw);
+            own_db += own_dy;
+            s = pk2(own_gw, 0.0f);
+            t = pk2(own_gw * own_n, 0.0f);
+            if (r + stride < a.rows) load_own(r + stride);
+        }
 #pragma unroll
         for (int g = 0; g < P::kGroups; ++g) {
             if (!P::first(g, h)) continue;
@@ -235,6 +253,9 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         }
         const f32x2 minus_s = pk2(-st.x * inv_h, -st.x * inv_h), minus_t = pk2(-st.y * inv_h, -st.y * inv_h);
         if (dx != nullptr) {
+            if (has_own)
+                dx[r * a.hidden + at.column] =
+                    from_f<T>(rstd * (own_gw - st.x * inv_h - own_n * (st.y * inv_h)));
 #pragma unroll
             for (int g = 0; g < P::kGroups; ++g) {
                 if (!P::first(g, h)) continue;
@@ -246,13 +267,13 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
                     const f32x2 n = fmul2(fsub2(x.pair(0, i), mean2), rstd2);
                     out[i] = fmul2(rstd2, ffma2(n, minus_t, ffma2(dy.pair(0, i), w[i], minus_s)));
                 }
-                P::store(dx + r * h, g, h, out);
+                P::store(dx + r * a.hidden + head, g, h, out);
             }
         }
         buf ^= 1;
         if (buf == 0) phase ^= 1u;
     }
-    leave_sums<P>(a, dw, db, reinterpret_cast<float *>(smem));
+    leave_sums<P>(a, dw, db, OwnSums{head, h, at.column, has_own, own_dw, own_db}, reinterpret_cast<float *>(smem));
 }
 
 // Slices of partial sums joined: 32 columns by 8 runs of slices a block.
@@ -335,25 +356,18 @@ __global__ void __launch_bounds__(256) parameter_partial_kernel(const AffineArgs
 }  // namespace
 
 namespace {
-int staged_smem(int hidden, int bytes, int teams) { return ((hidden * 4 + 15) & ~15) + teams * 4 * hidden * bytes; }
-
-// Opts a kernel in to the most it may ask for, once a device.
-template <typename K>
-cudaError_t allow_smem(K kernel, std::atomic<bool> (&done)[64]) {
-    int dev = 0;
-    if (cudaError_t e = cudaGetDevice(&dev)) return e;
-    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) return e;
-    done[dev].store(true, std::memory_order_release);
-    return cudaSuccess;
+int staged_smem(int hidden, int bytes, int teams) {
+    return hidden / 4 * 16 + teams * 4 * (hidden * bytes / 16 * 16);
 }
 }  // namespace
 
 template <typename T>
 cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
-    const bool aligned = row_aligned(a.x) && row_aligned(a.grad) && row_aligned(a.dx) && row_aligned(a.weight);
+    const bool aligned = row_aligned(a.x) && row_aligned(a.grad) && row_aligned(a.dx);
+    const bool whole = aligned && a.hidden * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+    const bool ragged = !whole && start_alike(a.x, a.grad) && start_alike(a.x, a.dx) && ragged_length(a.hidden, sizeof(T));
     const bool params = a.dweight || a.dbias;
-    TeamPlan plan = team_plan(a.hidden, sizeof(T), aligned, kBackwardBlock);
+    TeamPlan plan = team_plan(a.hidden, sizeof(T), whole || ragged, kBackwardBlock);
     if (plan.pieces != 0 && plan.vec > 1 && staged_smem(a.hidden, sizeof(T), kBackwardBlock / plan.threads) > kMaxSmem)
         plan.pieces = 0;
     if (plan.pieces == 0) {
@@ -372,7 +386,8 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     }
     plan.teams = plan.vec > 1 ? kBackwardBlock / plan.threads : std::min(15, kBackwardBlock / plan.threads);
     const int64_t ctas = std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, kSlices);
-    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, ctas));
+    const int period = ragged ? plan.vec : 1;
+    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, ragged_grid(a.rows, ctas, period)));
     const cudaError_t e = with_shape<T, kBackwardBlock>(plan, [&](auto vec, auto pieces, auto threads) {
         const dim3 block(plan.threads, plan.teams);
         const int sums = params ? plan.teams * 2 * a.hidden * static_cast<int>(sizeof(float)) : 0;
@@ -383,10 +398,15 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
             kernel<<<grid, block, sums, stream>>>(a);
         } else {
             const int smem = std::max(sums, staged_smem(a.hidden, sizeof(T), plan.teams));
-            auto kernel = staged_backward_kernel<T, pieces, threads>;
-            static std::atomic<bool> done[64];
+            auto launch = [&](auto kernel, std::atomic<bool>(&done)[64]) {
                 if (cudaError_t f = allow_smem(kernel, done)) return f;
-            kernel<<<grid, block, smem, stream>>>(a);
+                kernel<<<grid, block, smem, stream>>>(a);
+                return cudaSuccess;
+            };
+            static std::atomic<bool> done[2][64];
+            const cudaError_t f = ragged ? launch(staged_backward_kernel<T, pieces, threads, true>, done[1])
+                                         : launch(staged_backward_kernel<T, pieces, threads, false>, done[0]);
+            if (f) return f;
         }
         return cudaGetLastError();
     });

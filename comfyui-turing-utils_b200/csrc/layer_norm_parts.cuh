@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -56,8 +57,8 @@ __device__ __forceinline__ float2 block_sum(float2 v) {
     return s;
 }
 
-// A thread's part of a row: kPieces loads of kVec elements (16 bytes), or of single elements where rows
-// do not start on 16 bytes.  Elements are handled in pairs; a group is the pairs that share a load (or
+// A thread's part of a row: kPieces loads of kVec elements (16 bytes), or of single elements where the tensors
+// start differently within 16 bytes.  Elements are handled in pairs; a group is the pairs that share a load (or
 // two single loads).
 // kThreads: of the team, 0 where only the launch knows.  A team is no larger than its row needs, so of wide
 // loads only the last one can lie beyond the row.
@@ -196,6 +197,84 @@ __device__ __forceinline__ float both(f32x2 v) {
     return lo + hi;
 }
 
+// Rows that do not start on 16 bytes, in tensors that start alike within 16 bytes: what lies on 16 bytes (inner)
+// is handled as in aligned rows, and each element before it (head) and behind it (tail) by a thread of its own:
+// threads 0 to 7 of a team take the head's, 8 to 15 the tail's, in every row the same.  For that a CTA's rows
+// start alike: row r starts as row r + kVec does, so CTAs take every kVec-th row.
+template <int kVec>
+struct Ragged {
+    int head, inner, column;  // inner: a multiple of kVec; column: of the thread's own element
+    bool own;
+
+    template <typename T>
+    __device__ __forceinline__ Ragged(const T *row, int h) {
+        head = (-static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T))) & (kVec - 1);
+        inner = (h - head) / kVec * kVec;
+        const int slot = threadIdx.x, tail = h - head - inner;
+        own = slot < 8 ? slot < head : slot < 8 + tail;
+        column = slot < 8 ? slot : head + inner + slot - 8;
+    }
+};
+
+// The rows of a team: every kPeriod-th one's from blockIdx.x % kPeriod on are shared among the CTAs of that
+// remainder.  The grid is a multiple of kPeriod, or smaller than it.
+template <int kPeriod>
+struct TeamRows {
+    int64_t first, stride;
+
+    __device__ __forceinline__ TeamRows(int teams, int team) {
+        const int64_t groups = gridDim.x < kPeriod ? 1 : gridDim.x / kPeriod;
+        first = blockIdx.x % kPeriod + kPeriod * (static_cast<int64_t>(blockIdx.x / kPeriod) * teams + team);
+        stride = kPeriod * groups * teams;
+    }
+};
+
+inline int64_t ragged_grid(int64_t rows, int64_t ctas, int period) {
+    return rows < period ? rows : std::max<int64_t>(1, ctas / period) * period;
+}
+
+template <typename T>
+__device__ __forceinline__ float weight_at(const void *p, bool fp32, int c, float fill) {
+    return p == nullptr ? fill : fp32 ? static_cast<const float *>(p)[c] : to_f(static_cast<const T *>(p)[c]);
+}
+
+// Weights in shared memory as fp32, a piece of eight as two fours, the first ones of all pieces together and
+// the second ones: lanes then read 16 bytes 16 bytes apart, without bank conflicts.
+template <typename T, int kVec>
+__device__ __forceinline__ void stage_weights(float *to, const void *p, bool fp32, float fill, int head, int inner) {
+    const int second_half = kVec == 8 ? inner / 2 : 0;
+    const int step = blockDim.x * blockDim.y;
+#pragma unroll 8
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < inner; c += step) {
+        const int at = kVec == 8 ? (c & 4 ? second_half : 0) + (c >> 3) * 4 + (c & 3) : c;
+        to[at] = weight_at<T>(p, fp32, head + c, fill);
+    }
+}
+template <int kVec>
+__device__ __forceinline__ void staged_weights(const float *from, int inner, int column, f32x2 (&w)[kVec / 2]) {
+    const int second_half = kVec == 8 ? inner / 2 : 0;
+#pragma unroll
+    for (int i = 0; i < kVec / 2; i += 2) {
+        const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(
+            kVec == 8 ? from + (i ? second_half : 0) + column / 2 : from + column);
+        w[i] = u.x;
+        w[i + 1] = u.y;
+    }
+}
+
+constexpr int kMaxSmem = 220 * 1024;
+
+// Opts a kernel in to the most it may ask for, once a device.
+template <typename K>
+cudaError_t allow_smem(K kernel, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) return e;
+    done[dev].store(true, std::memory_order_release);
+    return cudaSuccess;
+}
+
 // blockDim = (threads of a team, teams).
 
 template <typename F>
@@ -222,9 +301,9 @@ struct TeamPlan {
 // Five wide pieces (sixteen single elements) a thread at most, and as few threads as hold the row that way:
 // more rows are in flight, and what a row costs a warp besides its elements is spread over more of them.
 // With wide pieces the kernels know the team's size: a power of two up to `block`, or `block`.
-inline TeamPlan team_plan(int64_t hidden, int bytes, bool aligned, int block) {
+inline TeamPlan team_plan(int64_t hidden, int bytes, bool wide, int block) {
     TeamPlan p{};
-    p.vec = aligned && hidden * bytes % 16 == 0 ? 16 / bytes : 1;
+    p.vec = wide ? 16 / bytes : 1;
     const int64_t count = hidden / p.vec;
     const int most = p.vec == 1 ? 16 : 5;
     int64_t threads = ((count + most - 1) / most + 31) / 32 * 32;
@@ -242,6 +321,13 @@ inline TeamPlan team_plan(int64_t hidden, int bytes, bool aligned, int block) {
 }
 
 inline bool row_aligned(const void *p) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// The same place within 16 bytes; a gradient that is not asked for counts as on 16 bytes, as those that are do:
+// the others then have the same bits with it and without it.
+inline bool start_alike(const void *p, const void *q) {
+    return ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15u) == 0;
+}
+// Shorter rows than this are not split into a head, an inner part and a tail.
+inline bool ragged_length(int64_t hidden, int bytes) { return hidden * bytes >= 64; }
 
 // Calls f(vec, pieces, threads) with the plan's values as constants (threads 0 with single elements).  With
 // wide loads that is 32 threads and one to five pieces, or more threads and what fewer do not hold: three to

@@ -241,3 +241,47 @@ def test_refusals(k):
     x.requires_grad_(True)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(k.turing_layer_norm(x, w, b).sum(), x, create_graph=True)
+
+
+# Rows of a C caller that start anywhere within 16 bytes: x, dy and the results at one offset, or the results
+# at another than x; results in the middle of a larger buffer, whose other values stay.
+@pytest.mark.parametrize("dtype,offset,result_offset", [(torch.bfloat16, 0, 0), (torch.bfloat16, 3, 3), (torch.float16, 7, 7),
+                                                        (torch.float32, 1, 1), (torch.float32, 2, 2), (torch.bfloat16, 5, 0),
+                                                        (torch.float32, 0, 3)])
+@pytest.mark.parametrize("rows,hidden", [(1, 32), (7, 33), (8, 47), (9, 256), (41, 1281), (700, 2562), (30, 5119),
+                                         (1300, 5124), (3, 10247)])
+def test_rows_anywhere_within_16_bytes(k, rows, hidden, dtype, offset, result_offset):
+    from comfyui_turing_utils_kernel import _lib
+
+    lib = _lib.load()
+    x, w, b, dy = make(rows, hidden, dtype, torch.float32, rows + hidden + offset)
+    kind = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[dtype]
+    guard = 24
+
+    def placed(t, at):
+        buf = torch.full((t.numel() + 2 * guard,), -77.0, dtype=dtype, device="cuda")
+        view = buf[guard + at:guard + at + t.numel()]
+        view.copy_(t.reshape(-1))
+        return buf, view.view(rows, hidden)
+
+    def outside(buf, at):
+        return torch.cat((buf[:guard + at], buf[guard + at + rows * hidden:]))
+
+    _, x = placed(x, offset)
+    _, dy = placed(dy, offset)
+    w = torch.cat((w[:1], w))[1:]  # 4 bytes off 16
+    y_buf, y = placed(torch.zeros_like(x), result_offset)
+    dx_buf, dx = placed(torch.zeros_like(x), result_offset)
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    dw, db = torch.empty(hidden, device="cuda"), torch.empty(hidden, device="cuda")
+    room = lib.ctu_layer_norm_backward_workspace_bytes(rows, hidden) // 4
+    work = torch.full((room + 64,), -77.0, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.ctu_layer_norm(x.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                  rows, hidden, EPS, kind, 2, stream))
+    _lib.check(lib.ctu_layer_norm_backward(dy.data_ptr(), x.data_ptr(), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                           dx.data_ptr(), dw.data_ptr(), db.data_ptr(), work.data_ptr(), rows, hidden,
+                                           kind, 2, stream))
+    check(y, (dx, dw, db), x, w, b, dy)
+    assert (outside(y_buf, result_offset) == -77).all() and (outside(dx_buf, result_offset) == -77).all()
+    assert (work[room:] == -77).all()
