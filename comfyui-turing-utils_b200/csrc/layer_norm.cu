@@ -5,8 +5,9 @@
 // Statistics and sums are fp32 whatever the storage type; each result is rounded once.  Bound by memory:
 // a team of lanes (a warp, or a CTA of several) keeps a row in registers, as loaded, so x is read once;
 // arithmetic is on packed fp32 pairs.  32760 x 5120 bf16: 115 us, 5.84 TB/s (0.90 of a copy's rate); with the
-// team's size a launch parameter, so that each access computed its address and bounds, 154 us.  Rows that do not
-// start on 16 bytes: RAGGED_FIGURES.  Rows wider than a team holds take the looping kernel.
+// team's size a launch parameter, so that each access computed its address and bounds, 154 us.  Rows off 16
+// bytes: 32760 x 5121 147 us (with loads of single elements 540 us).  Rows wider than a team holds take the
+// looping kernel.
 #include "layer_norm_parts.cuh"
 
 namespace ctu {
@@ -83,6 +84,7 @@ __global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const 
     constexpr int kVec = 16 / sizeof(T);
     using P = Part<T, kVec, kPieces, kThreads>;
     __shared__ float2 part[kThreads > 32 ? kForwardBlock / kThreads : 1][2][20];
+    __shared__ float ends[2][16];
     extern __shared__ __align__(16) float weights[];
     const int h = a.hidden;
     const int team = threadIdx.y;
@@ -94,21 +96,19 @@ __global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const 
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
     const float inv_h = 1.0f / static_cast<float>(h);
     P x;
-    float own = 0.0f, own_w = 0.0f, own_b = 0.0f;
-    auto load = [&](int64_t r) {
-        const T *row = from + r * h;
-        x.load(row + at.head, inner);
-        if (at.own) own = to_f(row[at.column]);
-    };
-    if (mine.first < a.rows) load(mine.first);
+    float own = 0.0f;
     stage_weights<T, kVec>(weights, a.weight, fp32, 1.0f, at.head, inner);
     stage_weights<T, kVec>(weights + inner, a.bias, fp32, 0.0f, at.head, inner);
-    if (at.own) {
-        own_w = weight_at<T>(a.weight, fp32, at.column, 1.0f);
-        own_b = weight_at<T>(a.bias, fp32, at.column, 0.0f);
+    if (at.own && team == 0) {
+        ends[0][threadIdx.x] = weight_at<T>(a.weight, fp32, at.column, 1.0f);
+        ends[1][threadIdx.x] = weight_at<T>(a.bias, fp32, at.column, 0.0f);
     }
     __syncthreads();
-    for (int64_t r = mine.first; r < a.rows;) {
+    const int rows = static_cast<int>(a.rows), stride = static_cast<int>(mine.stride);
+    for (int r = static_cast<int>(mine.first); r < rows; r += stride) {
+        const T *const row = from + static_cast<int64_t>(r) * h;
+        x.load(row + at.head, inner);
+        if (at.own) own = to_f(row[at.column]);
         f32x2 s = pk2(own, 0.0f);
 #pragma unroll
         for (int g = 0; g < P::kGroups; ++g)
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const 
         const float mean = sum(make_float2(both(s), 0.0f)).x * inv_h;
         const f32x2 mean2 = pk2(mean, mean);
         const float own_d = at.own ? own - mean : 0.0f;
+        x.keep_packed();
         f32x2 q = pk2(own_d * own_d, 0.0f);
 #pragma unroll
         for (int g = 0; g < P::kGroups; ++g) {
@@ -134,7 +135,8 @@ __global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const 
             a.rstd[r] = rstd;
         }
         const f32x2 rstd2 = pk2(rstd, rstd);
-        T *const out = static_cast<T *>(a.out) + r * h;
+        x.keep_packed();
+        T *const out = static_cast<T *>(a.out) + static_cast<int64_t>(r) * h;
 #pragma unroll
         for (int g = 0; g < P::kGroups; ++g) {
             if (!P::first(g, inner)) continue;
@@ -145,9 +147,7 @@ __global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const 
             for (int i = 0; i < P::kPairs; ++i) y[i] = ffma2(fmul2(fsub2(x.pair(g, i), mean2), rstd2), w[i], b[i]);
             P::store(out + at.head, g, inner, y);
         }
-        if (at.own) out[at.column] = from_f<T>(fmaf(own_d * rstd, own_w, own_b));
-        r += mine.stride;
-        if (r < a.rows) load(r);
+        if (at.own) out[at.column] = from_f<T>(fmaf((own - mean) * rstd, ends[0][threadIdx.x], ends[1][threadIdx.x]));
     }
 }
 
@@ -187,8 +187,14 @@ cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream) {
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         const bool whole = aligned && a.hidden * static_cast<int64_t>(sizeof(T)) % 16 == 0;
-        const bool ragged = !whole && start_alike(a.x, a.out) && ragged_length(a.hidden, sizeof(T));
+        const bool ragged = !whole && start_alike(a.x, a.out) && ragged_length(a.hidden, sizeof(T)) &&
+                            a.rows < (int64_t{1} << 30);  // counted in 32 bits
         TeamPlan plan = team_plan(a.hidden, sizeof(T), whole || ragged, kForwardBlock);
+        // With five pieces of eight elements a thread registers spill (32760 x 5121: 155 us, with three 147).
+        if (ragged && plan.pieces == 5 && sizeof(T) == 2 && plan.threads < kForwardBlock) {
+            plan.threads *= 2;
+            plan.pieces = 3;
+        }
         if (plan.pieces == 0) {
             const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
             return with_weight<T>(a, [&](auto w) {

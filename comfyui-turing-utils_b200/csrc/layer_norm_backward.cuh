@@ -7,13 +7,15 @@
 // registers; one CTA an SM leaves one partial sum per column, joined in order by a second kernel (equal
 // shapes add in equal order).  Sums are fp32; each result is rounded once.
 //
-// Bytes in flight bound it: where rows start on 16 bytes, a team's next rows of x and dy are copied into
-// shared memory (bulk copies, two rows deep) while it works on one, and the weights are there as fp32, so
-// registers hold the sums alone.  Other rows are kept in registers as loaded; rows wider than a team holds
-// take the looping kernels.
+// Bytes in flight bound it: a team's next rows of x and dy are copied into shared memory (bulk copies, two
+// rows deep; fp32 rows beyond 10240 values, one deep) while it works on one, and the weights are there as fp32,
+// so registers hold the sums alone.  Of rows off 16 bytes that is the inner part.  Where x, dy and dx do not
+// start alike within 16 bytes, rows are kept in registers, loaded by single elements; rows wider than a team
+// holds take the looping kernels.
 //
 // Measured: 4096 x 5120 bf16 36 us and 5 for the join (54 us with rows in registers); each further row costs
-// what its bytes take at 5.7 TB/s.
+// what its bytes take at 5.7 TB/s.  32760 x 5121 245 us (aligned, 5120 wide: 180); 6000 x 13823 fp32 194 us,
+// 5.1 TB/s (looping 486).
 #pragma once
 
 #include "layer_norm_parts.cuh"
@@ -144,6 +146,8 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
     using P = Part<T, kVec, kPieces, kTeam>;
     constexpr int kTeams = kBackwardBlock / kTeam;
     constexpr bool kNamed = kTeam > 32 && kTeams > 1;
+    constexpr int kDepth = kPieces > 5 ? 1 : 2;  // rows in shared memory: of the widest, one
+    static_assert(kDepth == 2 || kTeams == 1, "the barrier below is the CTA's");
     __shared__ float2 part[kTeams][2][20];
     __shared__ uint64_t bars[kTeams][2];
     extern __shared__ __align__(16) uint8_t smem[];
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         mbar_init(&bars[team][1], 1);
         fence_mbar_init();
         if (first < a.rows) load(first, 0);
-        if (first + stride < a.rows) load(first + stride, 1);
+        if (kDepth == 2 && first + stride < a.rows) load(first + stride, 1);
     }
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
     stage_weights<T, kVec>(weights, a.weight, fp32, 1.0f, head, h);
@@ -247,7 +251,7 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         const float2 st = sum(make_float2(both(s), both(t)));
         // Every thread of the team is past the row before: its buffer takes the row after the next.
         if (kTeam == 32) __syncwarp();
-        if (threadIdx.x == 0 && r != first && r + stride < a.rows) {
+        if (kDepth == 2 && threadIdx.x == 0 && r != first && r + stride < a.rows) {
             fence_proxy_async_smem();
             load(r + stride, buf ^ 1);
         }
@@ -270,8 +274,17 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
                 P::store(dx + r * a.hidden + head, g, h, out);
             }
         }
-        buf ^= 1;
-        if (buf == 0) phase ^= 1u;
+        if (kDepth == 2) {
+            buf ^= 1;
+            if (buf == 0) phase ^= 1u;
+        } else {
+            __syncthreads();
+            if (threadIdx.x == 0 && r + stride < a.rows) {
+                fence_proxy_async_smem();
+                load(r + stride, 0);
+            }
+            phase ^= 1u;
+        }
     }
     leave_sums<P>(a, dw, db, OwnSums{head, h, at.column, has_own, own_dw, own_db}, reinterpret_cast<float *>(smem));
 }
@@ -356,8 +369,8 @@ __global__ void __launch_bounds__(256) parameter_partial_kernel(const AffineArgs
 }  // namespace
 
 namespace {
-int staged_smem(int hidden, int bytes, int teams) {
-    return hidden / 4 * 16 + teams * 4 * (hidden * bytes / 16 * 16);
+int staged_smem(int hidden, int bytes, int teams, int depth) {
+    return hidden / 4 * 16 + teams * 2 * depth * (hidden * bytes / 16 * 16);
 }
 }  // namespace
 
@@ -368,7 +381,9 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     const bool ragged = !whole && start_alike(a.x, a.grad) && start_alike(a.x, a.dx) && ragged_length(a.hidden, sizeof(T));
     const bool params = a.dweight || a.dbias;
     TeamPlan plan = team_plan(a.hidden, sizeof(T), whole || ragged, kBackwardBlock);
-    if (plan.pieces != 0 && plan.vec > 1 && staged_smem(a.hidden, sizeof(T), kBackwardBlock / plan.threads) > kMaxSmem)
+    const int depth = plan.pieces > 5 ? 1 : 2;
+    if (plan.pieces != 0 && plan.vec > 1 &&
+        staged_smem(a.hidden, sizeof(T), kBackwardBlock / plan.threads, depth) > kMaxSmem)
         plan.pieces = 0;
     if (plan.pieces == 0) {
         const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
@@ -397,7 +412,7 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
                 if (cudaError_t f = allow_smem(kernel, done)) return f;
             kernel<<<grid, block, sums, stream>>>(a);
         } else {
-            const int smem = std::max(sums, staged_smem(a.hidden, sizeof(T), plan.teams));
+            const int smem = std::max(sums, staged_smem(a.hidden, sizeof(T), plan.teams, depth));
             auto launch = [&](auto kernel, std::atomic<bool>(&done)[64]) {
                 if (cudaError_t f = allow_smem(kernel, done)) return f;
                 kernel<<<grid, block, smem, stream>>>(a);

@@ -90,6 +90,13 @@ struct Part {
                 single[p] = c < h ? row[c] : from_f<T>(0.0f);
         }
     }
+    // Makes the compiler convert the elements again where they are used next, instead of keeping them as fp32.
+    __device__ __forceinline__ void keep_packed() {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+            if constexpr (kWide && sizeof(T) == 2)
+                asm volatile("" : "+r"(wide[p].x), "+r"(wide[p].y), "+r"(wide[p].z), "+r"(wide[p].w));
+    }
     __device__ __forceinline__ f32x2 pair(int g, int i) const {
         if constexpr (!kWide) return pk2(to_f(single[2 * g]), to_f(single[2 * g + 1]));
         const uint32_t w[4] = {wide[g].x, wide[g].y, wide[g].z, wide[g].w};
@@ -298,7 +305,8 @@ struct TeamPlan {
     int vec, pieces, threads, teams;
 };
 
-// Five wide pieces (sixteen single elements) a thread at most, and as few threads as hold the row that way:
+// Five wide pieces (sixteen single elements; seven of four fp32 values where five do not hold the row) a thread
+// at most, and as few threads as hold the row that way:
 // more rows are in flight, and what a row costs a warp besides its elements is spread over more of them.
 // With wide pieces the kernels know the team's size: a power of two up to `block`, or `block`.
 inline TeamPlan team_plan(int64_t hidden, int bytes, bool wide, int block) {
@@ -307,7 +315,10 @@ inline TeamPlan team_plan(int64_t hidden, int bytes, bool wide, int block) {
     const int64_t count = hidden / p.vec;
     const int most = p.vec == 1 ? 16 : 5;
     int64_t threads = ((count + most - 1) / most + 31) / 32 * 32;
-    if (threads > block) return p;
+    if (threads > block) {
+        if (!wide || bytes != 4 || count > 7 * block) return p;
+        threads = block;
+    }
     if (p.vec > 1) {
         int64_t t = 32;
         while (t < threads) t *= 2;
@@ -340,8 +351,11 @@ cudaError_t with_threads(int threads, F f) {
     if constexpr (kVec == 1) {
         return f(vec, pieces, integral_constant<int, 0>());
     } else {
-        if (threads == 32) return f(vec, pieces, integral_constant<int, 32>());
-        if constexpr (kPieces >= 3) {
+        if constexpr (kPieces <= 5)
+            if (threads == 32) return f(vec, pieces, integral_constant<int, 32>());
+        if constexpr (kPieces > 5) {
+            if (threads == kBlock) return f(vec, pieces, integral_constant<int, kBlock>());
+        } else if constexpr (kPieces >= 3) {
             switch (threads) {
             case 64: return f(vec, pieces, integral_constant<int, 64>());
             case 128: return f(vec, pieces, integral_constant<int, 128>());
@@ -370,8 +384,14 @@ cudaError_t with_shape(const TeamPlan &p, F f) {
     case 2: return with_threads<kBlock, kFull, 2>(p.threads, f);
     case 3: return with_threads<kBlock, kFull, 3>(p.threads, f);
     case 4: return with_threads<kBlock, kFull, 4>(p.threads, f);
-    default: return with_threads<kBlock, kFull, 5>(p.threads, f);
+    case 5: return with_threads<kBlock, kFull, 5>(p.threads, f);
+    default: break;
     }
+    if constexpr (sizeof(T) == 4) {
+        if (p.pieces == 6) return with_threads<kBlock, kFull, 6>(p.threads, f);
+        if (p.pieces == 7) return with_threads<kBlock, kFull, 7>(p.threads, f);
+    }
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace

@@ -285,3 +285,18 @@ def test_rows_anywhere_within_16_bytes(k, rows, hidden, dtype, offset, result_of
     check(y, (dx, dw, db), x, w, b, dy)
     assert (outside(y_buf, result_offset) == -77).all() and (outside(dx_buf, result_offset) == -77).all()
     assert (work[room:] == -77).all()
+
+
+# fp32 rows that take more than five pieces a thread, more rows than CTAs.
+@pytest.mark.parametrize("rows,hidden", [(450, 10244), (310, 12289), (150, 14336), (149, 14335), (20, 14345)])
+def test_widest_fp32_rows(k, rows, hidden):
+    x, w, b, dy = make(rows, hidden, torch.float32, torch.float32, hidden)
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    y = k.turing_layer_norm(x, w, b, EPS)
+    grads = torch.autograd.grad(y, (x, w, b), dy)
+    check(y.detach(), grads, x.detach(), w.detach(), b.detach(), dy)
+    # The weights' gradients alone: the rows' own are not asked for.
+    y = k.turing_layer_norm(x.detach(), w, b, EPS)
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    assert torch.equal(dw, grads[1]) and torch.equal(db, grads[2])
