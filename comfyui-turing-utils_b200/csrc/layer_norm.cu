@@ -6,7 +6,7 @@
 // a team of lanes (a warp, or a CTA of several) keeps a row in registers, as loaded, so x is read once;
 // arithmetic is on packed fp32 pairs.  32760 x 5120 bf16: 115 us, 5.84 TB/s (0.90 of a copy's rate); with the
 // team's size a launch parameter, so that each access computed its address and bounds, 154 us.  Rows off 16
-// bytes: 32760 x 5121 147 us (with loads of single elements 540 us).  Rows wider than a team holds take the
+// bytes: 32760 x 5121 119 us (with loads of single elements 540 us).  Rows wider than a team holds take the
 // looping kernel.
 #include "layer_norm_parts.cuh"
 
@@ -117,7 +117,6 @@ __global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const 
         const float mean = sum(make_float2(both(s), 0.0f)).x * inv_h;
         const f32x2 mean2 = pk2(mean, mean);
         const float own_d = at.own ? own - mean : 0.0f;
-        x.keep_packed();
         f32x2 q = pk2(own_d * own_d, 0.0f);
 #pragma unroll
         for (int g = 0; g < P::kGroups; ++g) {
@@ -135,7 +134,6 @@ __global__ void __launch_bounds__(kForwardBlock, 2) ragged_forward_kernel(const 
             a.rstd[r] = rstd;
         }
         const f32x2 rstd2 = pk2(rstd, rstd);
-        x.keep_packed();
         T *const out = static_cast<T *>(a.out) + static_cast<int64_t>(r) * h;
 #pragma unroll
         for (int g = 0; g < P::kGroups; ++g) {
@@ -190,11 +188,6 @@ cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream) {
         const bool ragged = !whole && start_alike(a.x, a.out) && ragged_length(a.hidden, sizeof(T)) &&
                             a.rows < (int64_t{1} << 30);  // counted in 32 bits
         TeamPlan plan = team_plan(a.hidden, sizeof(T), whole || ragged, kForwardBlock);
-        // With five pieces of eight elements a thread registers spill (32760 x 5121: 155 us, with three 147).
-        if (ragged && plan.pieces == 5 && sizeof(T) == 2 && plan.threads < kForwardBlock) {
-            plan.threads *= 2;
-            plan.pieces = 3;
-        }
         if (plan.pieces == 0) {
             const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, a.num_sms * 8));
             return with_weight<T>(a, [&](auto w) {

@@ -14,7 +14,7 @@
 // holds take the looping kernels.
 //
 // Measured: 4096 x 5120 bf16 36 us and 5 for the join (54 us with rows in registers); each further row costs
-// what its bytes take at 5.7 TB/s.  32760 x 5121 245 us (aligned, 5120 wide: 180); 6000 x 13823 fp32 194 us,
+// what its bytes take at 5.7 TB/s.  32760 x 5121 204 us (aligned, 5120 wide: 180); 6000 x 13823 fp32 194 us,
 // 5.1 TB/s (looping 486).
 #pragma once
 
@@ -150,11 +150,17 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
     static_assert(kDepth == 2 || kTeams == 1, "the barrier below is the CTA's");
     __shared__ float2 part[kTeams][2][20];
     __shared__ uint64_t bars[kTeams][2];
+    // Of a thread's own element, in shared memory as registers are short (32760 x 5121 bf16: 246 us with them in
+    // registers and rows counted in 64 bits, 204 so): weight, sums of dw and db, and the row's dy * w and xhat.
+    enum { kOwnW, kOwnDw, kOwnDb, kOwnGw, kOwnN };
+    __shared__ float ends[kRagged ? kTeams : 1][5][16];
     extern __shared__ __align__(16) uint8_t smem[];
     const int team = threadIdx.y;
     const TeamRows<kRagged ? kVec : 1> mine(kTeams, team);
-    const int64_t stride = mine.stride, first = mine.first;
-    const Ragged<kVec> at(static_cast<const T *>(a.x) + first * a.hidden, a.hidden);
+    // Rows are counted in 32 bits: backward_as sees to it that they can be.
+    const int stride = static_cast<int>(mine.stride), first = static_cast<int>(mine.first);
+    const int rows_end = static_cast<int>(a.rows);
+    const Ragged<kVec> at(static_cast<const T *>(a.x) + static_cast<int64_t>(first) * a.hidden, a.hidden);
     const int head = kRagged ? at.head : 0;
     const int h = kRagged ? at.inner : a.hidden;  // of a row's part on 16 bytes
     const bool has_own = kRagged && at.own;
@@ -165,29 +171,34 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
     const float inv_h = 1.0f / static_cast<float>(a.hidden);
     T *const dx = static_cast<T *>(a.dx);
 
-    auto load = [&](int64_t r, int buf) {  // one thread of the team
+    auto load = [&](int r, int buf) {  // one thread of the team
         uint8_t *dst = rows + buf * 2 * row_bytes;
-        mbar_arrive_expect_tx(&bars[team][buf], 2 * row_bytes);
-        bulk_load(dst, static_cast<const T *>(a.x) + r * a.hidden + head, row_bytes, &bars[team][buf]);
-        bulk_load(dst + row_bytes, static_cast<const T *>(a.grad) + r * a.hidden + head, row_bytes, &bars[team][buf]);
+        uint64_t *bar = &bars[team][buf];
+        const int64_t from = static_cast<int64_t>(r) * a.hidden + head;
+        mbar_arrive_expect_tx(bar, 2 * row_bytes);
+        bulk_load(dst, static_cast<const T *>(a.x) + from, row_bytes, bar);
+        bulk_load(dst + row_bytes, static_cast<const T *>(a.grad) + from, row_bytes, bar);
     };
     if (threadIdx.x == 0) {
         mbar_init(&bars[team][0], 1);
         mbar_init(&bars[team][1], 1);
         fence_mbar_init();
-        if (first < a.rows) load(first, 0);
-        if (kDepth == 2 && first + stride < a.rows) load(first + stride, 1);
+        if (first < rows_end) load(first, 0);
+        if (kDepth == 2 && first + stride < rows_end) load(first + stride, 1);
     }
     const bool fp32 = a.weight_dtype == CTU_DTYPE_FP32;
     stage_weights<T, kVec>(weights, a.weight, fp32, 1.0f, head, h);
-    float own_x = 0.0f, own_dy = 0.0f, own_w = 0.0f, own_dw = 0.0f, own_db = 0.0f;
-    auto load_own = [&](int64_t r) {
-        own_x = to_f(static_cast<const T *>(a.x)[r * a.hidden + at.column]);
-        own_dy = to_f(static_cast<const T *>(a.grad)[r * a.hidden + at.column]);
+    float own_x = 0.0f, own_dy = 0.0f;
+    auto own = [&](int what) -> float & { return ends[kRagged ? team : 0][what][threadIdx.x]; };
+    auto load_own = [&](int r) {
+        const int64_t from = static_cast<int64_t>(r) * a.hidden + at.column;
+        own_x = to_f(static_cast<const T *>(a.x)[from]);
+        own_dy = to_f(static_cast<const T *>(a.grad)[from]);
     };
     if (has_own) {
-        own_w = weight_at<T>(a.weight, fp32, at.column, 1.0f);
-        if (first < a.rows) load_own(first);
+        own(kOwnW) = weight_at<T>(a.weight, fp32, at.column, 1.0f);
+        own(kOwnDw) = own(kOwnDb) = 0.0f;
+        if (first < rows_end) load_own(first);
     }
     __syncthreads();
 
@@ -205,31 +216,31 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         staged_weights<kVec>(weights, h, c, w);
     };
     float next_mean = 0.0f, next_rstd = 0.0f;
-    if (first < a.rows) {
+    if (first < rows_end) {
         next_mean = a.mean[first];
         next_rstd = a.rstd[first];
     }
     int buf = 0;
     uint32_t phase = 0;
-    for (int64_t r = first; r < a.rows; r += stride) {
+    for (int r = first; r < rows_end; r += stride) {
         const float mean = next_mean, rstd = next_rstd;
         const f32x2 mean2 = pk2(mean, mean), rstd2 = pk2(rstd, rstd);
-        if (r + stride < a.rows) {
+        if (r + stride < rows_end) {
             next_mean = a.mean[r + stride];
             next_rstd = a.rstd[r + stride];
         }
         mbar_wait(&bars[team][buf], phase, nullptr, a.err, kErrTimeoutFull);
         const uint8_t *row = rows + buf * 2 * row_bytes;
         f32x2 s = pk2(0.0f, 0.0f), t = s;
-        float own_n = 0.0f, own_gw = 0.0f;
         if (has_own) {
-            own_n = (own_x - mean) * rstd;
-            own_gw = own_dy * own_w;
-            own_dw = fmaf(own_dy, own_n, own_dw);
-            own_db += own_dy;
-            s = pk2(own_gw, 0.0f);
-            t = pk2(own_gw * own_n, 0.0f);
-            if (r + stride < a.rows) load_own(r + stride);
+            const float n = (own_x - mean) * rstd, gw = own_dy * own(kOwnW);
+            own(kOwnDw) = fmaf(own_dy, n, own(kOwnDw));
+            own(kOwnDb) += own_dy;
+            own(kOwnGw) = gw;
+            own(kOwnN) = n;
+            s = pk2(gw, 0.0f);
+            t = pk2(gw * n, 0.0f);
+            if (r + stride < rows_end) load_own(r + stride);
         }
 #pragma unroll
         for (int g = 0; g < P::kGroups; ++g) {
@@ -251,15 +262,15 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         const float2 st = sum(make_float2(both(s), both(t)));
         // Every thread of the team is past the row before: its buffer takes the row after the next.
         if (kTeam == 32) __syncwarp();
-        if (kDepth == 2 && threadIdx.x == 0 && r != first && r + stride < a.rows) {
+        if (kDepth == 2 && threadIdx.x == 0 && r != first && r + stride < rows_end) {
             fence_proxy_async_smem();
             load(r + stride, buf ^ 1);
         }
         const f32x2 minus_s = pk2(-st.x * inv_h, -st.x * inv_h), minus_t = pk2(-st.y * inv_h, -st.y * inv_h);
         if (dx != nullptr) {
             if (has_own)
-                dx[r * a.hidden + at.column] =
-                    from_f<T>(rstd * (own_gw - st.x * inv_h - own_n * (st.y * inv_h)));
+                dx[static_cast<int64_t>(r) * a.hidden + at.column] =
+                    from_f<T>(rstd * (own(kOwnGw) - st.x * inv_h - own(kOwnN) * (st.y * inv_h)));
 #pragma unroll
             for (int g = 0; g < P::kGroups; ++g) {
                 if (!P::first(g, h)) continue;
@@ -271,7 +282,7 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
                     const f32x2 n = fmul2(fsub2(x.pair(0, i), mean2), rstd2);
                     out[i] = fmul2(rstd2, ffma2(n, minus_t, ffma2(dy.pair(0, i), w[i], minus_s)));
                 }
-                P::store(dx + r * a.hidden + head, g, h, out);
+                P::store(dx + static_cast<int64_t>(r) * a.hidden + head, g, h, out);
             }
         }
         if (kDepth == 2) {
@@ -279,14 +290,14 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
             if (buf == 0) phase ^= 1u;
         } else {
             __syncthreads();
-            if (threadIdx.x == 0 && r + stride < a.rows) {
+            if (threadIdx.x == 0 && r + stride < rows_end) {
                 fence_proxy_async_smem();
                 load(r + stride, 0);
             }
             phase ^= 1u;
         }
     }
-    leave_sums<P>(a, dw, db, OwnSums{head, h, at.column, has_own, own_dw, own_db}, reinterpret_cast<float *>(smem));
+    leave_sums<P>(a, dw, db, OwnSums{head, h, at.column, has_own, has_own ? own(kOwnDw) : 0.0f, has_own ? own(kOwnDb) : 0.0f}, reinterpret_cast<float *>(smem));
 }
 
 // Slices of partial sums joined: 32 columns by 8 runs of slices a block.
@@ -380,7 +391,8 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     const bool whole = aligned && a.hidden * static_cast<int64_t>(sizeof(T)) % 16 == 0;
     const bool ragged = !whole && start_alike(a.x, a.grad) && start_alike(a.x, a.dx) && ragged_length(a.hidden, sizeof(T));
     const bool params = a.dweight || a.dbias;
-    TeamPlan plan = team_plan(a.hidden, sizeof(T), whole || ragged, kBackwardBlock);
+    const bool counted = a.rows < (int64_t{1} << 30);
+    TeamPlan plan = team_plan(a.hidden, sizeof(T), counted && (whole || ragged), kBackwardBlock);
     const int depth = plan.pieces > 5 ? 1 : 2;
     if (plan.pieces != 0 && plan.vec > 1 &&
         staged_smem(a.hidden, sizeof(T), kBackwardBlock / plan.threads, depth) > kMaxSmem)
@@ -401,7 +413,7 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     }
     plan.teams = plan.vec > 1 ? kBackwardBlock / plan.threads : std::min(15, kBackwardBlock / plan.threads);
     const int64_t ctas = std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, kSlices);
-    const int period = ragged ? plan.vec : 1;
+    const int period = ragged ? plan.vec : 1;  // vec 1: of single elements
     const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, ragged_grid(a.rows, ctas, period)));
     const cudaError_t e = with_shape<T, kBackwardBlock>(plan, [&](auto vec, auto pieces, auto threads) {
         const dim3 block(plan.threads, plan.teams);

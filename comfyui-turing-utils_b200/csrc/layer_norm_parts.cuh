@@ -90,13 +90,6 @@ struct Part {
                 single[p] = c < h ? row[c] : from_f<T>(0.0f);
         }
     }
-    // Makes the compiler convert the elements again where they are used next, instead of keeping them as fp32.
-    __device__ __forceinline__ void keep_packed() {
-#pragma unroll
-        for (int p = 0; p < kPieces; ++p)
-            if constexpr (kWide && sizeof(T) == 2)
-                asm volatile("" : "+r"(wide[p].x), "+r"(wide[p].y), "+r"(wide[p].z), "+r"(wide[p].w));
-    }
     __device__ __forceinline__ f32x2 pair(int g, int i) const {
         if constexpr (!kWide) return pk2(to_f(single[2 * g]), to_f(single[2 * g + 1]));
         const uint32_t w[4] = {wide[g].x, wide[g].y, wide[g].z, wide[g].w};
