@@ -297,7 +297,9 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
             phase ^= 1u;
         }
     }
-    leave_sums<P>(a, dw, db, OwnSums{head, h, at.column, has_own, has_own ? own(kOwnDw) : 0.0f, has_own ? own(kOwnDb) : 0.0f}, reinterpret_cast<float *>(smem));
+    leave_sums<P>(a, dw, db,
+                  OwnSums{head, h, at.column, has_own, has_own ? own(kOwnDw) : 0.0f, has_own ? own(kOwnDb) : 0.0f},
+                  reinterpret_cast<float *>(smem));
 }
 
 // Slices of partial sums joined: 32 columns by 8 runs of slices a block.
@@ -389,7 +391,8 @@ template <typename T>
 cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     const bool aligned = row_aligned(a.x) && row_aligned(a.grad) && row_aligned(a.dx);
     const bool whole = aligned && a.hidden * static_cast<int64_t>(sizeof(T)) % 16 == 0;
-    const bool ragged = !whole && start_alike(a.x, a.grad) && start_alike(a.x, a.dx) && ragged_length(a.hidden, sizeof(T));
+    const bool ragged =
+        !whole && start_alike(a.x, a.grad) && start_alike(a.x, a.dx) && ragged_length(a.hidden, sizeof(T));
     const bool params = a.dweight || a.dbias;
     const bool counted = a.rows < (int64_t{1} << 30);
     TeamPlan plan = team_plan(a.hidden, sizeof(T), counted && (whole || ragged), kBackwardBlock);
@@ -415,7 +418,7 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     const int64_t ctas = std::min<int64_t>((a.rows + plan.teams - 1) / plan.teams, kSlices);
     const int period = ragged ? plan.vec : 1;  // vec 1: of single elements
     const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, ragged_grid(a.rows, ctas, period)));
-    const cudaError_t e = with_shape<T, kBackwardBlock>(plan, [&](auto vec, auto pieces, auto threads) {
+    const cudaError_t e = with_shape<T, kBackwardBlock, sizeof(T) == 4>(plan, [&](auto vec, auto pieces, auto threads) {
         const dim3 block(plan.threads, plan.teams);
         const int sums = params ? plan.teams * 2 * a.hidden * static_cast<int>(sizeof(float)) : 0;
         if constexpr (vec == 1) {

@@ -114,7 +114,8 @@ struct Part {
         }
     }
     // One group of weights (of the input's type or fp32), `fill` where there are none.
-    static __device__ __forceinline__ void weights(const void *p, bool fp32, int g, int h, float fill, f32x2 (&out)[kPairs]) {
+    static __device__ __forceinline__ void weights(const void *p, bool fp32, int g, int h, float fill,
+                                                   f32x2 (&out)[kPairs]) {
         if (p == nullptr) {
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) out[i] = pk2(fill, fill);
@@ -299,8 +300,8 @@ struct TeamPlan {
 };
 
 // Five wide pieces (sixteen single elements; seven of four fp32 values where five do not hold the row) a thread
-// at most, and as few threads as hold the row that way:
-// more rows are in flight, and what a row costs a warp besides its elements is spread over more of them.
+// at most, and as few threads as hold the row that way: more rows are in flight, and what a row costs a warp
+// besides its elements is spread over more of them.
 // With wide pieces the kernels know the team's size: a power of two up to `block`, or `block`.
 inline TeamPlan team_plan(int64_t hidden, int bytes, bool wide, int block) {
     TeamPlan p{};
@@ -335,7 +336,7 @@ inline bool ragged_length(int64_t hidden, int bytes) { return hidden * bytes >= 
 
 // Calls f(vec, pieces, threads) with the plan's values as constants (threads 0 with single elements).  With
 // wide loads that is 32 threads and one to five pieces, or more threads and what fewer do not hold: three to
-// five.
+// five; with kSeven also six and seven, of `block` threads, or of half as many with 16-bit values.
 template <int kBlock, int kVec, int kPieces, typename F>
 cudaError_t with_threads(int threads, F f) {
     using std::integral_constant;
@@ -347,7 +348,8 @@ cudaError_t with_threads(int threads, F f) {
         if constexpr (kPieces <= 5)
             if (threads == 32) return f(vec, pieces, integral_constant<int, 32>());
         if constexpr (kPieces > 5) {
-            if (threads == kBlock) return f(vec, pieces, integral_constant<int, kBlock>());
+            constexpr int kWidest = kVec == 8 ? kBlock / 2 : kBlock;
+            if (threads == kWidest) return f(vec, pieces, integral_constant<int, kWidest>());
         } else if constexpr (kPieces >= 3) {
             switch (threads) {
             case 64: return f(vec, pieces, integral_constant<int, 64>());
@@ -361,7 +363,7 @@ cudaError_t with_threads(int threads, F f) {
     }
 }
 
-template <typename T, int kBlock, typename F>
+template <typename T, int kBlock, bool kSeven, typename F>
 cudaError_t with_shape(const TeamPlan &p, F f) {
     constexpr int kFull = 16 / sizeof(T);
     if (p.vec == 1) {
@@ -380,7 +382,7 @@ cudaError_t with_shape(const TeamPlan &p, F f) {
     case 5: return with_threads<kBlock, kFull, 5>(p.threads, f);
     default: break;
     }
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (kSeven) {
         if (p.pieces == 6) return with_threads<kBlock, kFull, 6>(p.threads, f);
         if (p.pieces == 7) return with_threads<kBlock, kFull, 7>(p.threads, f);
     }
