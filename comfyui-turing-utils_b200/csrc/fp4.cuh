@@ -93,7 +93,7 @@ constexpr int kPairRows = 256;  // output rows of a pair tile
 constexpr int kPairCols = 256;
 int linear_pair_smem();
 const void *linear_pair_kernel(int format);
-int linear_pair_threads(bool few_tiles);
+int linear_pair_threads(bool few_tiles, int64_t n, int64_t k);
 
 // Gradient with respect to the input: dx[m, k] = grad[m, n] w[n, k], rotated back.
 struct GradArgs {

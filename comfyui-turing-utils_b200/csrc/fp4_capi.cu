@@ -310,11 +310,11 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
     }
     const void *kernel = fp4::linear_pair_kernel(format);
     int clusters = 0;
-    if (int rc = pair_clusters(g_linear_plan[format], kernel, fp4::linear_pair_threads(true), fp4::linear_pair_smem(), q,
-                               &clusters))
+    if (int rc = pair_clusters(g_linear_plan[format], kernel, fp4::linear_pair_threads(true, n, k),
+                               fp4::linear_pair_smem(), q, &clusters))
         return rc;
     void *params[] = {&map_a, &map_b, &map_as, &map_bs, &map_out, &args};
-    return launch_pairs(kernel, fp4::linear_pair_threads(tiles <= 2 * clusters), fp4::linear_pair_smem(),
+    return launch_pairs(kernel, fp4::linear_pair_threads(tiles <= 2 * clusters, n, k), fp4::linear_pair_smem(),
                         std::min<int64_t>(tiles, clusters), params, static_cast<cudaStream_t>(stream));
 }
 

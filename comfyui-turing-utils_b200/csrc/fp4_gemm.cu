@@ -61,8 +61,8 @@ struct Shared {
     uint64_t drain;
     uint32_t tmem_base;
     int abort_flag;
-    float col_scale[kPairCols];
-    float col_bias[kPairCols];
+    alignas(16) float col_scale[kPairCols];
+    alignas(16) float col_bias[kPairCols];
 };
 
 constexpr int kSmem = kStructOffset + static_cast<int>(sizeof(Shared)) + 1024;
@@ -248,6 +248,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             tc_fence_after();
             const int m_warp = m0 + quad * 32;
             const float a_s = m_warp + lane < args.m ? args.a_scale[m_warp + lane] : 0.0f;
+            const f32x2 a_s2 = pk2(a_s, a_s);
 #pragma unroll 1
             for (int i = share; i < kPairCols / kOutCols; i += sharers) {
                 // The piece with the shared columns first: the last one of the first accumulator, the first
@@ -274,15 +275,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
+                        const int col = c * kOutCols + 32 * h + 8 * q;
                         uint32_t p[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int e = 8 * q + 2 * j;
-                            const int col = c * kOutCols + 32 * h + e;
-                            p[j] = pack_bf16x2(
-                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][e]), a_s), S.col_scale[col], S.col_bias[col]),
-                                __fmaf_rn(__fmul_rn(__uint_as_float(acc[h][e + 1]), a_s), S.col_scale[col + 1],
-                                          S.col_bias[col + 1]));
+                        for (int j = 0; j < 4; j += 2) {
+                            const ulonglong2 scale = *reinterpret_cast<const ulonglong2 *>(&S.col_scale[col + 2 * j]);
+                            const ulonglong2 bias = *reinterpret_cast<const ulonglong2 *>(&S.col_bias[col + 2 * j]);
+                            const uint32_t *from = acc[h] + 8 * q + 2 * j;
+                            float v[4];
+                            const f32x2 lo = fmul2(pk2(__uint_as_float(from[0]), __uint_as_float(from[1])), a_s2);
+                            const f32x2 hi = fmul2(pk2(__uint_as_float(from[2]), __uint_as_float(from[3])), a_s2);
+                            unpk2(ffma2(lo, scale.x, bias.x), v[0], v[1]);
+                            unpk2(ffma2(hi, scale.y, bias.y), v[2], v[3]);
+                            p[j] = pack_bf16x2(v[0], v[1]);
+                            p[j + 1] = pack_bf16x2(v[2], v[3]);
                         }
                         st_shared_v4(staged + 128u * lane + ((static_cast<uint32_t>(4 * h + q) ^ (lane & 7u)) << 4), p);
                     }
@@ -315,9 +321,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
 
 int linear_pair_smem() { return kSmem; }
 // Eight epilogue warps shorten the way from a tile's last MMA to its output, which is what few tiles wait
-// for (1025 x 1537 x 1568: 12.7 us against 14.8 with four); four leave more to the MMAs where tiles follow
-// one another.
-int linear_pair_threads(bool few_tiles) { return few_tiles ? kThreadCount : 32 * (2 + 4); }
+// for (1025 x 1537 x 1568: 12.7 us against 14.8 with four), what short tiles do (13679 x 1856 x 2304: 35 against
+// 39) and what rows off 16 bytes need, which warps write themselves (8894 x 8395 x 1888: 125 against 160).  Four
+// leave more to the MMAs of long tiles that follow one another (32760 x 13824 x 5120: 871 against 899).
+int linear_pair_threads(bool few_tiles, int64_t n, int64_t k) {
+    return few_tiles || n % 8 != 0 || k < 4096 ? kThreadCount : 32 * (2 + 4);
+}
 const void *linear_pair_kernel(int format) {
     return format == kNvfp4 ? reinterpret_cast<const void *>(&fp4_linear_pair_kernel<kNvfp4>)
                             : reinterpret_cast<const void *>(&fp4_linear_pair_kernel<kMxfp4>);
