@@ -5,7 +5,7 @@
 //
 // A thread keeps the same columns for every row its team takes and holds their sums of dw and db in
 // registers; one CTA an SM leaves one partial sum per column, joined in order by a second kernel (equal
-// shapes add in equal order).  Sums are fp32; each result is rounded once.
+// shapes that start alike within 16 bytes add in equal order).  Sums are fp32; each result is rounded once.
 //
 // Bytes in flight bound it: a team's next rows of x and dy are copied into shared memory (bulk copies, two
 // rows deep; fp32 rows beyond 10240 values, one deep) while it works on one, and the weights are there as fp32,

@@ -316,7 +316,7 @@ CTU_API int ctu_layer_norm(const void *x, const void *weight, const void *bias, 
  * Its backward pass: dx [rows, hidden] (dtype), dweight and dbias [hidden] (weight_dtype); any of the
  * three may be NULL.  workspace holds the partial sums of dweight and dbias
  * (ctu_layer_norm_backward_workspace_bytes); it is not needed for dx alone.  The order of every sum is
- * fixed by the shapes, so equal inputs give equal bits.
+ * fixed by the shapes, the types and where the tensors start within 16 bytes: equal calls give equal bits.
  */
 CTU_API int64_t ctu_layer_norm_backward_workspace_bytes(int64_t rows, int64_t hidden);
 CTU_API int ctu_layer_norm_backward(const void *grad, const void *x, const void *weight, const float *mean,

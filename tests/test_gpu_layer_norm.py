@@ -300,3 +300,43 @@ def test_widest_fp32_rows(k, rows, hidden):
     y = k.turing_layer_norm(x.detach(), w, b, EPS)
     dw, db = torch.autograd.grad(y, (w, b), dy)
     assert torch.equal(dw, grads[1]) and torch.equal(db, grads[2])
+
+
+# Rows that share 16 bytes with their neighbours.
+@pytest.mark.parametrize("dtype,hidden", [(torch.bfloat16, 641), (torch.float16, 5121), (torch.float32, 1027)])
+def test_rows_off_16_bytes_stay_alone(k, dtype, hidden):
+    x, w, b, dy = make(40, hidden, dtype, torch.float32, 8)
+    leaf = x.clone().requires_grad_(True)
+    clean = k.turing_layer_norm(leaf, w, b, EPS)
+    clean_dx = torch.autograd.grad(clean, leaf, dy)[0]
+    bad = x.clone()
+    bad[3, 0], bad[7, -1], bad[20, hidden // 2] = float("nan"), float("inf"), float("-inf")
+    bad.requires_grad_(True)
+    y = k.turing_layer_norm(bad, w, b, EPS)
+    dx = torch.autograd.grad(y, bad, dy)[0]
+    rows = [i in (3, 7, 20) for i in range(40)]
+    assert torch.isnan(y).all(1).tolist() == rows and torch.isnan(dx).any(1).tolist() == rows
+    keep = [i for i in range(40) if not rows[i]]
+    assert torch.equal(y[keep], clean[keep]) and torch.equal(dx[keep], clean_dx[keep])
+
+
+@pytest.mark.parametrize("dtype,hidden", [(torch.bfloat16, 1537), (torch.float32, 10245)])
+def test_off_16_bytes_captured_and_again(k, dtype, hidden):
+    x, w, b, dy = make(900, hidden, dtype, torch.float32, 9)
+
+    def step():
+        y, mean, rstd = torch.ops.turing_utils.layer_norm(x, w, b, EPS)
+        return (y, *torch.ops.turing_utils.layer_norm_backward(dy, x, mean, rstd, w, b, 7))
+
+    first = [t.clone() for t in step()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(2):
+        for t in held:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, c) for a, c in zip(first, held))
+    x.mul_(0.5)
+    graph.replay()
+    assert all(torch.equal(a, c) for a, c in zip(step(), held))
