@@ -340,3 +340,15 @@ def test_off_16_bytes_captured_and_again(k, dtype, hidden):
     x.mul_(0.5)
     graph.replay()
     assert all(torch.equal(a, c) for a, c in zip(step(), held))
+
+
+# Rows on 16 bytes, several to each of the backward pass's teams (one to sixteen a CTA), whose buffers are loaded again and
+# again; the last round of rows leaves some teams without one.
+@pytest.mark.parametrize("dtype,wdtype", TYPES)
+@pytest.mark.parametrize("rows,hidden", [(9001, 640), (5003, 1536), (3001, 5120), (1201, 10240), (701, 13824)])
+def test_several_rows_a_team(k, rows, hidden, dtype, wdtype):
+    x, w, b, dy = make(rows, hidden, dtype, wdtype, rows + hidden)
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    y = k.turing_layer_norm(x, w, b, EPS)
+    check(y.detach(), torch.autograd.grad(y, (x, w, b), dy), x.detach(), w.detach(), b.detach(), dy)
