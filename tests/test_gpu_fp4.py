@@ -559,3 +559,38 @@ def test_gradient_repeats_bits(k, m, n, width, rotation):
         width, 1, torch.cuda.current_stream().cuda_stream))
     assert torch.equal(buf[1 : 1 + m], first) and (buf[0] == 7).all() and (buf[-1] == 7).all()
     assert (work[room:] == 9).all()
+
+
+# ---------------------------------------------------------------------------- more tiles than pairs
+def random_operand(k, rows, width, fmt, seed):
+    """Codes, tiles and row scales drawn as bytes on the GPU, and the values that they stand for (float64,
+    there too): sizes for which the oracle on the host takes too long."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    low, high, dtype = (48, 73, torch.float8_e4m3fn) if fmt == "nvfp4" else (124, 130, torch.float8_e8m0fnu)
+    codes = torch.randint(0, 256, (rows, width // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.randint(low, high, (rows, width // oracle.BLOCK[fmt]), generator=g, device="cuda", dtype=torch.uint8)
+    row = torch.exp2(torch.randint(-6, -3, (rows, 1), generator=g, device="cuda").float())
+    grid = torch.from_numpy(np.concatenate((oracle.GRID, -oracle.GRID))).cuda()
+    v = grid[torch.stack((codes & 15, codes >> 4), 2).view(rows, width).int()]
+    v = v * torch.from_numpy(oracle.scale_values(fmt)).cuda()[scales.int()].repeat_interleave(oracle.BLOCK[fmt], 1)
+    return (codes, k.turing_fp4_block_scale_tiles(scales.view(dtype)), row), v * row.double()
+
+
+# A B200 runs 74 CTA pairs: each takes three to four tiles here, so both accumulators, the tensor-memory columns that they
+# share and the ring's phase go from tile to tile.  By size: output rows on 16 bytes (tile stores) or not, K from
+# 4096 on (four epilogue warps, on 16 bytes) or below (eight), one stage a tile, last tiles that end inside.
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,width", [(3850, 3976, 4128), (3850, 3975, 4128), (3850, 3976, 544), (3850, 3973, 544),
+                                       (4096, 4096, 256), (57100, 248, 4096), (200, 75000, 1056)])
+def test_linear_of_several_tiles_a_pair(k, fmt, m, n, width):
+    (a, a_s, a_r), av = random_operand(k, m, width, fmt, m + n)
+    (w, w_s, w_r), wv = random_operand(k, n, width, fmt, n + width)
+    bias = torch.linspace(-30, 30, n, device="cuda")
+    out = k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r, bias)
+    exact = av @ wv.t() + bias.double()
+    # linear_bound's, over the whole output.
+    steps = -(-width // 64) + 8
+    bound = HALF_BF16 * exact.abs() + 2 * steps * 2.0**-23 * (av.abs() @ wv.t().abs()) + 1e-37
+    worst = ((out.double() - exact).abs() / bound).max().item()
+    assert worst <= 1, worst
+    assert torch.equal(out, k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r, bias))
