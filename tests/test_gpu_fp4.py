@@ -576,6 +576,11 @@ def random_operand(k, rows, width, fmt, seed):
     return (codes, k.turing_fp4_block_scale_tiles(scales.view(dtype)), row), v * row.double()
 
 
+def rotate64(v):
+    r = torch.from_numpy(oracle.rotation_matrix()).to(v.device)
+    return (v.view(-1, 256) @ r).view(v.shape), r.abs()
+
+
 # A B200 runs 74 CTA pairs: each takes three to four tiles here, so both accumulators, the tensor-memory columns that they
 # share and the ring's phase go from tile to tile.  By size: output rows on 16 bytes (tile stores) or not, K from
 # 4096 on (four epilogue warps, on 16 bytes) or below (eight), one stage a tile, last tiles that end inside.
@@ -594,3 +599,30 @@ def test_linear_of_several_tiles_a_pair(k, fmt, m, n, width):
     worst = ((out.double() - exact).abs() / bound).max().item()
     assert worst <= 1, worst
     assert torch.equal(out, k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r, bias))
+
+
+# More work items than pairs: tiles of several rounds without a split, and whole tiles beside the parts of the last
+# round's, whose sums a second kernel joins; rows, columns and sums that end inside a tile.
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,width,rotation,mixed", [(4700, 1000, 4352, 256, False), (4790, 520, 4000, 0, False),
+                                                      (2450, 5000, 2080, 0, True), (2300, 4104, 2304, 256, True),
+                                                      (4096, 5120, 5120, 256, True)])
+def test_gradient_of_several_items_a_pair(k, fmt, m, n, width, rotation, mixed):
+    from comfyui_turing_utils_kernel import _lib
+
+    tiles = -(-m // 256) * -(-width // 256)
+    parts = (_lib.load().ctu_fp4_grad_workspace_bytes(m, n, width) - 2 * n * width) // (256 * 256 * 4)
+    assert tiles > 74 and (parts > tiles % 74 if mixed else parts == 0)
+    (w, w_s, w_r), wd = random_operand(k, n, width, fmt, n + width)
+    g = torch.randn(m, n, device="cuda", generator=torch.Generator("cuda").manual_seed(m)).bfloat16()
+    dx = k.turing_fp4_linear_grad_input(g, w, w_s, w_r, rotation)
+    exact, mags = g.double() @ wd, g.double().abs() @ wd.abs()
+    # As in test_grad_input.
+    off = (-(-n // 16) + 4) * 2.0**-23 * mags + 16 * 2.0**-24 * mags
+    if rotation:
+        exact, r = rotate64(exact)
+        off = (off.view(-1, 256) @ r).view(off.shape) + (12 + 16) * 2.0**-24 * (mags.view(-1, 256) @ r).view(off.shape)
+    bound = HALF_BF16 * (exact.abs() + off) + off + 1e-37
+    worst = ((dx.double() - exact).abs() / bound).max().item()
+    assert worst <= 1, worst
+    assert torch.equal(dx, k.turing_fp4_linear_grad_input(g, w, w_s, w_r, rotation))
