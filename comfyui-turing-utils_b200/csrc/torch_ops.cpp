@@ -11,6 +11,7 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -250,6 +251,13 @@ void no_second_derivative(const char *what) {
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative");  // create_graph=True
 }
 
+// A tangent would be lost below the autograd keys, and read as zero by whoever asks for it.
+void no_forward_mode(const char *what, std::initializer_list<OptTensor> inputs) {
+    for (const OptTensor &t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.has_value() || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
+                                    " has no forward-mode derivative");
+}
+
 struct LayerNormGrad : torch::autograd::Function<LayerNormGrad> {
     static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &weight, const OptTensor &bias,
                                  double epsilon) {
@@ -269,6 +277,7 @@ struct LayerNormGrad : torch::autograd::Function<LayerNormGrad> {
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
         no_second_derivative("LayerNorm");
+        no_forward_mode("the LayerNorm gradient", {grads[0]});
         static const auto op = c10::Dispatcher::singleton()
                                    .findSchemaOrThrow("turing_utils::layer_norm_backward", "")
                                    .typed<Three(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
@@ -283,6 +292,7 @@ struct LayerNormGrad : torch::autograd::Function<LayerNormGrad> {
 };
 
 Three layer_norm_autograd(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double epsilon) {
+    no_forward_mode("LayerNorm", {x, weight, bias});
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias))) {
         const variable_list out = LayerNormGrad::apply(x, weight, bias, epsilon);
         return {out[0], out[1], out[2]};
@@ -313,6 +323,7 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
 
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         no_second_derivative("the FP4 linear");
+        no_forward_mode("the FP4 linear's gradient", {grads[0]});
         static const auto op =
             c10::Dispatcher::singleton()
                 .findSchemaOrThrow("turing_utils::fp4_linear_grad_input", "")
@@ -326,6 +337,7 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
 
 Tensor convrot_fp4_linear_autograd(const Tensor &x, const Tensor &weight, const Tensor &weight_block_scale,
                                    const Tensor &weight_scale, const OptTensor &bias, int64_t rotation) {
+    no_forward_mode("the FP4 linear", {x, weight_scale, bias});
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight_scale.requires_grad() || wants_grad(bias)))
         return LinearGrad::apply(x, weight, weight_block_scale, weight_scale, bias, rotation);
     static const auto op = c10::Dispatcher::singleton()

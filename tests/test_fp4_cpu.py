@@ -181,3 +181,50 @@ def test_wrapper_refusals():
         dispatch.convrot_fp4_linear(x, x, x, x, convrot_groupsize=128)
     with pytest.raises(RuntimeError, match="does not fit"):
         fusions.affine_layer_norm(torch.nn.LayerNorm([2, 256]), x)
+
+
+def differentiable_calls():
+    """(call, differentiable leaves) of the differentiable ops on meta tensors."""
+    import comfyui_turing_utils_kernel as k
+
+    x = torch.empty((3, 512), dtype=torch.bfloat16, device="meta")
+    codes, scale, row = k.turing_fp4_quantize(torch.empty((24, 512), dtype=torch.bfloat16, device="meta"), "nvfp4", 256)
+    norm = torch.empty((2, 3, 64), device="meta"), torch.empty(64, device="meta"), torch.empty(64, device="meta")
+    return [(lambda x: k.turing_convrot_fp4_linear(x, codes, scale, row), (x,)), (k.turing_layer_norm, norm)]
+
+
+@pytest.mark.parametrize("requires_grad", (False, True))
+@pytest.mark.parametrize("no_grad", (False, True))
+def test_forward_mode_is_refused(requires_grad, no_grad):
+    """There is no forward-mode derivative: a tangent raises, it does not come out as zero."""
+    import torch.autograd.forward_ad as fwd
+
+    for call, leaves in differentiable_calls():
+        for i in range(len(leaves)):
+            args = [t.clone().requires_grad_(requires_grad) for t in leaves]
+            with fwd.dual_level(), torch.set_grad_enabled(not no_grad):
+                args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*args)
+                primals = [fwd.unpack_dual(t).primal for t in args]
+                assert call(*primals).shape == call(*leaves).shape  # without a tangent it runs inside the level too
+
+
+def test_functional_forward_mode_is_refused():
+    for call, leaves in differentiable_calls():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, leaves, tuple(torch.ones_like(t) for t in leaves))
+
+
+def test_tangent_of_a_gradient_is_refused():
+    """Forward mode over the backward pass: the gradient that comes in carries the tangent."""
+    import torch.autograd.forward_ad as fwd
+
+    for call, leaves in differentiable_calls():
+        args = [t.clone().requires_grad_(True) for t in leaves]
+        y = call(*args)
+        with fwd.dual_level():
+            grad = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, args, grad, retain_graph=True)
+        assert torch.autograd.grad(y, args, torch.ones_like(y))[0].shape == leaves[0].shape
