@@ -45,6 +45,7 @@ def _torch_command(out: Path) -> list[str]:
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            f'-DCTU_BUILT_FOR_TORCH="{torch.__version__}"',
             f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda}/include",
             str(CSRC / "torch_ops.cpp"), "-o", str(out), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
             f"-L{OUT_DIR}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
@@ -61,6 +62,16 @@ def _stale(target: Path, deps) -> bool:
         return True
     t = target.stat().st_mtime
     return any(Path(d).stat().st_mtime > t for d in deps)
+
+
+def _torch_stale(target: Path) -> bool:
+    """Older than its sources, or built for another torch than the installed one."""
+    import torch
+
+    if _stale(target, [CSRC / "torch_ops.cpp", INCLUDE / "ctu_b200.h"]):
+        return True
+    mark = b"ctu-built-for-torch=" + torch.__version__.encode() + b"\0"
+    return mark not in target.read_bytes()
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -89,7 +100,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link failed")
         os.replace(tmp, LIB)
-    if force or _stale(TORCH_LIB, [CSRC / "torch_ops.cpp", INCLUDE / "ctu_b200.h"]):
+    if force or _torch_stale(TORCH_LIB):
         tmp = TORCH_LIB.with_suffix(f".so.{os.getpid()}.tmp")
         res = subprocess.run(_torch_command(tmp), capture_output=True, text=True)
         if res.returncode != 0:

@@ -8,6 +8,7 @@ raises instead of computing anything.
 from __future__ import annotations
 
 import ctypes
+import re
 import threading
 from pathlib import Path
 
@@ -101,18 +102,29 @@ def load():
     return _lib
 
 
+def torch_bindings_version(path: Path) -> str | None:
+    """The torch version that the bindings at ``path`` were built for (a mark in the file), or None."""
+    mark = re.search(rb"ctu-built-for-torch=([^\0]+)\0", path.read_bytes())
+    return mark.group(1).decode() if mark else None
+
+
 def load_torch_ops() -> None:
-    """Register the ops of libctu_torch.so, the torch bindings next to the CUDA library."""
+    """Register the ops of libctu_torch.so, the torch bindings next to the CUDA library.  They use torch's
+    C++ interface, which changes between versions: a library for another torch is not loaded."""
     import torch
 
     load()
     path = _LIB_PATH.with_name("libctu_torch.so")
     if not path.exists():
         raise KernelUnavailable(f"{path} is not built; run comfyui-turing-utils_b200/build.py")
+    version = torch_bindings_version(path)
+    if version != torch.__version__:
+        raise KernelUnavailable(f"{path} is built for torch {version}, not for {torch.__version__}; "
+                                "run comfyui-turing-utils_b200/build.py")
     try:
         torch.ops.load_library(str(path))
     except OSError as exc:
-        raise KernelUnavailable(str(exc)) from exc
+        raise KernelUnavailable(f"{path}: {exc}") from exc
 
 
 def check(rc: int) -> None:

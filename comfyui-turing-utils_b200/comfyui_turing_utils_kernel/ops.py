@@ -8,6 +8,8 @@ the matching function of ``_C`` (the C-ABI shim); there is no CPU path.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _C, _lib
@@ -471,13 +473,35 @@ def _turing_w4a4_g128_linear_fake(activation, weight, activation_scale, weight_s
 # 4-bit floating point linear and affine layer norm (no reference ops; arithmetic and layouts in
 # ctu_b200.h).  A single token's call is bound by host time, so these ops, their checks and their
 # gradients are registered from C++ (csrc/torch_ops.cpp): 1 x 5120 x 5120 costs 17 us of host time as a
-# Python op over ctypes.  Their fake kernels are here.
-_lib.load_torch_ops()
+# Python op over ctypes.  Their fake kernels are here.  Where the library of bindings does not fit the installed
+# torch, these ops refuse and the others, which need no such library, work.
+try:
+    _lib.load_torch_ops()
+    _torch_ops_error = None
+except _lib.KernelUnavailable as exc:
+    _torch_ops_error = str(exc)
+
+
+def _register_fake(name: str):
+    return torch.library.register_fake(name) if _torch_ops_error is None else lambda fn: fn
+
+
+def _torch_op(fn):
+    """``fn``, or a refusal in its place where the bindings are not loaded."""
+    if _torch_ops_error is None:
+        return fn
+
+    @functools.wraps(fn)
+    def refuse(*args, **kwargs):
+        raise _lib.KernelUnavailable(_torch_ops_error)
+
+    return refuse
+
 
 _FP4_FORMATS = {"nvfp4": (16, torch.float8_e4m3fn), "mxfp4": (32, torch.float8_e8m0fnu)}
 
 
-@torch.library.register_fake("turing_utils::fp4_quantize")
+@_register_fake("turing_utils::fp4_quantize")
 def _fp4_quantize_fake(x, format="nvfp4", rotation=0):
     block, dtype = _FP4_FORMATS[format]
     rows, k = x.shape
@@ -486,6 +510,7 @@ def _fp4_quantize_fake(x, format="nvfp4", rotation=0):
             x.new_empty((rows, 1), dtype=torch.float32))
 
 
+@_torch_op
 def turing_fp4_quantize(x: torch.Tensor, format: str = "nvfp4", rotation: int = 0):
     """bf16/fp16 rows to 4-bit floating point: (packed codes, block scale tiles, row scales).
 
@@ -494,11 +519,12 @@ def turing_fp4_quantize(x: torch.Tensor, format: str = "nvfp4", rotation: int = 
     return torch.ops.turing_utils.fp4_quantize.default(x, format, rotation)
 
 
-@torch.library.register_fake("turing_utils::fp4_dequantize")
+@_register_fake("turing_utils::fp4_dequantize")
 def _fp4_dequantize_fake(codes, block_scale, scale, out_dtype=torch.bfloat16):
     return codes.new_empty((codes.size(0), codes.size(1) * 2), dtype=out_dtype)
 
 
+@_torch_op
 def turing_fp4_dequantize(codes: torch.Tensor, block_scale: torch.Tensor, scale: torch.Tensor,
                           out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that FP4 codes and scales stand for (rotated values stay rotated); ``scale`` is one
@@ -506,12 +532,13 @@ def turing_fp4_dequantize(codes: torch.Tensor, block_scale: torch.Tensor, scale:
     return torch.ops.turing_utils.fp4_dequantize.default(codes, block_scale, scale, out_dtype)
 
 
-@torch.library.register_fake("turing_utils::fp4_linear")
+@_register_fake("turing_utils::fp4_linear")
 def _fp4_linear_fake(activation, weight, activation_block_scale, weight_block_scale, activation_scale, weight_scale,
                      bias=None):
     return activation.new_empty((activation.size(0), weight.size(0)), dtype=torch.bfloat16)
 
 
+@_torch_op
 def turing_fp4_linear(activation: torch.Tensor, weight: torch.Tensor, activation_block_scale: torch.Tensor,
                       weight_block_scale: torch.Tensor, activation_scale: torch.Tensor, weight_scale: torch.Tensor,
                       bias: torch.Tensor | None = None) -> torch.Tensor:
@@ -520,11 +547,12 @@ def turing_fp4_linear(activation: torch.Tensor, weight: torch.Tensor, activation
                                                      activation_scale, weight_scale, bias)
 
 
-@torch.library.register_fake("turing_utils::fp4_linear_grad_input")
+@_register_fake("turing_utils::fp4_linear_grad_input")
 def _fp4_linear_grad_input_fake(grad_output, weight, weight_block_scale, weight_scale, rotation=0):
     return grad_output.new_empty((grad_output.size(0), weight.size(1) * 2))
 
 
+@_torch_op
 def turing_fp4_linear_grad_input(grad_output: torch.Tensor, weight: torch.Tensor, weight_block_scale: torch.Tensor,
                                  weight_scale: torch.Tensor, rotation: int = 0) -> torch.Tensor:
     """Gradient with respect to the input of a linear with frozen FP4 weights: bf16 [m, k]."""
@@ -532,11 +560,12 @@ def turing_fp4_linear_grad_input(grad_output: torch.Tensor, weight: torch.Tensor
                                                                 rotation)
 
 
-@torch.library.register_fake("turing_utils::convrot_fp4_linear")
+@_register_fake("turing_utils::convrot_fp4_linear")
 def _convrot_fp4_linear_fake(x, weight, weight_block_scale, weight_scale, bias=None, rotation=256):
     return x.new_empty((x.size(0), weight.size(0)), dtype=torch.bfloat16)
 
 
+@_torch_op
 def turing_convrot_fp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_block_scale: torch.Tensor,
                               weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
                               rotation: int = 256) -> torch.Tensor:
@@ -546,14 +575,14 @@ def turing_convrot_fp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_bloc
     return torch.ops.turing_utils.convrot_fp4_linear.default(x, weight, weight_block_scale, weight_scale, bias, rotation)
 
 
-@torch.library.register_fake("turing_utils::layer_norm")
+@_register_fake("turing_utils::layer_norm")
 def _layer_norm_fake(x, weight=None, bias=None, epsilon=1.0e-5):
     rows = x.numel() // x.size(-1)
     return (torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(rows, dtype=torch.float32),
             x.new_empty(rows, dtype=torch.float32))
 
 
-@torch.library.register_fake("turing_utils::layer_norm_backward")
+@_register_fake("turing_utils::layer_norm_backward")
 def _layer_norm_backward_fake(grad, x, mean, rstd, weight=None, bias=None, needs=7):
     none = x.new_empty(0)
     return (torch.empty_like(x, memory_format=torch.contiguous_format) if needs & 1 else none,
@@ -561,6 +590,7 @@ def _layer_norm_backward_fake(grad, x, mean, rstd, weight=None, bias=None, needs
             torch.empty_like(bias) if needs & 4 and bias is not None else none)
 
 
+@_torch_op
 def turing_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                       epsilon: float = 1.0e-5) -> torch.Tensor:
     """Affine layer norm over the last dimension, differentiable in x, weight and bias.

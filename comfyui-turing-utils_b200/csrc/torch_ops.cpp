@@ -18,6 +18,10 @@
 
 #include "../../include/ctu_b200.h"
 
+// The torch build that this library fits, read from the file before it is loaded.
+extern "C" __attribute__((visibility("default"), used)) const char ctu_built_for_torch[] =
+    "ctu-built-for-torch=" CTU_BUILT_FOR_TORCH;
+
 namespace {
 
 using at::Tensor;
