@@ -61,6 +61,7 @@ SIGNATURES = {
     "ctu_fp4_dequantize": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp]),
     "ctu_fp4_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "ctu_debug_set_fp4_kernel": (_i32, [_i32]),
+    "ctu_debug_inject_timeout": (_i32, [_i32, _u64]),
     "ctu_fp4_grad_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "ctu_fp4_linear_grad_input": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "ctu_debug_set_gemm_kernel": (_i32, [_i32]),

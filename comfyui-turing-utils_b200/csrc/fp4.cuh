@@ -31,6 +31,13 @@ __host__ __device__ constexpr int64_t scale_offset(int64_t r, int64_t b, int64_t
     return ((r >> 7) * col_tiles + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
 }
 
+// Limit of a kernel's waits.  Test hook: wait `never` (counted from 0) of the first CTA for a copy is on a barrier
+// that nothing arrives on; -1: none.
+struct WaitLimit {
+    uint64_t ns;
+    int never;
+};
+
 struct QuantArgs {
     const void *x;          // [rows, k]
     uint8_t *codes;         // [rows, k / 2]
@@ -75,6 +82,7 @@ struct LinearArgs {
     int w_scale_count;
     int format;
     int split;  // CTAs of a cluster that share K (the kernel for few rows)
+    WaitLimit wait;
 };
 
 // Kernel for few rows: a strip of 128 weight rows per CTA, `tokens` activation rows at a time.

@@ -13,6 +13,7 @@
 #include "fp4.cuh"
 #include "host.cuh"
 #include "layer_norm.cuh"
+#include "ptx.cuh"
 
 namespace {
 
@@ -138,6 +139,13 @@ std::atomic<int> g_fp4_kernel{0};
 bool few_rows(int64_t m, int64_t n, int64_t k, int num_sms) {
     const int64_t strips = (n + fp4::kStripRows - 1) / fp4::kStripRows;
     return m <= 64 || (m <= 128 && 2 * strips <= num_sms && k >= 1024);
+}
+
+// Limit of the kernels' waits, and one that a test makes run out.
+std::atomic<uint64_t> g_wait_ns{ctu::kWaitLimitNs};
+std::atomic<int> g_wait_never{-1};
+fp4::WaitLimit wait_limit() {
+    return {g_wait_ns.load(std::memory_order_relaxed), g_wait_never.load(std::memory_order_relaxed)};
 }
 
 SmemPlan g_small_plan[8];
@@ -271,7 +279,7 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
     if (int rc = kernel_device(&q, &err)) return rc;
     const int col_tiles = format == CTU_FP4_NVFP4 ? 4 : 2;
     fp4::LinearArgs args{a_scale, w_scale, bias, out, err, static_cast<int>(m), static_cast<int>(n),
-                         static_cast<int>(k), w_scale_count == 1 ? 1 : 0, format, 1};
+                         static_cast<int>(k), w_scale_count == 1 ? 1 : 0, format, 1, wait_limit()};
     const int forced = g_fp4_kernel.load(std::memory_order_relaxed);
     if (forced == 2 || (forced == 0 && few_rows(m, n, k, q.num_sms))) {
         const fp4::SmallKernel sk = fp4::linear_small_kernel(format, m);
@@ -321,6 +329,14 @@ int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_block_sc
 int ctu_debug_set_fp4_kernel(int which) {
     if (which < 0 || which > 2) return fail(CTU_ERR_INVALID_ARGUMENT, "unknown FP4 product kernel %d", which);
     return g_fp4_kernel.exchange(which);
+}
+
+int ctu_debug_inject_timeout(int which, uint64_t limit_ns) {
+    if (which >= 0 && (limit_ns == 0 || limit_ns > 5000000000ull))
+        return fail(CTU_ERR_INVALID_ARGUMENT, "wait limit must be in (0, 5 s]");
+    g_wait_ns.store(which < 0 ? ctu::kWaitLimitNs : limit_ns, std::memory_order_relaxed);
+    g_wait_never.store(which < 0 ? -1 : which, std::memory_order_relaxed);
+    return CTU_OK;
 }
 
 int64_t ctu_fp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k) {

@@ -53,8 +53,10 @@ struct Shared {
     uint64_t empty[9];
     uint64_t acc_full;
     uint64_t drain;
+    uint64_t issued;  // `copies` is final
     uint32_t tmem_base;
     int abort_flag;
+    int copies;
 };
 
 __device__ __forceinline__ void tma_load_3d(void *smem_dst, const void *tmap, int x, int y, int z, uint64_t *bar) {
@@ -148,10 +150,12 @@ __global__ void __launch_bounds__(kThreadCount)
         }
         mbar_init(&S.acc_full, 1);
         mbar_init(&S.drain, 1);
+        mbar_init(&S.issued, 1);
         S.abort_flag = 0;
         fence_mbar_init();
     }
     volatile int *abort_flag = &S.abort_flag;
+    const uint64_t limit = args.wait.ns;
     auto load = [&](int s, int kb) {
         mbar_arrive_expect_tx(&S.full[s], kStageTx);
         tma_load_2d(smem + s * kABytes, &tmap_w, kb * 128, n0, &S.full[s]);
@@ -178,20 +182,15 @@ __global__ void __launch_bounds__(kThreadCount)
             uint32_t ph = 1;
             int fills = first;
             for (; fills < nk; ++fills) {
-                if (!mbar_wait(&S.empty[s], ph ^ 1u, abort_flag, args.err, kErrTimeoutEmpty)) break;
+                if (!mbar_wait(&S.empty[s], ph ^ 1u, abort_flag, args.err, kErrTimeoutEmpty, limit)) break;
                 load(s, k_begin + fills);
                 if (++s == kStages) {
                     s = 0;
                     ph ^= 1u;
                 }
             }
-            if (fills < nk || *abort_flag) {
-                // Copies in flight land before the CTA leaves.
-                for (int i = 0; i < kStages && i < fills; ++i) {
-                    const int f = fills - 1 - i;
-                    mbar_wait(&S.full[f % kStages], (f / kStages) & 1, nullptr, args.err, kErrTimeoutDrain);
-                }
-            }
+            S.copies = fills;
+            mbar_arrive(&S.issued);
         }
     } else if (warp == 1) {
         int s = 0;
@@ -202,8 +201,10 @@ __global__ void __launch_bounds__(kThreadCount)
         const uint32_t as0 = smem_desc_low(smem_u32(smem + L::kAScaleOffset));
         const uint32_t bs0 = smem_desc_low(smem_u32(smem + L::kBScaleOffset));
         bool ok = true;
-        for (int kb = 0; kb < nk; ++kb) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&S.full[s], ph, abort_flag, args.err, kErrTimeoutFull));
+        const int never = blockIdx.x == 0 ? args.wait.never : -1;
+        const int stop = never >= 0 ? min(nk, never) : nk;
+        for (int kb = 0; kb < stop; ++kb) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&S.full[s], ph, abort_flag, args.err, kErrTimeoutFull, limit));
             if (!ok) break;
             tc_fence_after();
             const uint32_t sa = tmem_base + L::kScaleCol + set * 32;
@@ -236,28 +237,40 @@ __global__ void __launch_bounds__(kThreadCount)
                 ph ^= 1u;
             }
         }
+        if (stop < nk) ok = __all_sync(0xffffffffu, mbar_wait(&S.drain, 0u, abort_flag, args.err, kErrTimeoutFull, limit));
         if (!ok) {  // no last commit comes: wait for what was issued
             if (elect_one()) mma_commit(&S.drain);
             __syncwarp();
-            mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+            mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain, limit);
         }
     }
     // Everything issued has completed before shared and tensor memory are used otherwise or freed: the
     // last commit covers all MMAs, and each MMA's stage had landed.
     bool alive = true;
-    if (warp >= 1) alive = __all_sync(0xffffffffu, mbar_wait(&S.acc_full, 0u, abort_flag, args.err, kErrTimeoutAccum));
+    if (warp >= 1)
+        alive = __all_sync(0xffffffffu, mbar_wait(&S.acc_full, 0u, abort_flag, args.err, kErrTimeoutAccum, limit));
     tc_fence_after();
 
     const int valid = min(kTokens, args.m - m0);
     if (warp >= 2) {
-        // Partial sums to shared memory, [token][column of the strip]; the lanes are columns here.
+        // Partial sums to shared memory, [token][column of the strip]; the lanes are columns here.  Where a wait
+        // gave up they are NaN, and so is what the cluster makes of them.
         float *part = reinterpret_cast<float *>(smem);
         const int row = (warp & 3) * 32 + lane;
+        if (!alive && mbar_wait(&S.issued, 0u, nullptr, args.err, kErrTimeoutDrain, limit)) {
+            // Copies in flight land before shared memory is used otherwise and before the CTA leaves.
+            for (int f = max(0, S.copies - kStages); f < S.copies; ++f)
+                if (!mbar_wait(&S.full[f % kStages], (f / kStages) & 1, nullptr, args.err, kErrTimeoutDrain, limit)) break;
+        }
 #pragma unroll 1
-        for (int c = 0; c < valid && alive; c += 16) {
+        for (int c = 0; c < valid; c += 16) {
             uint32_t acc[16];
             tmem_ld_32x32b_x16(tmem_base + c + (static_cast<uint32_t>((warp & 3) * 32) << 16), acc);
             tmem_ld_wait();
+            if (!alive) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[j] = 0x7fc00000u;
+            }
 #pragma unroll
             for (int j = 0; j < 16; ++j)
                 if (c + j < valid) part[(c + j) * kStrip + row] = __uint_as_float(acc[j]);
@@ -270,7 +283,7 @@ __global__ void __launch_bounds__(kThreadCount)
             named_barrier(1, 32 * kEpilogueWarps);
         // A warp takes a token, a lane four columns of it.
         const int n = n0 + 4 * lane;
-        if (n < args.n && alive) {
+        if (n < args.n) {
             float w_s[4], bias[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

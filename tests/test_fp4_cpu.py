@@ -228,3 +228,9 @@ def test_tangent_of_a_gradient_is_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(y, args, grad, retain_graph=True)
         assert torch.autograd.grad(y, args, torch.ones_like(y))[0].shape == leaves[0].shape
+
+
+def test_timeout_hook_refusals(lib):
+    for limit in (0, 5_000_000_001):
+        assert refused(lib, lib.ctu_debug_inject_timeout(0, limit), "limit")
+    assert lib.ctu_debug_inject_timeout(3, 1000) == 0 and lib.ctu_debug_inject_timeout(-1, 0) == 0
