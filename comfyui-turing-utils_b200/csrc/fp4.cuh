@@ -50,6 +50,7 @@ struct QuantArgs {
     int dtype;     // CTU_DTYPE_BF16 / FP16
     int num_sms;
     uint32_t *err;
+    WaitLimit wait;
     // Rows side by side: up to eight groups of 256 columns, in a warp (8, 4 or 2 of one, two or four groups,
     // else 1); beyond, in a CTA.
     int side_by_side;

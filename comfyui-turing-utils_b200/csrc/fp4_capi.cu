@@ -210,7 +210,7 @@ int ctu_fp4_quantize(const void *x, int64_t rows, int64_t k, int dtype, int form
     DeviceQuery q;
     uint32_t *err;
     if (int rc = kernel_device(&q, &err)) return rc;
-    fp4::QuantArgs a{x, codes, block_scales, row_scales, rows, static_cast<int>(k), format, rotation, dtype, q.num_sms, err};
+    fp4::QuantArgs a{x, codes, block_scales, row_scales, rows, static_cast<int>(k), format, rotation, dtype, q.num_sms, err, wait_limit()};
     const int groups = static_cast<int>((k + 255) / 256);
     a.side_by_side = groups == 1 ? 8 : groups == 2 ? 4 : groups <= 4 ? 2 : 1;
     // A CTA's warps hold eight groups each: two rows where one would leave more than a tenth of the lanes

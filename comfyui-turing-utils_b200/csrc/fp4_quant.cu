@@ -300,23 +300,26 @@ __device__ __forceinline__ void radix4_pair(f32x2 &x0, f32x2 &x1, f32x2 &x2, f32
 // shared memory.  A lane first holds 64 columns in a row (lane q: 64 q ..) and takes the strides 1, 4
 // and 16 in registers, two tuples to an instruction where the pairing allows; then the four lanes
 // exchange 16-column pieces through the same 8 KB, and stride 64 is in registers too, with whole blocks
-// of 16 left in each lane.  The next row's load runs under the codes of this one.
+// of 16 left in each lane.  The next row's load runs under the codes of this one.  After a wait that gave up a
+// warp loads no more, and its rows come out as those that hold a NaN.
 template <int kFormat, bool kHalf, bool kMulti, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads)
     rotate_quantize_kernel(const __grid_constant__ CUtensorMap tmap, const QuantArgs a) {
     __shared__ float red[2][48];
-    __shared__ uint64_t bars[24];
+    __shared__ uint64_t bars[24], dead;  // dead: nothing arrives on it (test hook)
     extern __shared__ uint8_t smem_raw[];
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)) + warp * 8192;
     const uint32_t base = smem_u32(smem);
     uint64_t *bar = &bars[warp];
+    const uint64_t limit = a.wait.ns;
     const int slots = a.side_by_side;
     const int span = kMulti ? 32 : 32 / slots;
     const int groups = a.k / 256;
-    const int64_t teams = kMulti ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4;
-    const int64_t team = kMulti ? blockIdx.x : blockIdx.x * 4ll + warp;
+    // Rows are counted in 32 bits: x has fewer than 2^31 lines of 64 values.
+    const int rows = static_cast<int>(a.rows), step = static_cast<int>(gridDim.x) * (kMulti ? 1 : 4) * slots;
+    const int first = static_cast<int>(kMulti ? blockIdx.x : blockIdx.x * 4 + warp) * slots;
     const int place = warp * 8 + (lane >> 2);
     const int slot = kMulti ? place / groups : lane / span;
     Place at;
@@ -326,16 +329,17 @@ __global__ void __launch_bounds__(kMaxThreads)
     // several whole rows.
     const int mine = kMulti ? min(8, groups * slots - warp * 8) : slots > 1 ? 8 : groups;
     const int copies = (mine + a.load_groups - 1) / a.load_groups;
-    auto load = [&](int64_t r0) {  // lane 0
+    auto load = [&](int r0) {  // lane 0
         mbar_arrive_expect_tx(bar, static_cast<uint32_t>(copies * a.load_groups * 512));
-        const int64_t line = r0 * (a.k / 64) + (kMulti ? warp * 32 : 0);
+        const int line = r0 * (a.k / 64) + (kMulti ? warp * 32 : 0);
         for (int c = 0; c < copies; ++c)
-            tma_load_2d(smem + c * a.load_groups * 512, &tmap, 0, static_cast<int>(line + c * a.load_groups * 4), bar);
+            tma_load_2d(smem + c * a.load_groups * 512, &tmap, 0, line + c * a.load_groups * 4, bar);
     };
     if (lane == 0) {
         mbar_init(bar, 1);
+        if (warp == 0) mbar_init(&dead, 1);
         fence_mbar_init();
-        if (team * slots < a.rows) load(team * slots);
+        if (first < rows) load(first);
     }
     __syncwarp();
     // 16-byte chunk c of (column digit d3, d2) of this lane's group in the exchange: the address bits are
@@ -347,13 +351,15 @@ __global__ void __launch_bounds__(kMaxThreads)
         return area + ((d3 * 16u + (d2 >> 1) * 8u + low) << 4);
     };
     uint32_t phase = 0;
-    int flip = 0;
-    for (int64_t r0 = team * slots; r0 < a.rows; r0 += teams * slots, flip ^= 1) {
+    bool alive = true;
+    int it = 0;
+    for (int r0 = first; r0 < rows; r0 += step, ++it) {
         at.row = r0 + slot;
         at.active = slot < slots && at.row < a.rows && at.group < groups;
-        mbar_wait(bar, phase, nullptr, a.err, kErrTimeoutFull);
-        phase ^= 1u;
-        __syncwarp();
+        const bool never = it == a.wait.never && blockIdx.x == 0 && warp == 0;
+        if (alive)
+            alive = __all_sync(0xffffffffu, mbar_wait(never ? &dead : bar, never ? 0u : phase, nullptr, a.err, kErrTimeoutFull, limit));
+        if (alive) phase ^= 1u;  // else the phase of the copy that may be in flight
         // x[h][i]: column 16 h + i in the low half, 16 (h + 2) + i in the high half.
         f32x2 x[2][16];
         {
@@ -415,7 +421,7 @@ __global__ void __launch_bounds__(kMaxThreads)
         }
         fence_proxy_async_smem();  // the exchange is over before the next load writes here
         __syncwarp();
-        if (lane == 0 && r0 + teams * slots < a.rows) load(r0 + teams * slots);
+        if (lane == 0 && alive && r0 + step < rows) load(r0 + step);
         float amax[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
@@ -427,8 +433,10 @@ __global__ void __launch_bounds__(kMaxThreads)
                 amax[j] = max_abs3_nan(amax[j], lo, hi);
             }
         }
-        finish<kFormat, kMulti, true>(a, at, amax, span, red[flip], slot, [&](int j, int p) { return v[j][p]; });
+        if (!alive) amax[0] = __uint_as_float(0x7fc00000u);
+        finish<kFormat, kMulti, true>(a, at, amax, span, red[it & 1], slot, [&](int j, int p) { return v[j][p]; });
     }
+    if (!alive) mbar_wait(bar, phase, nullptr, a.err, kErrTimeoutDrain, limit);  // it lands before the CTA leaves
     clear_padding(a, kFormat);
 }
 

@@ -81,3 +81,36 @@ def test_few_rows(k, lib, fmt, m, n, width, which):
         assert torch.equal(call(), whole)
     finally:
         lib.ctu_debug_set_fp4_kernel(before)
+
+
+# ---------------------------------------------------------------------------- rotating quantizer
+@pytest.mark.parametrize("fmt", ("nvfp4", "mxfp4"))
+# Several rows a warp, a row a warp, two rows a CTA of several warps, a row a CTA; the first wait and a later one.
+@pytest.mark.parametrize("rows,width,which", [(70000, 256, 1), (20000, 1280, 2), (9, 2048, 0), (3000, 5120, 1), (1000, 13824, 1),
+                                              (5, 49152, 0)])
+def test_rotating_quantizer(k, lib, fmt, rows, width, which):
+    x = torch.randn(rows, width, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).bfloat16()
+    room = lib.ctu_fp4_block_scale_bytes(rows, width, 0 if fmt == "nvfp4" else 1)
+
+    def call():
+        codes = torch.full((rows, width // 2), 171, dtype=torch.uint8, device="cuda")
+        scales = torch.full((room,), 171, dtype=torch.uint8, device="cuda")
+        row = torch.full((rows,), UNTOUCHED, device="cuda")
+        check(lib.ctu_fp4_quantize(x.data_ptr(), rows, width, 0, 0 if fmt == "nvfp4" else 1, 256, codes.data_ptr(),
+                                   scales.data_ptr(), row.data_ptr(), stream()))
+        # A row's block scales, [rows, blocks], out of the tiles.
+        blocks = width // (16 if fmt == "nvfp4" else 32)
+        plain = scales.view(-(-rows // 128), -1, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-(-rows // 128) * 128, -1)
+        return codes, plain[:rows, :blocks], row
+
+    whole = call()
+    with timeout(which):
+        cut = call()
+    # Each row is as it should be, or comes out as a row with a NaN does: those of the first CTA's rows that the warp has a
+    # part of, from that wait on.
+    same = torch.stack([(p == q).view(rows, -1).all(1) for p, q in zip(whole, cut)])
+    lost = torch.stack([(cut[0] == 0).all(1), (cut[1] == 0).all(1), torch.isnan(cut[2])])
+    done, lost = same.all(0), lost.all(0)
+    assert (done ^ lost).all() and lost.any() and 100 * lost.sum() <= max(rows, 2500)
+    assert bool(lost[0]) == (which == 0)
+    assert all(torch.equal(p, q) for p, q in zip(call(), whole))
