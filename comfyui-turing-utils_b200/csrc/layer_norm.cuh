@@ -27,6 +27,8 @@ struct AffineArgs {
     int weight_dtype;  // CTU_DTYPE_* of weight, bias and their gradients
     int num_sms;
     uint32_t *err;     // the device's error word (bounded waits)
+    uint64_t wait_ns;  // their limit
+    int wait_never;    // test hook: this wait (counted from 0) of the first team is on a barrier nothing arrives on; -1
 };
 
 // Row slices whose partial sums of the weight's and bias's gradients are joined at the end.

@@ -149,7 +149,9 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
     constexpr int kDepth = kPieces > 5 ? 1 : 2;  // rows in shared memory: of the widest, one
     static_assert(kDepth == 2 || kTeams == 1, "the barrier below is the CTA's");
     __shared__ float2 part[kTeams][2][20];
-    __shared__ uint64_t bars[kTeams][2];
+    __shared__ uint64_t bars[kTeams][2], dead;  // dead: nothing arrives on it (test hook)
+    // Whether a wait of a team gave up (its other waits then do at once), and rows whose copies were issued.
+    __shared__ int gave_up[kTeams], issued[kTeams];
     // Of a thread's own element, in shared memory as registers are short (32760 x 5121 bf16: 246 us with them in
     // registers and rows counted in 64 bits, 204 so): weight, sums of dw and db, and the row's dy * w and xhat.
     enum { kOwnW, kOwnDw, kOwnDb, kOwnGw, kOwnN };
@@ -178,10 +180,13 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         mbar_arrive_expect_tx(bar, 2 * row_bytes);
         bulk_load(dst, static_cast<const T *>(a.x) + from, row_bytes, bar);
         bulk_load(dst + row_bytes, static_cast<const T *>(a.grad) + from, row_bytes, bar);
+        ++issued[team];
     };
     if (threadIdx.x == 0) {
         mbar_init(&bars[team][0], 1);
         mbar_init(&bars[team][1], 1);
+        if (team == 0) mbar_init(&dead, 1);
+        gave_up[team] = issued[team] = 0;
         fence_mbar_init();
         if (first < rows_end) load(first, 0);
         if (kDepth == 2 && first + stride < rows_end) load(first + stride, 1);
@@ -220,6 +225,9 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         next_mean = a.mean[first];
         next_rstd = a.rstd[first];
     }
+    // After a wait that gave up the team's rows and its columns' sums are NaN, and no more is loaded.
+    const float nan = __uint_as_float(0x7fc00000u);
+    volatile int *const lost = &gave_up[team];
     int buf = 0;
     uint32_t phase = 0;
     for (int r = first; r < rows_end; r += stride) {
@@ -229,16 +237,18 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
             next_mean = a.mean[r + stride];
             next_rstd = a.rstd[r + stride];
         }
-        mbar_wait(&bars[team][buf], phase, nullptr, a.err, kErrTimeoutFull);
+        const bool never = r == first + a.wait_never * stride && blockIdx.x == 0 && team == 0;
+        mbar_wait(never ? &dead : &bars[team][buf], never ? 0u : phase, lost, a.err, kErrTimeoutFull, a.wait_ns);
+        const float start = *lost ? nan : 0.0f;
         const uint8_t *row = rows + buf * 2 * row_bytes;
-        f32x2 s = pk2(0.0f, 0.0f), t = s;
+        f32x2 s = pk2(0.0f, start), t = pk2(0.0f, 0.0f);
         if (has_own) {
             const float n = (own_x - mean) * rstd, gw = own_dy * own(kOwnW);
             own(kOwnDw) = fmaf(own_dy, n, own(kOwnDw));
             own(kOwnDb) += own_dy;
             own(kOwnGw) = gw;
             own(kOwnN) = n;
-            s = pk2(gw, 0.0f);
+            s = pk2(gw, start);
             t = pk2(gw * n, 0.0f);
             if (r + stride < rows_end) load_own(r + stride);
         }
@@ -262,7 +272,7 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         const float2 st = sum(make_float2(both(s), both(t)));
         // Every thread of the team is past the row before: its buffer takes the row after the next.
         if (kTeam == 32) __syncwarp();
-        if (kDepth == 2 && threadIdx.x == 0 && r != first && r + stride < rows_end) {
+        if (kDepth == 2 && threadIdx.x == 0 && !*lost && r != first && r + stride < rows_end) {
             fence_proxy_async_smem();
             load(r + stride, buf ^ 1);
         }
@@ -290,15 +300,29 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
             if (buf == 0) phase ^= 1u;
         } else {
             __syncthreads();
-            if (threadIdx.x == 0 && r + stride < rows_end) {
+            if (threadIdx.x == 0 && !*lost && r + stride < rows_end) {
                 fence_proxy_async_smem();
                 load(r + stride, 0);
             }
             phase ^= 1u;
         }
     }
+    const bool whole = !*lost;
+    if (!whole) {
+        if (threadIdx.x == 0) {
+            // Copies in flight land before shared memory is used otherwise.
+            for (int i = max(0, issued[team] - kDepth); i < issued[team]; ++i)
+                if (!mbar_wait(&bars[team][i & (kDepth - 1)], (kDepth == 2 ? i >> 1 : i) & 1, nullptr, a.err, kErrTimeoutDrain, a.wait_ns))
+                    break;
+        }
+#pragma unroll
+        for (int g = 0; g < P::kGroups; ++g)
+#pragma unroll
+            for (int i = 0; i < P::kPairs; ++i) dw[g][i] = db[g][i] = pk2(nan, nan);
+    }
+    const bool own_sums = has_own && whole;
     leave_sums<P>(a, dw, db,
-                  OwnSums{head, h, at.column, has_own, has_own ? own(kOwnDw) : 0.0f, has_own ? own(kOwnDb) : 0.0f},
+                  OwnSums{head, h, at.column, has_own, own_sums ? own(kOwnDw) : nan, own_sums ? own(kOwnDb) : nan},
                   reinterpret_cast<float *>(smem));
 }
 

@@ -114,3 +114,37 @@ def test_rotating_quantizer(k, lib, fmt, rows, width, which):
     assert (done ^ lost).all() and lost.any() and 100 * lost.sum() <= max(rows, 2500)
     assert bool(lost[0]) == (which == 0)
     assert all(torch.equal(p, q) for p, q in zip(call(), whole))
+
+
+# ---------------------------------------------------------------------------- layer norm, backward pass
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+# Sixteen teams a CTA, four or two, one; on and off 16 bytes; rows two deep, and (the last, fp32) one deep.
+@pytest.mark.parametrize("rows,hidden,which", [(9000, 320, 1), (5000, 641, 2), (3000, 2560, 0), (2000, 5121, 1), (700, 10240, 2),
+                                               (450, 10244, 1)])
+def test_layer_norm_backward(k, lib, dtype, rows, hidden, which):
+    from test_gpu_layer_norm import formulas, make
+
+    x, w, b, dy = make(rows, hidden, dtype, torch.float32, rows)
+    f = formulas(x, w, b, dy)
+    mean, rstd = f["mean"].float().view(-1), f["rstd"].float().view(-1)
+    room = lib.ctu_layer_norm_backward_workspace_bytes(rows, hidden)
+
+    def call():
+        dx = torch.full_like(x, UNTOUCHED)
+        dw, db = torch.full_like(w, UNTOUCHED), torch.full_like(b, UNTOUCHED)
+        work = torch.full((room // 4,), UNTOUCHED, device="cuda")
+        kind = {torch.bfloat16: 0, torch.float32: 2}[dtype]
+        check(lib.ctu_layer_norm_backward(dy.data_ptr(), x.data_ptr(), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                          dx.data_ptr(), dw.data_ptr(), db.data_ptr(), work.data_ptr(), rows, hidden, kind, 2,
+                                          stream()))
+        return dx, dw, db
+
+    whole = call()
+    with timeout(which):
+        dx, dw, db = call()
+    # The first team's rows from that wait on, and every column's sums.
+    done, lost = (dx == whole[0]).all(1), torch.isnan(dx).all(1)
+    assert (done ^ lost).all() and lost.any() and 20 * lost.sum() <= rows
+    assert bool(lost[0]) == (which == 0)
+    assert torch.isnan(dw).all() and torch.isnan(db).all()
+    assert all(torch.equal(p, q) for p, q in zip(call(), whole))
