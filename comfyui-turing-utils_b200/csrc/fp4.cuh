@@ -113,6 +113,7 @@ struct GradArgs {
     int rotation;
     int whole;  // tiles that are not split, the first ones
     int split;  // parts of the others' sums over n
+    WaitLimit wait;
 };
 constexpr int kGradCols = 256;
 int grad_pair_smem();

@@ -397,7 +397,7 @@ int ctu_fp4_linear_grad_input(const void *grad, const uint8_t *w, const uint8_t 
     const GradPlan plan = grad_plan(m, n, k);
     fp4::GradArgs args{dx, reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + 2 * n * k), err,
                        static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), rotation, static_cast<int>(plan.whole),
-                       static_cast<int>(plan.split)};
+                       static_cast<int>(plan.split), wait_limit()};
     void *params[] = {&map_a, &map_b, &map_out, &args};
     if (int rc = launch_pairs(kernel, fp4::grad_pair_threads(), fp4::grad_pair_smem(),
                               std::min<int64_t>(plan.whole + (plan.tiles - plan.whole) * plan.split, clusters), params, s))

@@ -20,6 +20,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <climits>
+
 #include "fp4.cuh"
 #include "fp4_mma.cuh"
 #include "ptx.cuh"
@@ -121,7 +123,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = S.tmem_base;
-    const PairAbort guard{&S.abort_flag, mapa_shared(smem_u32(&S.abort_flag), rank ^ 1u), args.err};
+    const PairAbort guard{&S.abort_flag, mapa_shared(smem_u32(&S.abort_flag), rank ^ 1u), args.err, args.wait.ns};
     volatile int *abort_flag = &S.abort_flag;
 
     if (warp == 0) {
@@ -150,7 +152,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     }
                 }
             }
-            if (!ok || *abort_flag) settle_inflight_copies();
         }
     } else if (warp == 1) {
         if (leader) {
@@ -166,6 +167,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const uint32_t as0 = smem_desc_low(smem_u32(smem + kAScaleOffset));
             const uint32_t bs0 = smem_desc_low(smem_u32(smem + kBScaleOffset));
             const uint32_t empty0 = smem_u32(&S.empty[0]);
+            int left = pair == 0 && args.wait.never >= 0 ? args.wait.never : INT_MAX;  // stages until the test's wait
             for (int t = pair; t < num_tiles && ok; t += num_pairs, ++local) {
                 const uint32_t ab = local & 1;
                 // A warp's first piece of a tile read: its part of the tile before is, and the shared columns.
@@ -174,7 +176,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + ab * kSecondAcc;
-                for (int kb = 0; kb < nk; ++kb) {
+                const int stop = min(nk, left);
+                left -= stop;
+                for (int kb = 0; kb < stop; ++kb) {
                     ok = __all_sync(0xffffffffu, guard.wait(&S.full[s], ph, kErrTimeoutFull));
                     if (!ok) break;
                     tc_fence_after();
@@ -211,10 +215,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                         ph ^= 1u;
                     }
                 }
+                if (ok && stop < nk) ok = __all_sync(0xffffffffu, guard.wait(&S.drain, 0u, kErrTimeoutFull));
             }
             if (elect_one()) {
                 mma_commit_pair_local(&S.drain);
-                mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+                mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain, args.wait.ns);
             }
             __syncwarp();
         }
@@ -244,10 +249,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             if (alive) {
                 alive = __all_sync(0xffffffffu, guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum));
             }
-            if (!alive) continue;
             tc_fence_after();
             const int m_warp = m0 + quad * 32;
-            const float a_s = m_warp + lane < args.m ? args.a_scale[m_warp + lane] : 0.0f;
+            // After a wait that gave up every output of the pair is NaN.
+            float a_s = m_warp + lane < args.m ? args.a_scale[m_warp + lane] : 0.0f;
+            if (!alive) a_s = __uint_as_float(0x7fc00000u);
             const f32x2 a_s2 = pk2(a_s, a_s);
 #pragma unroll 1
             for (int i = share; i < kPairCols / kOutCols; i += sharers) {
@@ -312,6 +318,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
 
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) settle_inflight_copies();  // whichever wait gave up
     cluster_sync();
     if (warp == 1) {
         tc_fence_after();

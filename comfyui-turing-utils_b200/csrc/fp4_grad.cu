@@ -21,6 +21,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <climits>
+
 #include "fp4.cuh"
 #include "fp4_mma.cuh"
 #include "ptx.cuh"
@@ -173,7 +175,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = S.tmem_base;
-    const PairAbort guard{&S.abort_flag, mapa_shared(smem_u32(&S.abort_flag), rank ^ 1u), args.err};
+    const PairAbort guard{&S.abort_flag, mapa_shared(smem_u32(&S.abort_flag), rank ^ 1u), args.err, args.wait.ns};
     volatile int *abort_flag = &S.abort_flag;
 
     if (warp == 0) {
@@ -202,7 +204,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                     }
                 }
             }
-            if (!ok || *abort_flag) settle_inflight_copies();
         }
     } else if (warp == 1) {
         if (leader) {
@@ -215,6 +216,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
             const uint32_t a0 = smem_desc_low(smem_u32(smem));
             const uint32_t b0 = ((smem_u32(smem + kBOffset) & 0x3FFFFu) >> 4) | kDescBLow;
             const uint32_t empty0 = smem_u32(&S.empty[0]);
+            int left = pair == 0 && args.wait.never >= 0 ? args.wait.never : INT_MAX;  // stages until the test's wait
             for (int t = pair; t < num_tiles && ok; t += num_pairs, ++local) {
                 int m_tile, n_tile, part, first, last;
                 work_item(t, m_tile, n_tile, part, first, last);
@@ -223,7 +225,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + ab * kGradCols;
-                for (int kb = first; kb < last; ++kb) {
+                const int stop = first + min(last - first, left);
+                left -= stop - first;
+                for (int kb = first; kb < stop; ++kb) {
                     ok = __all_sync(0xffffffffu, guard.wait(&S.full[s], ph, kErrTimeoutFull));
                     if (!ok) break;
                     tc_fence_after();
@@ -243,10 +247,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
                         ph ^= 1u;
                     }
                 }
+                if (ok && stop < last) ok = __all_sync(0xffffffffu, guard.wait(&S.drain, 0u, kErrTimeoutFull));
             }
             if (elect_one()) {
                 mma_commit_pair_local(&S.drain);
-                mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain);
+                mbar_wait(&S.drain, 0u, nullptr, args.err, kErrTimeoutDrain, args.wait.ns);
             }
             __syncwarp();
         }
@@ -260,7 +265,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
         for (int t = pair; t < num_tiles; t += num_pairs, ++local) {
             const int ab = local & 1;
             if (alive) alive = __all_sync(0xffffffffu, guard.wait(&S.acc_full[ab], (local >> 1) & 1, kErrTimeoutAccum));
-            if (!alive) continue;
             tc_fence_after();
             int m_tile, n_tile, part, first, last;
             work_item(t, m_tile, n_tile, part, first, last);
@@ -311,6 +315,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x16(acc + q * 64 + c * 16, r[q]);
                 tmem_ld_wait();
+                if (!alive) {  // after a wait that gave up every output and sum of the pair is NaN
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) r[q][i] = 0x7fc00000u;
+                }
                 if constexpr (kRotate) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) radix4(r[0][i], r[1][i], r[2][i], r[3][i]);
@@ -342,6 +352,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadCount, 1)
 
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) settle_inflight_copies();  // whichever wait gave up
     cluster_sync();
     if (warp == 1) {
         tc_fence_after();

@@ -200,18 +200,19 @@ struct PairAbort {
     volatile int *flag;
     uint32_t peer_flag;
     uint32_t *err;
+    uint64_t limit;  // of a wait, ns
 
     __device__ __forceinline__ void raise() const {
         *flag = 1;
         st_cluster_u32(peer_flag, 1u);
     }
     __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, uint32_t code) const {
-        if (mbar_wait(bar, parity, flag, err, code)) return true;
+        if (mbar_wait(bar, parity, flag, err, code, limit)) return true;
         raise();
         return false;
     }
     __device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, uint32_t code) const {
-        if (mbar_wait_cluster(bar, parity, flag, err, code)) return true;
+        if (mbar_wait_cluster(bar, parity, flag, err, code, limit)) return true;
         raise();
         return false;
     }

@@ -392,7 +392,8 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar_addr, uint32_
 // Bounded wait with cluster-scope acquire (for barriers that receive arrivals or
 // transaction bytes from the peer CTA).
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
-                                                  uint32_t *err, uint32_t code) {
+                                                  uint32_t *err, uint32_t code,
+                                                  uint64_t limit_ns = kWaitLimitNs) {
     const uint32_t addr = smem_u32(bar);
     if (mbar_try_wait_cluster(addr, parity)) return true;
     const uint64_t start = globaltimer();
@@ -400,7 +401,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
         if (mbar_try_wait_cluster(addr, parity)) return true;
         if ((i & 31u) == 0u) {
             if (abort_flag != nullptr && *abort_flag) return false;
-            if (globaltimer() - start > kWaitLimitNs) {
+            if (globaltimer() - start > limit_ns) {
                 if (abort_flag != nullptr) *abort_flag = 1;
                 atomicOr(err, code);
                 return false;

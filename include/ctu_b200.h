@@ -364,11 +364,10 @@ CTU_API int ctu_fp4_linear(const uint8_t *a, const uint8_t *w, const uint8_t *a_
 CTU_API int ctu_debug_set_fp4_kernel(int which);
 
 /*
- * Test hook: in later launches of the few-row FP4 product, the rotating quantizer and the layer norm's backward pass over
- * rows in shared memory, the first CTA's (or team's) wait `which` (0, 1, ...) for a copy is on a
- * barrier that nothing arrives on, and waits give up after limit_ns (at most 5 s).  The kernel must stop cleanly,
- * raise its flags in the device error word and leave no finite result that hangs on that copy.  which < 0: back to
- * normal.
+ * Test hook: in later launches of the FP4 products and gradients, the rotating quantizer and the layer norm's backward
+ * pass over rows in shared memory, wait `which` (0, 1, ...) for a copy in the first CTA (pair, team) is on a barrier that
+ * nothing arrives on, and waits give up after limit_ns (at most 5 s).  The kernel must stop cleanly, raise its flags in
+ * the device error word and leave NaN for every result that hangs on that copy.  which < 0: back to normal.
  */
 CTU_API int ctu_debug_inject_timeout(int which, uint64_t limit_ns);
 

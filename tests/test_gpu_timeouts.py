@@ -148,3 +148,58 @@ def test_layer_norm_backward(k, lib, dtype, rows, hidden, which):
     assert bool(lost[0]) == (which == 0)
     assert torch.isnan(dw).all() and torch.isnan(db).all()
     assert all(torch.equal(p, q) for p, q in zip(call(), whole))
+
+
+# ---------------------------------------------------------------------------- CTA pairs: product and gradient
+def lost_tiles(whole, cut, along_rows):
+    """Numbers of the 256 x 256 tiles that are NaN, counted along rows or down columns; the others have their bits."""
+    (m, n), found = whole.shape, []
+    rows, cols = -(-m // 256), -(-n // 256)
+    for i in range(rows):
+        for j in range(cols):
+            at = (slice(256 * i, 256 * i + 256), slice(256 * j, 256 * j + 256))
+            if torch.isnan(cut[at]).all():
+                found.append(i * cols + j if along_rows else j * rows + i)
+            else:
+                assert torch.equal(cut[at], whole[at])
+    return sorted(found)
+
+
+@pytest.mark.parametrize("fmt", ("nvfp4", "mxfp4"))
+# One tile a pair; several, lost in the second one, with eight epilogue warps, with own stores, and with four warps.
+@pytest.mark.parametrize("m,n,width,which", [(300, 1153, 800, 0), (3850, 3976, 544, 4), (3850, 3973, 544, 3),
+                                             (3850, 3976, 4128, 20)])
+def test_pair_product(k, lib, fmt, m, n, width, which):
+    (a, a_s, a_r), _ = random_operand(k, m, width, fmt, 1)
+    (w, w_s, w_r), _ = random_operand(k, n, width, fmt, 2)
+
+    def call():
+        return k.turing_fp4_linear(a, w, a_s, w_s, a_r, w_r)
+
+    whole = call()
+    with timeout(which):
+        cut = call()
+    lost = lost_tiles(whole, cut, True)
+    if which < -(-width // 256):
+        assert lost == [0]
+    else:  # the first pair's tiles from the second on
+        assert lost and lost[0] >= 60 and lost == [lost[0] * (i + 1) for i in range(len(lost))]
+    assert torch.equal(call(), whole)
+
+
+@pytest.mark.parametrize("fmt", ("nvfp4", "mxfp4"))
+# Every tile split; several whole tiles a pair, lost in the second one; a whole tile and a part of a split one.
+@pytest.mark.parametrize("m,n,width,rotation,which,lost", [(40, 5120, 5120, 256, 2, [0]), (4700, 1000, 4352, 256, 20, [74, 148, 222, 296]),
+                                                           (2450, 5000, 2080, 0, 3, [0, 74])])
+def test_pair_gradient(k, lib, fmt, m, n, width, rotation, which, lost):
+    (w, w_s, w_r), _ = random_operand(k, n, width, fmt, 2)
+    g = torch.randn(m, n, device="cuda", generator=torch.Generator("cuda").manual_seed(m)).bfloat16()
+
+    def call():
+        return k.turing_fp4_linear_grad_input(g, w, w_s, w_r, rotation)
+
+    whole = call()
+    with timeout(which):
+        cut = call()
+    assert lost_tiles(whole, cut, False) == lost
+    assert torch.equal(call(), whole)
