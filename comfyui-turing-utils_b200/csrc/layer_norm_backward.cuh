@@ -330,13 +330,13 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
 template <typename W>
 __global__ void __launch_bounds__(256) team_join_kernel(const AffineArgs a, int slices) {
     __shared__ float part[8][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;  // of 2 * hidden: dw, then db
-    const int total = 2 * a.hidden;
+    // Columns of 2 * hidden, dw's and then db's: more than 31 bits count at the widest row.
+    const int64_t total = 2 * static_cast<int64_t>(a.hidden), c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;
     float s = 0.0f;
     if (c < total) {
         const int first = slices * threadIdx.y / 8, last = slices * (threadIdx.y + 1) / 8;
 #pragma unroll 10
-        for (int i = first; i < last; ++i) s += a.workspace[static_cast<int64_t>(i) * total + c];
+        for (int i = first; i < last; ++i) s += a.workspace[i * total + c];
     }
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
@@ -411,6 +411,8 @@ int staged_smem(int hidden, int bytes, int teams, int depth) {
 }
 }  // namespace
 
+static unsigned join_blocks(int hidden) { return static_cast<unsigned>((2 * static_cast<int64_t>(hidden) + 31) / 32); }
+
 template <typename T>
 cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     const bool aligned = row_aligned(a.x) && row_aligned(a.grad) && row_aligned(a.dx);
@@ -433,7 +435,7 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
             if (params) {
                 parameter_partial_kernel<T>
                     <<<dim3((a.hidden + 31) / 32, slices), dim3(32, 8), 0, stream>>>(a, slices);
-                team_join_kernel<W><<<(2 * a.hidden + 31) / 32, dim3(32, 8), 0, stream>>>(a, slices);
+                team_join_kernel<W><<<join_blocks(a.hidden), dim3(32, 8), 0, stream>>>(a, slices);
             }
             return cudaGetLastError();
         });
@@ -467,7 +469,7 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
     if (e != cudaSuccess || !params) return e;
     return with_weight<T>(a, [&](auto w) {
         team_join_kernel<decltype(w)>
-            <<<(2 * a.hidden + 31) / 32, dim3(32, 8), 0, stream>>>(a, static_cast<int>(grid));
+            <<<join_blocks(a.hidden), dim3(32, 8), 0, stream>>>(a, static_cast<int>(grid));
         return cudaGetLastError();
     });
 }

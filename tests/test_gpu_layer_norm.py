@@ -352,3 +352,22 @@ def test_several_rows_a_team(k, rows, hidden, dtype, wdtype):
         t.requires_grad_(True)
     y = k.turing_layer_norm(x, w, b, EPS)
     check(y.detach(), torch.autograd.grad(y, (x, w, b), dy), x.detach(), w.detach(), b.detach(), dy)
+
+
+def test_widest_row_accepted(k):
+    """One row of 2^30 values: twice the width, which the join of the sums counts to, is beyond 31 bits."""
+    from comfyui_turing_utils_kernel import _lib
+
+    lib, hidden = _lib.load(), 1 << 30
+    x = torch.full((hidden,), 0.5, dtype=torch.bfloat16, device="cuda")
+    x[::2] = -0.5  # mean 0; xhat of one size
+    dy = torch.ones_like(x)
+    dy[-1], dy[0] = 3.0, -2.0
+    mean, rstd = torch.zeros(1, device="cuda"), torch.full((1,), 2.0, device="cuda")
+    dw, db = torch.full_like(x, -77), torch.full_like(x, -77)
+    work = torch.empty(lib.ctu_layer_norm_backward_workspace_bytes(1, hidden), dtype=torch.uint8, device="cuda")
+    _lib.check(lib.ctu_layer_norm_backward(dy.data_ptr(), x.data_ptr(), None, mean.data_ptr(), rstd.data_ptr(), None,
+                                           dw.data_ptr(), db.data_ptr(), work.data_ptr(), 1, hidden, 0, 0,
+                                           torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(db, dy)  # one row: its gradient, exact in every step
+    assert torch.equal(dw, dy * (2 * x))
