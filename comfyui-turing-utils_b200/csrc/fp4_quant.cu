@@ -113,16 +113,17 @@ __device__ __forceinline__ float row_max(float amax, int span, float *red, int g
     return amax;
 }
 
-// t / 6 to nearest (a product with the reciprocal and one correction by its exact remainder, Markstein),
-// for t in the range where the e4m3 rounding that follows can tell.
+// t / 6 to nearest, for t in the range where the e4m3 rounding that follows can tell: a product with the reciprocal,
+// corrected by its exact remainder (Markstein's step, IBM J. Res. Dev. 34(1), 1990).  This, the reciprocal and the
+// quotient below are checked against IEEE division for every significand, and for every scale on the GPU.
 __device__ __forceinline__ float sixth(float t) {
     const float c = 1.0f / 6.0f;
     const float q = __fmul_rn(t, c);
     return __fmaf_rn(__fmaf_rn(q, -6.0f, t), c, q);
 }
 
-// 1 / s of a block scale: the hardware's approximation and one Newton step.  With s of four significant
-// bits the result is the nearest fp32 value.
+// 1 / s of a block scale: the hardware's approximation, within one unit in the last place, and one step of Newton's
+// iteration.  With s of four significant bits the result is the nearest fp32 value.
 __device__ __forceinline__ float scale_reciprocal(float s) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s));
@@ -157,7 +158,7 @@ __device__ __forceinline__ void finish(const QuantArgs &a, const Place &at, floa
         if (kFormat == kNvfp4) {
             byte = __nv_cvt_float_to_fp8(sixth(amax[j] * inv_row), __NV_SATFINITE, __NV_E4M3);
             const float s = block_scale_value(byte, kNvfp4);
-            // v / s rounded to nearest by the same two steps, so that ties of the code grid stay ties.
+            // v / s rounded to nearest by Markstein's step, so that ties of the code grid stay ties.
             // The signs are placed so that a zero keeps its own; a zero scale leaves such zeros.
             const float inv = byte == 0 ? 0.0f : scale_reciprocal(s);
             const f32x2 minus_inv = pk2(-inv, -inv), s2 = pk2(s, s);

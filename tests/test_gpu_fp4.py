@@ -626,3 +626,28 @@ def test_gradient_of_several_items_a_pair(k, fmt, m, n, width, rotation, mixed):
     worst = ((dx.double() - exact).abs() / bound).max().item()
     assert worst <= 1, worst
     assert torch.equal(dx, k.turing_fp4_linear_grad_input(g, w, w_s, w_r, rotation))
+
+
+# ---------------------------------------------------------------------------- every block scale's division
+def test_quantizer_every_block_scale(k):
+    """All 126 positive e4m3 scales as divisors: of bf16 values on and beside every border of the code grid, and of
+    rotated, so fp32, values."""
+    values = oracle.e4m3_values()[1:127]
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)
+    x = torch.zeros(127, 64, dtype=torch.bfloat16)
+    for i, s in enumerate(values):
+        on = (borders * float(s)).bfloat16()  # four bits of scale, three of border: exact
+        off = torch.where(torch.arange(7) % 2 == i % 2, 1, -1).to(torch.int16)
+        beside = (on.view(torch.int16) + off).view(torch.bfloat16)
+        x[i, :16] = torch.cat((torch.tensor([6.0 * s]).bfloat16(), on, beside, -on[:1]))
+        x[i, 63] = 2688.0  # row scale 1
+    _, scales, row = oracle.quantize(x[:126].float().numpy(), "nvfp4", 0)
+    assert (scales[:, 0] == np.arange(1, 127)).all() and (row == 1).all()
+    check_quantized(k, x, "nvfp4", 0)
+    # Groups of 256 columns below the row's largest by up to 2^18, so that their scales are all of them.
+    g = torch.Generator().manual_seed(11)
+    y = torch.randn(400, 20, 256, generator=g) * torch.exp2(-18 * torch.rand(400, 20, 1, generator=g))
+    y = y.view(400, -1).bfloat16()
+    _, scales, _ = oracle.quantize(y.float().numpy(), "nvfp4", 256)
+    assert set(range(1, 127)) <= set(np.unique(scales).tolist())
+    check_quantized(k, y, "nvfp4", 256)
