@@ -477,9 +477,8 @@ int ctu_layer_norm_backward(const void *grad, const void *x, const void *weight,
     a.weight_dtype = weight_dtype;
     a.num_sms = q.num_sms;
     a.err = err;
-    a.wait_ns = wait_limit().ns;
-    a.wait_never = wait_limit().never;
-    CTU_CUDA(ctu::norm::launch_layer_norm_backward(a, static_cast<cudaStream_t>(stream)));
+    const fp4::WaitLimit wait = wait_limit();
+    CTU_CUDA(ctu::norm::launch_layer_norm_backward(a, {wait.ns, wait.never}, static_cast<cudaStream_t>(stream)));
     return CTU_OK;
 }
 

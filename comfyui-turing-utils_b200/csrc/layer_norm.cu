@@ -237,8 +237,8 @@ cudaError_t launch_layer_norm(const AffineArgs &a, cudaStream_t stream) {
 
 int64_t backward_slices(int64_t rows, int64_t) { return std::max<int64_t>(1, std::min<int64_t>(kSlices, rows)); }
 
-cudaError_t launch_layer_norm_backward(const AffineArgs &a, cudaStream_t stream) {
-    return with_type(a.dtype, [&](auto t) { return backward_as<decltype(t)>(a, stream); });
+cudaError_t launch_layer_norm_backward(const AffineArgs &a, const WaitLimit &wait, cudaStream_t stream) {
+    return with_type(a.dtype, [&](auto t) { return backward_as<decltype(t)>(a, wait, stream); });
 }
 
 }  // namespace norm

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kBackwardBlock) team_backward_kernel(const Aff
 // Wide rows through shared memory.  blockDim = (kTeam, teams); dynamic shared memory holds the weights as
 // fp32, then [teams][2 buffers][x, dy] rows, and the teams' sums at the end.
 template <typename T, int kPieces, int kTeam, bool kRagged>
-__global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const AffineArgs a) {
+__global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const AffineArgs a, const WaitLimit wait) {
     constexpr int kVec = 16 / sizeof(T);
     using P = Part<T, kVec, kPieces, kTeam>;
     constexpr int kTeams = kBackwardBlock / kTeam;
@@ -237,8 +237,8 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
             next_mean = a.mean[r + stride];
             next_rstd = a.rstd[r + stride];
         }
-        const bool never = r == first + a.wait_never * stride && blockIdx.x == 0 && team == 0;
-        mbar_wait(never ? &dead : &bars[team][buf], never ? 0u : phase, lost, a.err, kErrTimeoutFull, a.wait_ns);
+        const bool never = r == first + wait.never * stride && blockIdx.x == 0 && team == 0;
+        mbar_wait(never ? &dead : &bars[team][buf], never ? 0u : phase, lost, a.err, kErrTimeoutFull, wait.ns);
         const float start = *lost ? nan : 0.0f;
         const uint8_t *row = rows + buf * 2 * row_bytes;
         f32x2 s = pk2(0.0f, start), t = pk2(0.0f, 0.0f);
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
         if (threadIdx.x == 0) {
             // Copies in flight land before shared memory is used otherwise.
             for (int i = max(0, issued[team] - kDepth); i < issued[team]; ++i)
-                if (!mbar_wait(&bars[team][i & (kDepth - 1)], (kDepth == 2 ? i >> 1 : i) & 1, nullptr, a.err, kErrTimeoutDrain, a.wait_ns))
+                if (!mbar_wait(&bars[team][i & (kDepth - 1)], (kDepth == 2 ? i >> 1 : i) & 1, nullptr, a.err, kErrTimeoutDrain, wait.ns))
                     break;
         }
 #pragma unroll
@@ -414,7 +414,7 @@ int staged_smem(int hidden, int bytes, int teams, int depth) {
 static unsigned join_blocks(int hidden) { return static_cast<unsigned>((2 * static_cast<int64_t>(hidden) + 31) / 32); }
 
 template <typename T>
-cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
+cudaError_t backward_as(const AffineArgs &a, const WaitLimit &wait, cudaStream_t stream) {
     const bool aligned = row_aligned(a.x) && row_aligned(a.grad) && row_aligned(a.dx);
     const bool whole = aligned && a.hidden * static_cast<int64_t>(sizeof(T)) % 16 == 0;
     const bool ragged =
@@ -456,7 +456,7 @@ cudaError_t backward_as(const AffineArgs &a, cudaStream_t stream) {
             const int smem = std::max(sums, staged_smem(a.hidden, sizeof(T), plan.teams, depth));
             auto launch = [&](auto kernel, std::atomic<bool>(&done)[64]) {
                 if (cudaError_t f = allow_smem(kernel, done)) return f;
-                kernel<<<grid, block, smem, stream>>>(a);
+                kernel<<<grid, block, smem, stream>>>(a, wait);
                 return cudaSuccess;
             };
             static std::atomic<bool> done[2][64];

@@ -5,7 +5,7 @@
 namespace ctu {
 namespace norm {
 
-template cudaError_t backward_as<float>(const AffineArgs &, cudaStream_t);
+template cudaError_t backward_as<float>(const AffineArgs &, const WaitLimit &, cudaStream_t);
 
 }  // namespace norm
 }  // namespace ctu
