@@ -134,7 +134,7 @@ int encode_scales(CUtensorMap *map, const void *scales, int64_t rows, int64_t k,
 std::atomic<int> g_fp4_kernel{0};
 
 // The kernel for few rows up to 64 of them, and up to 128 where its strips leave half of the SMs to split
-// K over.  us, it against the pair kernel: 64 x 5120 x 5120 8.8 / 13.1, 64 x 13824 x 5120 14.0 / 13.5,
+// K over.  us with the weights in the L2, it against the pair kernel: 64 x 5120 x 5120 8.8 / 13.1, 64 x 13824 x 5120 14.0 / 13.5,
 // 128 x 5120 x 5120 11.1 / 13.7, 128 x 13824 x 5120 19.4 / 14.3, 128 x 512 x 512 11.0 / 8.2.
 bool few_rows(int64_t m, int64_t n, int64_t k, int num_sms) {
     const int64_t strips = (n + fp4::kStripRows - 1) / fp4::kStripRows;

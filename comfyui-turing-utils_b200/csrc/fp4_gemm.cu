@@ -7,12 +7,16 @@
 // B, the scales of its own A rows and those of all 256 B rows; one M = 256, N = 256, K = 64 instruction of
 // the leader reads both CTAs' halves.
 //
-// What bounds it is the L2: at 32760 x 13824 x 5120 stages of 256 x 128, 256 x 192 and 256 x 256 take the
-// same 600 cycles, 12.6 TB/s of tiles and scales whatever the tile, so the tile is as large as tensor
-// memory allows (951 us with 192 columns and two separate accumulators).  Two accumulators of 256 columns
-// and the scales need 560 of the 512 columns: the second accumulator starts 48 columns before the
-// first one's end, and the epilogue of a tile reads the shared columns first and then lets the next
+// The tile is as large as tensor memory allows: each column more is an operand row read once for more MMAs
+// (32760 x 13824 x 5120: 951 us with 192 columns and two separate accumulators, 891 so).  Two accumulators of
+// 256 columns and the scales need 560 of the 512 columns: the second accumulator starts 48 columns before
+// the first one's end, and the epilogue of a tile reads the shared columns first and then lets the next
 // tile's MMAs start.
+//
+// What bounds it is the tensor pipe and the way from tile to tile.  Four MMAs of a stage take 512 cycles; a stage of 76 KB
+// takes 526 (18944 x 1024 with K = 5120 and 10240), so the scale copies are nearly hidden, and a tile 2500 more
+// whatever its K (with 47 rounds of tiles against four).  16384 x 13824 x 5120 is 667 cycles a stage in all, the
+// pipe 76 % busy, the L2 52 % (14 TB/s).
 //
 // Roles: warp 0 loads (TMA), warp 1 of the leader copies scales into tensor memory and issues the
 // MMAs, warps 2..9 write the output.  Every wait is bounded.
@@ -330,7 +334,7 @@ int linear_pair_smem() { return kSmem; }
 // Eight epilogue warps shorten the way from a tile's last MMA to its output, which is what few tiles wait
 // for (1025 x 1537 x 1568: 12.7 us against 14.8 with four), what short tiles do (13679 x 1856 x 2304: 35 against
 // 39) and what rows off 16 bytes need, which warps write themselves (8894 x 8395 x 1888: 125 against 160).  Four
-// leave more to the MMAs of long tiles that follow one another (32760 x 13824 x 5120: 871 against 899).
+// leave more to the MMAs of long tiles that follow one another (32760 x 13824 x 5120: 3 % less time).
 int linear_pair_threads(bool few_tiles, int64_t n, int64_t k) {
     return few_tiles || n % 8 != 0 || k < 4096 ? kThreadCount : 32 * (2 + 4);
 }

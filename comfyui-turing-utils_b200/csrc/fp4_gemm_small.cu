@@ -8,8 +8,9 @@
 // out the tokens, add the partials in rank order (equal calls give equal bits) and write the output, a
 // warp 256 contiguous bytes of a token.
 //
-// Measured: 1 x 5120 x 5120 6.4 us, 17 x 13824 x 5120 10.9 us; latencies of launch, load, MMA and cluster
-// barriers bound it, not the 2.3 and 5.9 us that the weights' bytes take.
+// Measured: 1 x 5120 x 5120 6.1 us and 17 x 13824 x 5120 10.4 us with the weights in the L2, as in a loop over one
+// layer; 7.6 and 11.7 us with weights from HBM, as a model's layers in turn have them.  Latencies of launch, load, MMA and
+// cluster barriers bound it, not the 2.3 and 5.9 us that the weights' bytes take from HBM.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -31,8 +32,8 @@ constexpr int kScaleBytes = 4 * 512;
 constexpr int kEpilogueWarps = 4;
 constexpr int kThreadCount = 32 * (2 + kEpilogueWarps);
 
-// One CTA an SM with as deep a ring as fits: what bounds a strip is bytes in flight (13824 x 5120, 17
-// tokens: 10.2 us with four stages of 24 KB, two CTAs an SM).
+// One CTA an SM with as deep a ring as fits: what bounds a strip is bytes in flight (1 x 5120 x 5120: 9.3 us with
+// four stages of 24 KB and two CTAs an SM, 6.4 so; 17 x 13824 x 5120 takes as long either way).
 template <int kTokens>
 struct Small {
     static constexpr int kStages = kTokens <= 32 ? 9 : kTokens == 64 ? 8 : 6;

@@ -11,9 +11,11 @@
 // longer row takes several warps, which meet once, for the row's largest magnitude.  Values stay in
 // registers from the load to the codes.
 //
-// Measured: 32760 x 5120 rotated 158 us (16 fp32 operations an element and 15 warps an SM, not HBM, bound
-// it; one row at a time in shared memory 535 us), 4097 x 13824 fp16 unrotated 30 us (5.0 TB/s).  The
-// dequantizer 80 us at 32760 x 5120 (5.4 TB/s; 102 with a division for each eight values).
+// Measured, 32760 x 5120 rotated: nvfp4 157 us, mxfp4 138 (one row at a time in shared memory 535).  No pipe is full:
+// the fp32 pipe is 48 % busy, the issue slots 53 %, DRAM 29 %; the 15 warps that 128 registers leave an SM do not hide
+// the latencies of a chain of 16 fp32 operations an element and the row's barrier.  Unrotated: nvfp4 32760 x 5120 89 us (4.8
+// TB/s), mxfp4 4097 x 13824 fp16 29 us (5.0 TB/s).  The dequantizer 79 us at 32760 x 5120 (5.4 TB/s; 102 with a
+// division for each eight values).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -4,7 +4,7 @@
 //
 // Statistics and sums are fp32 whatever the storage type; each result is rounded once.  Bound by memory:
 // a team of lanes (a warp, or a CTA of several) keeps a row in registers, as loaded, so x is read once;
-// arithmetic is on packed fp32 pairs.  32760 x 5120 bf16: 115 us, 5.84 TB/s (0.90 of a copy's rate); with the
+// arithmetic is on packed fp32 pairs.  32760 x 5120 bf16: 114 us, 5.9 TB/s (0.91 of a copy's rate); with the
 // team's size a launch parameter, so that each access computed its address and bounds, 154 us.  Rows off 16
 // bytes: 32760 x 5121 119 us (with loads of single elements 540 us).  Rows wider than a team holds take the
 // looping kernel.

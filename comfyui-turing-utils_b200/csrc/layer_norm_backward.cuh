@@ -13,9 +13,8 @@
 // start alike within 16 bytes, rows are kept in registers, loaded by single elements; rows wider than a team
 // holds take the looping kernels.
 //
-// Measured: 4096 x 5120 bf16 36 us and 5 for the join (54 us with rows in registers); each further row costs
-// what its bytes take at 5.7 TB/s.  32760 x 5121 204 us (aligned, 5120 wide: 180); 6000 x 13823 fp32 194 us,
-// 5.1 TB/s (looping 486).
+// Measured: 4096 x 5120 bf16 36 us and 5 for the join (54 us with rows in registers); 32760 x 5120 173 us (5.8
+// TB/s), 5121 wide 210; 6000 x 13823 fp32 195 us, 5.1 TB/s (looping 486); one row of 5120 11.7 us, two launches.
 #pragma once
 
 #include "layer_norm_parts.cuh"
@@ -153,7 +152,7 @@ __global__ void __launch_bounds__(kBackwardBlock) staged_backward_kernel(const A
     // Whether a wait of a team gave up (its other waits then do at once), and rows whose copies were issued.
     __shared__ int gave_up[kTeams], issued[kTeams];
     // Of a thread's own element, in shared memory as registers are short (32760 x 5121 bf16: 246 us with them in
-    // registers and rows counted in 64 bits, 204 so): weight, sums of dw and db, and the row's dy * w and xhat.
+    // registers and rows counted in 64 bits, 210 so): weight, sums of dw and db, and the row's dy * w and xhat.
     enum { kOwnW, kOwnDw, kOwnDb, kOwnGw, kOwnN };
     __shared__ float ends[kRagged ? kTeams : 1][5][16];
     extern __shared__ __align__(16) uint8_t smem[];
