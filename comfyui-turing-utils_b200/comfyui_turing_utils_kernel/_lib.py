@@ -118,7 +118,10 @@ def load_torch_ops() -> None:
     path = _LIB_PATH.with_name("libctu_torch.so")
     if not path.exists():
         raise KernelUnavailable(f"{path} is not built; run comfyui-turing-utils_b200/build.py")
-    version = torch_bindings_version(path)
+    try:
+        version = torch_bindings_version(path)
+    except OSError as exc:
+        raise KernelUnavailable(f"{path}: {exc}") from exc
     if version != torch.__version__:
         raise KernelUnavailable(f"{path} is built for torch {version}, not for {torch.__version__}; "
                                 "run comfyui-turing-utils_b200/build.py")

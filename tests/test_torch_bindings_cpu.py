@@ -87,6 +87,13 @@ def test_library_that_does_not_load(package):
     assert len(res.stdout.splitlines()) >= 6 and res.stdout.count(TORCH_LIB.name) >= 6
 
 
+def test_library_that_cannot_be_read(package):
+    (package / TORCH_LIB.name).mkdir()
+    res = run(package.parent)
+    assert res.returncode == 0, res.stderr
+    assert res.stdout.count(TORCH_LIB.name) >= 6
+
+
 def test_library_of_another_torch_is_stale(tmp_path):
     spec = importlib.util.spec_from_file_location("ctu_build", ROOT / "build.py")
     build = importlib.util.module_from_spec(spec)
